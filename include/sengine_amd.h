@@ -47,7 +47,9 @@ extern "C" {
 enum {
   SENGINE_ENC_BITS = 0, /* 1 bit per value, value = bit (binary spikes) */
   SENGINE_ENC_F16 = 1,  /* fp16 NHWC (any fp16 value on input; 0.0 / 1.0 on output) */
-  SENGINE_ENC_F32 = 2   /* fp32 NHWC (pack/unpack and weights only) */
+  SENGINE_ENC_F32 = 2,  /* fp32 NHWC (pack/unpack and weights only) */
+  SENGINE_ENC_BF16 = 3, /* bfloat16 (token operators only) */
+  SENGINE_ENC_E4M3 = 4  /* 8-bit float, OCP e4m3 (token operators only) */
 };
 
 /* Neuron models (sengine/ir.py:44-48 NeuronType, models/neurons.py). */
@@ -475,6 +477,78 @@ int sengine_amd_fused_call_raw_weight(const sengine_conv_lif_desc* d, const void
 int sengine_amd_prepare_weight(const sengine_conv_lif_desc* d, const void* weight, int32_t w_enc, int32_t w_layout,
                                hipStream_t stream);
 int sengine_amd_release_weights(void);
+
+/*
+ * Token operators: what a reader of a token stream (Spikformer's (T*B, N, C) rows, or any
+ * encoder's) is made of.  Rows of tokens are strided: `*_stride` counts elements, the values of
+ * a row lie side by side.  Type fields hold SENGINE_ENC_F16 / _BF16 / _F32 / _E4M3.
+ */
+
+/*
+ * Root-mean-square norm with the residual's addition.  Per row: s = x + residual (or x), y =
+ * s / sqrt(mean(s^2) + eps) * weight (1 where null).  stream_out (or null) receives s and out
+ * receives y, both in x's type; with out_type = SENGINE_ENC_E4M3 out receives y / c as e4m3 and
+ * scale[row] = c = max|y| / 448 (1 for a row of zeros).  Everything before a store is fp32; y is
+ * formed from the unrounded s.  residual and stream_out are of x's type, weight of x's type or
+ * fp32.  1 <= D <= 32768, rows < 2^31; an output may be the input it has the rows of.
+ */
+typedef struct sengine_rms_norm_desc {
+  int64_t rows;
+  int64_t x_stride, residual_stride, out_stride, stream_stride;
+  int32_t D;
+  int32_t in_type, weight_type, out_type;
+  float eps;
+} sengine_rms_norm_desc;
+int sengine_amd_rms_norm(const sengine_rms_norm_desc* d, const void* x, const void* residual, const void* weight,
+                         void* out, void* stream_out, float* scale, hipStream_t stream);
+
+/* Activations of sengine_amd_linear.  GELU: z * Phi(z) by the error function; GELU_TANH: its tanh
+ * form; SILU: z * sigmoid(z). */
+enum {
+  SENGINE_ACT_NONE = 0,
+  SENGINE_ACT_RELU = 1,
+  SENGINE_ACT_GELU = 2,
+  SENGINE_ACT_GELU_TANH = 3,
+  SENGINE_ACT_SILU = 4
+};
+
+/*
+ * out[m, n] = act(x_scale[m] * weight_scale[n] * sum_k x[m, k] weight[n, k] + bias[n]) +
+ * residual[m, n].  x (M, K) and weight (N, K; nn.Linear's layout) are both fp16, both bf16 or both
+ * e4m3; the scales (fp32, null = 1) go with e4m3.  out and residual have out_type (fp16, bf16 or
+ * fp32), bias has bias_type (one of the same); bias and residual may be null.  The sum and the
+ * epilogue are fp32, out is rounded once.  (The 8-bit matrix instructions keep about 16 bits of a
+ * sum; e4m3 operands with an fp32 output are multiplied as fp16 instead, at half the rate.)  out may
+ * be residual itself.
+ */
+typedef struct sengine_linear_desc {
+  int64_t M;
+  int64_t x_stride, weight_stride, residual_stride, out_stride;
+  int32_t N, K;
+  int32_t in_type, out_type, bias_type, activation;
+} sengine_linear_desc;
+int sengine_amd_linear(const sengine_linear_desc* d, const void* x, const void* weight, const float* x_scale,
+                       const float* weight_scale, const void* bias, const void* residual, void* out,
+                       hipStream_t stream);
+
+/*
+ * Cross attention of q (B, Lq, Hq, d) to encoder states k, v (B, Lk, Hkv, d): out[b, i, h] =
+ * softmax_j(scale * q[b, i, h] . k[b, j, g]) v[b, j, g], g = h / (Hq / Hkv), over the keys that
+ * count: j < key_lengths[b] (int32, clamped to 0..Lk; null = Lk) and key_mask[b * mask_stride + j]
+ * != 0 (bytes; null = all).  A query with no key gets zeros; a key or value that does not count is
+ * never used, whatever it holds.  q, k, v and out are fp16 or bf16 with strides per (batch, row,
+ * head) in elements and the d values of a head side by side; d is a multiple of 8 up to 128.  A
+ * batch stride of 0 shares the encoder's states between the sequences.
+ */
+typedef struct sengine_cross_desc {
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  int64_t mask_stride;
+  int32_t B, Lq, Lk, Hq, Hkv, d;
+  int32_t type;
+  float scale;
+} sengine_cross_desc;
+int sengine_amd_cross_attention(const sengine_cross_desc* d, const void* q, const void* k, const void* v,
+                                const int32_t* key_lengths, const void* key_mask, void* out, hipStream_t stream);
 
 /*
  * Peak calibration on the box (the role of the reference's sengine/tuning/hw_calibrate.py:

@@ -10,7 +10,8 @@ import threading
 
 from .build import LIB_PATH
 
-ENC_BITS, ENC_F16, ENC_F32 = 0, 1, 2
+ENC_BITS, ENC_F16, ENC_F32, ENC_BF16, ENC_E4M3 = 0, 1, 2, 3, 4
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 NEURON_LIF, NEURON_IF, NEURON_MS = 0, 1, 2
 WLAYOUT_OIHW, WLAYOUT_HWIO = 0, 1
 
@@ -31,10 +32,44 @@ class ConvLifDesc(ctypes.Structure):
     ]
 
 
+class RmsNormDesc(ctypes.Structure):
+    """Mirror of ``sengine_rms_norm_desc``."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64), ("stream_stride", ctypes.c_int64), ("D", ctypes.c_int32),
+        ("in_type", ctypes.c_int32), ("weight_type", ctypes.c_int32), ("out_type", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class LinearDesc(ctypes.Structure):
+    """Mirror of ``sengine_linear_desc``."""
+
+    _fields_ = [
+        ("M", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("weight_stride", ctypes.c_int64),
+        ("residual_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("N", ctypes.c_int32),
+        ("K", ctypes.c_int32), ("in_type", ctypes.c_int32), ("out_type", ctypes.c_int32),
+        ("bias_type", ctypes.c_int32), ("activation", ctypes.c_int32),
+    ]
+
+
+class CrossDesc(ctypes.Structure):
+    """Mirror of ``sengine_cross_desc``."""
+
+    _fields_ = [
+        ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+        ("out_stride", ctypes.c_int64 * 3), ("mask_stride", ctypes.c_int64), ("B", ctypes.c_int32),
+        ("Lq", ctypes.c_int32), ("Lk", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hkv", ctypes.c_int32),
+        ("d", ctypes.c_int32), ("type", ctypes.c_int32), ("scale", ctypes.c_float),
+    ]
+
+
 _P = ctypes.c_void_p
 _DP = ctypes.POINTER(ConvLifDesc)
 _I32, _I64, _F = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 _SZP = ctypes.POINTER(ctypes.c_size_t)
+_NDP, _LDP, _CDP = ctypes.POINTER(RmsNormDesc), ctypes.POINTER(LinearDesc), ctypes.POINTER(CrossDesc)
 
 # name -> (restype, argtypes); every symbol declared in include/sengine_amd.h
 SIGNATURES = {
@@ -83,6 +118,9 @@ SIGNATURES = {
     "sengine_amd_sew_head_ws": (ctypes.c_int, [_I32, _I32, _I32, _I32, _I32, _P, _P, _P, _I32, _P, _P, _I64, _P]),
     "sengine_amd_dense_conv_bn": (ctypes.c_int, [_DP, _P, _P, _P, _P, _P, _P]),
     "sengine_amd_multistep_neuron": (ctypes.c_int, [_I32, _I64, _I32, _I32, _F, _F, _F, _P, _P, _I32, _P, _P, _P]),
+    "sengine_amd_rms_norm": (ctypes.c_int, [_NDP, _P, _P, _P, _P, _P, _P, _P]),
+    "sengine_amd_linear": (ctypes.c_int, [_LDP, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "sengine_amd_cross_attention": (ctypes.c_int, [_CDP, _P, _P, _P, _P, _P, _P, _P]),
     "sengine_amd_pack_spikes": (ctypes.c_int, [_P, _I32, _I64, _I32, _P, _P]),
     "sengine_amd_unpack_spikes": (ctypes.c_int, [_P, _I64, _I32, _P, _I32, _P]),
 }

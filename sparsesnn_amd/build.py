@@ -24,7 +24,7 @@ ARCH = "gfx950"
 
 SOURCES = ["capi.hip", "fused_sparse.hip", "fused_sparse_lds.hip", "fused_tile1.hip", "fused_tile1ds.hip",
            "fused_tile3.hip", "fused_tile3s.hip", "compress.hip", "fallback.hip", "sew.hip", "ssa.hip", "msres.hip",
-           "calib.hip", "weights.hip"]
+           "calib.hip", "weights.hip", "rms_norm.hip", "linear.hip", "cross_attention.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",

@@ -8,6 +8,7 @@ pointers and cannot check buffer sizes itself).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 from dataclasses import dataclass, replace
@@ -16,8 +17,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import (ENC_BITS, ENC_F16, ENC_F32, NEURON_IF, NEURON_LIF, NEURON_MS, WLAYOUT_HWIO, WLAYOUT_OIHW,
-                   ConvLifDesc, SEngineError, check)
+from ._lib import (ACTIVATIONS, ENC_BF16, ENC_BITS, ENC_E4M3, ENC_F16, ENC_F32, NEURON_IF, NEURON_LIF, NEURON_MS, WLAYOUT_HWIO, WLAYOUT_OIHW,
+                   ConvLifDesc, CrossDesc, LinearDesc, RmsNormDesc, SEngineError, check)
 
 __all__ = [
     "ConvSpec", "make_desc", "geometry", "set_fused_kernel", "compress_2_4", "pack_dense_weights", "pack_spikes",
@@ -26,7 +27,7 @@ __all__ = [
     "ENC_BITS", "ENC_F16", "ENC_F32", "NEURON_LIF", "NEURON_IF", "NEURON_MS", "WLAYOUT_OIHW", "WLAYOUT_HWIO",
     "neuron_code", "fused_sparse_conv_bn_add_neuron", "spiking_self_attention", "stem_conv_bn_neuron",
     "fused_sparse_conv_bn_lif_pair", "fused_sparse_conv_bn_lif_split", "fused_sparse_conv_bn_lif_tail", "tail_eligible",
-    "fused_plan",
+    "fused_plan", "rms_norm", "linear", "cross_attention", "ENC_BF16", "ENC_E4M3",
 ]
 
 
@@ -849,4 +850,255 @@ def multistep_neuron(x: torch.Tensor, T: int, neuron: str = "lif", tau: float = 
     check(lib.sengine_amd_multistep_neuron(T, n, neuron_code(neuron), int(hard), float(tau),
                                            float(v_threshold), float(v_reset if hard else 0.0), _ptr(x), _ptr(state),
                                            out_enc, _ptr(out), _ptr(h_trace), _stream(x.device)), "multistep_neuron")
+    return out
+
+
+# ------------------------------------------------------------------ token operators
+
+_TOKEN_TYPES = {torch.float16: ENC_F16, torch.bfloat16: ENC_BF16, torch.float32: ENC_F32,
+                torch.float8_e4m3fn: ENC_E4M3}
+
+
+def _type_code(t: torch.Tensor, allowed, name: str) -> int:
+    if t.dtype not in allowed:
+        raise SEngineError(f"{name}: expected dtype {' or '.join(str(d) for d in allowed)}, got {t.dtype}")
+    return _TOKEN_TYPES[t.dtype]
+
+
+def _token_input(t, name: str, device=None):
+    """A tensor that a token operator reads: on the device, and not one that asks for a gradient
+    (these operators have no backward; it is refused rather than cut off)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise SEngineError(f"{name} must be on a HIP device (got {t.device})")
+    if device is not None and t.device != device:
+        raise SEngineError(f"{name} is on {t.device}, the others on {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise SEngineError(f"{name} requires a gradient: the token operators are inference only "
+                           "(call them under torch.no_grad())")
+
+
+def _token_rows(t: torch.Tensor, name: str):
+    """(rows, row stride in elements) of (..., width), whose rows must lie evenly spaced."""
+    if t.is_contiguous():
+        return (t.numel() // t.shape[-1] if t.shape[-1] else math.prod(t.shape[:-1])), t.shape[-1]
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise SEngineError(f"{name}: the values of a row must lie side by side")
+    dims = [(n, st) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    for (_, outer), (n, inner) in zip(dims, dims[1:]):
+        if outer != n * inner:
+            raise SEngineError(f"{name}: the rows must be evenly spaced (shape {tuple(t.shape)}, "
+                               f"strides {t.stride()})")
+    return math.prod(t.shape[:-1]), dims[-1][1] if dims else t.shape[-1]
+
+
+def _token_vector(t, n: int, name: str, device):
+    _token_input(t, name, device)
+    if t.numel() != n or not t.is_contiguous():
+        raise SEngineError(f"{name}: expected {n} contiguous elements, got shape {tuple(t.shape)}")
+
+
+def _token_out(t, shape, dtype, name: str, device):
+    """An output given by the caller; returns its row stride."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device != device:
+        raise SEngineError(f"{name} is on {t.device}, the input on {device}")
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise SEngineError(f"{name}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise SEngineError(f"{name} requires a gradient: the token operators are inference only")
+    return _token_rows(t, name)[1]
+
+
+@functools.lru_cache(maxsize=1024)
+def _rms_norm_desc(*fields):
+    return ctypes.byref(RmsNormDesc(*fields))
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+             eps: float = 1e-6, out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
+             stream_out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
+    """Root-mean-square norm of rows x (..., D) with the residual's addition: s = x + residual,
+    y = s / sqrt(mean(s^2) + eps) * weight, in fp32, y formed from the unrounded s.
+
+    x is fp16, bf16 or fp32; residual and stream have its shape and type; weight (D,) its type or
+    fp32.  Returns (y, stream) with y in x's type, or with out_dtype=torch.float8_e4m3fn
+    (y, stream, scale): y's codes and one fp32 scale a row (shape x.shape[:-1]), y ~ codes * scale.
+    stream is s rounded to x's type, None without a residual.  `out`, `stream_out` (which may be
+    `residual`, updated in place) and `scale` take the results where given."""
+    _token_input(x, "x")
+    dev, code = x.device, _type_code(x, (torch.float16, torch.bfloat16, torch.float32), "x")
+    if x.dim() == 0:
+        raise SEngineError("x: expected (..., D)")
+    shape, D = x.shape, x.shape[-1]
+    rows, xs = _token_rows(x, "x")
+    rs = ws = 0
+    if residual is not None:
+        _token_input(residual, "residual", dev)
+        if residual.shape != shape or residual.dtype != x.dtype:
+            raise SEngineError(f"residual: expected {x.dtype} {tuple(shape)}, got {residual.dtype} "
+                               f"{tuple(residual.shape)}")
+        rs = _token_rows(residual, "residual")[1]
+    elif stream_out is not None:
+        raise SEngineError("stream_out: there is no residual to add")
+    if weight is not None:
+        _token_vector(weight, D, "weight", dev)
+        ws = _type_code(weight, (x.dtype, torch.float32), "weight")
+    eight = out_dtype is torch.float8_e4m3fn
+    if out_dtype is None:
+        out_dtype = x.dtype
+    elif out_dtype is not x.dtype and not eight:
+        raise SEngineError(f"out_dtype: expected {x.dtype} or torch.float8_e4m3fn, got {out_dtype}")
+    if out is None:
+        out, os_ = torch.empty(shape, dtype=out_dtype, device=dev), D
+    else:
+        os_ = _token_out(out, shape, out_dtype, "out", dev)
+    ss = D
+    if residual is not None:
+        if stream_out is None:
+            stream_out = torch.empty(shape, dtype=x.dtype, device=dev)
+        else:
+            ss = _token_out(stream_out, shape, x.dtype, "stream_out", dev)
+    if eight:
+        if scale is None:
+            scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+        else:
+            _token_vector(scale, rows, "scale", dev)
+            _type_code(scale, (torch.float32,), "scale")
+    elif scale is not None:
+        raise SEngineError("scale goes with out_dtype=torch.float8_e4m3fn")
+    check(_lib.load().sengine_amd_rms_norm(
+        _rms_norm_desc(rows, xs, rs, os_, ss, D, code, ws, _TOKEN_TYPES[out_dtype], eps), x.data_ptr(),
+        _ptr(residual), _ptr(weight), out.data_ptr(), _ptr(stream_out), _ptr(scale), _stream(dev)), "rms_norm")
+    return (out, stream_out, scale) if eight else (out, stream_out)
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_desc(*fields):
+    return ctypes.byref(LinearDesc(*fields))
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+           residual: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None,
+           weight_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x weight^T + bias) + residual of token rows x (..., K) with weight (N, K), nn.Linear's
+    layout; activation 'none' | 'relu' | 'gelu' (by the error function) | 'gelu_tanh' | 'silu'.
+
+    x and weight are both fp16, both bf16, or both float8_e4m3fn with fp32 scales of x's rows
+    (x_scale, as rms_norm returns it) and of weight's rows (weight_scale, (N,)).  The sums and what
+    follows them are fp32 (the 8-bit matrix instructions keep about 16 bits of a sum, which a 16-bit
+    result hides; an fp32 result of e4m3 operands takes the 16-bit ones at half the rate); the result is rounded once to out_dtype (fp16, bf16 or fp32; x's type,
+    for e4m3 bf16, by default).  residual (..., N) has out_dtype, bias (N,) fp16, bf16 or fp32;
+    `out` may be `residual`."""
+    _token_input(x, "x")
+    dev = x.device
+    code = _type_code(x, (torch.float16, torch.bfloat16, torch.float8_e4m3fn), "x")
+    _token_input(weight, "weight", dev)
+    if x.dim() == 0 or weight.dim() != 2 or weight.dtype != x.dtype or weight.shape[1] != x.shape[-1]:
+        raise SEngineError(f"weight: expected {x.dtype} (N, K) for x {tuple(x.shape)}, got {weight.dtype} "
+                           f"{tuple(weight.shape)}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    N, K = weight.shape
+    M, xs = _token_rows(x, "x")
+    wst = _token_rows(weight, "weight")[1]
+    eight = code == ENC_E4M3
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if eight else x.dtype
+    ocode = _TOKEN_TYPES.get(out_dtype, ENC_E4M3)
+    if ocode == ENC_E4M3:
+        raise SEngineError(f"out_dtype: expected float16, bfloat16 or float32, got {out_dtype}")
+    for t, n, name in ((x_scale, M, "x_scale"), (weight_scale, N, "weight_scale")):
+        if t is not None:
+            if not eight:
+                raise SEngineError(f"{name} goes with float8_e4m3fn operands")
+            _token_vector(t, n, name, dev)
+            _type_code(t, (torch.float32,), name)
+    bcode = 0
+    if bias is not None:
+        _token_vector(bias, N, "bias", dev)
+        bcode = _type_code(bias, (torch.float16, torch.bfloat16, torch.float32), "bias")
+    shape = (*x.shape[:-1], N)
+    rs = 0
+    if residual is not None:
+        _token_input(residual, "residual", dev)
+        if residual.shape != shape or residual.dtype != out_dtype:
+            raise SEngineError(f"residual: expected {out_dtype} {shape}, got {residual.dtype} "
+                               f"{tuple(residual.shape)}")
+        rs = _token_rows(residual, "residual")[1]
+    if out is None:
+        out, os_ = torch.empty(shape, dtype=out_dtype, device=dev), N
+    else:
+        os_ = _token_out(out, shape, out_dtype, "out", dev)
+    check(_lib.load().sengine_amd_linear(
+        _linear_desc(M, xs, wst, rs, os_, N, K, code, ocode, bcode, ACTIVATIONS[activation]), x.data_ptr(),
+        weight.data_ptr(), _ptr(x_scale), _ptr(weight_scale), _ptr(bias), _ptr(residual), out.data_ptr(),
+        _stream(dev)), "linear")
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _cross_desc(qs, ks, vs, os_, *fields):
+    s3 = ctypes.c_int64 * 3
+    return ctypes.byref(CrossDesc(s3(*qs[:3]), s3(*ks[:3]), s3(*vs[:3]), s3(*os_[:3]), *fields))
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float] = None,
+                    key_lengths: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q (B, Lq, Hq, d) to an encoder's states k, v (B, Lk, Hkv, d), Hq a multiple of
+    Hkv (query head h reads key head h // (Hq // Hkv)), d a multiple of 8 up to 128; fp16 or bf16;
+    scale 1 / sqrt(d) by default.  Returns (B, Lq, Hq, d) in q's type.
+
+    key_lengths (B,) int32: the keys of each sequence that count (clamped to 0..Lk); key_mask
+    (B, Lk) bool: True where a key counts.  A query with no key that counts gets zeros; what lies
+    in the others is never used.  Any strides whose rows of d values are contiguous and begin at
+    multiples of 16 bytes; k and v expanded over the batch (one encoder pass, many queries) are read
+    as they are."""
+    _token_input(q, "q")
+    dev, code = q.device, _type_code(q, (torch.float16, torch.bfloat16), "q")
+    for t, name in ((k, "k"), (v, "v")):
+        _token_input(t, name, dev)
+        if t.dtype != q.dtype:
+            raise SEngineError(f"{name}: expected {q.dtype}, got {t.dtype}")
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise SEngineError(f"cross_attention: expected q (B, Lq, Hq, d) and k, v (B, Lk, Hkv, d), got "
+                           f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, Lq, Hq, d = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    if out is None:
+        out = torch.empty((B, Lq, Hq, d), dtype=q.dtype, device=dev)
+    else:
+        if not isinstance(out, torch.Tensor):
+            raise TypeError("out must be a torch.Tensor")
+        if out.device != dev or out.dtype != q.dtype or out.shape != q.shape:
+            raise SEngineError(f"out: expected {q.dtype} {tuple(q.shape)} on {dev}, got {out.dtype} "
+                               f"{tuple(out.shape)} on {out.device}")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise SEngineError("out requires a gradient: the token operators are inference only")
+    st = [t.stride() for t in (q, k, v, out)]
+    for t, s, name in zip((q, k, v, out), st, ("q", "k", "v", "out")):
+        if (s[3] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and s[2] % 8 == 0 and t.data_ptr() % 16 == 0) or not t.numel():
+            continue
+        if s[3] != 1 or t.data_ptr() % 16 or any(n > 1 and x % 8 for n, x in zip(t.shape, s[:3])):
+            raise SEngineError(f"{name}: rows of d values must be contiguous and begin at multiples of 16 bytes "
+                               f"(strides {s})")
+    if key_lengths is not None:
+        _token_vector(key_lengths, B, "key_lengths", dev)
+        if key_lengths.dtype != torch.int32:
+            raise SEngineError(f"key_lengths: expected dtype torch.int32, got {key_lengths.dtype}")
+    ms = 0
+    if key_mask is not None:
+        _token_input(key_mask, "key_mask", dev)
+        if key_mask.dtype != torch.bool or key_mask.shape != (B, Lk) or (Lk > 1 and key_mask.stride(1) != 1):
+            raise SEngineError(f"key_mask: expected torch.bool ({B}, {Lk}) with contiguous rows, got "
+                               f"{key_mask.dtype} {tuple(key_mask.shape)}")
+        ms = key_mask.stride(0)
+    check(_lib.load().sengine_amd_cross_attention(
+        _cross_desc(*st, ms, B, Lq, Lk, Hq, Hkv, d, code, 1.0 / math.sqrt(d) if scale is None else scale),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths), _ptr(key_mask), out.data_ptr(),
+        _stream(dev)), "cross_attention")
     return out

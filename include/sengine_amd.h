@@ -530,6 +530,15 @@ typedef struct sengine_linear_desc {
 int sengine_amd_linear(const sengine_linear_desc* d, const void* x, const void* weight, const float* x_scale,
                        const float* weight_scale, const void* bias, const void* residual, void* out,
                        hipStream_t stream);
+/*
+ * The same with scratch memory (16-byte aligned, of at least sengine_amd_linear_workspace's bytes; what it holds
+ * before does not matter): few output tiles of a long reduction are then computed in parts, by more workgroups,
+ * and joined in a fixed order.  Without it, or with less, one workgroup computes a tile.
+ */
+int sengine_amd_linear_workspace(const sengine_linear_desc* d, size_t* bytes);
+int sengine_amd_linear_ws(const sengine_linear_desc* d, const void* x, const void* weight, const float* x_scale,
+                          const float* weight_scale, const void* bias, const void* residual, void* out,
+                          void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /*
  * Cross attention of q (B, Lq, Hq, d) to encoder states k, v (B, Lk, Hkv, d): out[b, i, h] =

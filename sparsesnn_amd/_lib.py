@@ -120,6 +120,8 @@ SIGNATURES = {
     "sengine_amd_multistep_neuron": (ctypes.c_int, [_I32, _I64, _I32, _I32, _F, _F, _F, _P, _P, _I32, _P, _P, _P]),
     "sengine_amd_rms_norm": (ctypes.c_int, [_NDP, _P, _P, _P, _P, _P, _P, _P]),
     "sengine_amd_linear": (ctypes.c_int, [_LDP, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "sengine_amd_linear_workspace": (ctypes.c_int, [_LDP, _SZP]),
+    "sengine_amd_linear_ws": (ctypes.c_int, [_LDP, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "sengine_amd_cross_attention": (ctypes.c_int, [_CDP, _P, _P, _P, _P, _P, _P, _P]),
     "sengine_amd_pack_spikes": (ctypes.c_int, [_P, _I32, _I64, _I32, _P, _P]),
     "sengine_amd_unpack_spikes": (ctypes.c_int, [_P, _I64, _I32, _P, _I32, _P]),

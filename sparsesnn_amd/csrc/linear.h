@@ -16,85 +16,218 @@ struct LinearParams {
   int N, K;
   int kbytes;            // K in bytes
   int act, out_type, bias_type;
-  int vec;               // out and res rows begin at multiples of four elements
+  float* partial;        // sums of the reduction's parts (linear_tile.h), or null
+  int part_steps;        // 128-byte steps a part
+  int vec;               // N is a multiple of 8, out and res rows begin at multiples of 16 bytes
 };
 
-// gelu(z) = z * Phi(z), Phi by erf; gelu_tanh(z) = z * sigmoid(2 sqrt(2/pi) (z + 0.044715 z^3)),
-// which is the tanh form rewritten; silu(z) = z * sigmoid(z).
-__device__ __forceinline__ float activate(float z, int act) {
-  switch (act) {
-    case SENGINE_ACT_RELU:
-      return z < 0.f ? 0.f : z;  // a NaN stays
-    case SENGINE_ACT_GELU:
-      return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case SENGINE_ACT_GELU_TANH: {
-      const float u = 1.5957691216057308f * (z + 0.044715f * z * z * z);
-      return z / (1.f + __expf(-u));
-    }
-    case SENGINE_ACT_SILU:
-      return z / (1.f + __expf(-z));
-    default:
-      return z;
+template <int V>
+struct Int {
+  static constexpr int value = V;
+};
+
+// z * sigmoid(t), t given as u = t / ln 2: z / (1 + 2^-u).
+__device__ __forceinline__ float times_sigmoid2(float z, float u) {
+  return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-u));
+}
+
+// gelu(z) = z * Phi(z), written as z * sigmoid(z * P(z^2)): P is the logit of Phi over z, an even
+// function, as a polynomial of degree 6 in z^2 (weighted least squares towards the least largest error
+// over |z| <= 6, in base 2).  Phi is off by at most 2.7 units of 2^-24, and P keeps growing beyond.
+// Ten full-rate operations, an exponential and a reciprocal.
+// gelu_tanh(z) = z * sigmoid(2 sqrt(2/pi) (z + 0.044715 z^3)), the tanh form rewritten;
+// silu(z) = z * sigmoid(z).
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (ACT == SENGINE_ACT_RELU) {
+    return z < 0.f ? 0.f : z;  // a NaN stays
+  } else if constexpr (ACT == SENGINE_ACT_GELU) {
+    const float t = z * z;
+    float p = 5.067260833158116e-09f;
+    p = __builtin_fmaf(p, t, -3.816321054728178e-07f);
+    p = __builtin_fmaf(p, t, 1.1439842637628317e-05f);
+    p = __builtin_fmaf(p, t, -0.00015957998402882367f);
+    p = __builtin_fmaf(p, t, -9.404912998434156e-05f);
+    p = __builtin_fmaf(p, t, 0.10483512282371521f);
+    p = __builtin_fmaf(p, t, 2.3022093772888184f);
+    return times_sigmoid2(z, z * p);
+  } else if constexpr (ACT == SENGINE_ACT_GELU_TANH) {
+    // 2 sqrt(2/pi) / ln 2 and 0.044715 times it
+    return times_sigmoid2(z, z * __builtin_fmaf(z * z, 0.10294324f, 2.3022082f));
+  } else if constexpr (ACT == SENGINE_ACT_SILU) {
+    return times_sigmoid2(z, z * 1.4426950408889634f);
+  } else {
+    return z;
   }
 }
 
-// Four consecutive output columns n..n+3 of row m, from the fp32 sums of the reduction: scales,
-// bias, activation and residual in fp32, one rounding at the store.
-__device__ __forceinline__ void linear_store4(const LinearParams& p, int64_t m, int n, float4_t acc) {
-  if (m >= p.M || n >= p.N) return;
-  float v[4];
-  const int cnt = p.N - n < 4 ? p.N - n : 4;
-  const float sx = p.x_scale ? p.x_scale[m] : 1.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] = acc[i];
-    const int c = i < cnt ? n + i : n;
-    if (p.x_scale) v[i] *= sx;
-    if (p.w_scale) v[i] *= p.w_scale[c];
-    if (p.bias) v[i] += load_as_float(p.bias, p.bias_type, c);
-    v[i] = activate(v[i], p.act);
+// f(Int<ACT>) for the run-time activation.
+template <class F>
+__device__ __forceinline__ void by_activation(int act, F f) {
+  switch (act) {
+    case SENGINE_ACT_RELU:
+      f(Int<SENGINE_ACT_RELU>{});
+      break;
+    case SENGINE_ACT_GELU:
+      f(Int<SENGINE_ACT_GELU>{});
+      break;
+    case SENGINE_ACT_GELU_TANH:
+      f(Int<SENGINE_ACT_GELU_TANH>{});
+      break;
+    case SENGINE_ACT_SILU:
+      f(Int<SENGINE_ACT_SILU>{});
+      break;
+    default:
+      f(Int<SENGINE_ACT_NONE>{});
+      break;
   }
-  const int64_t o = m * p.out_stride + n, r = m * p.res_stride + n;
-  if (p.vec && cnt == 4) {
-    if (p.out_type == SENGINE_ENC_F32) {
-      if (p.res) {
-        float t[4];
-        load_floats<float, 4>(static_cast<const float*>(p.res) + r, t);
+}
+
+// NV neighbouring values of type O as they lie in memory.
+template <class O, int NV>
+struct Raw {
+  typedef O vec_t __attribute__((ext_vector_type(NV), aligned(NV * sizeof(O) < 16 ? NV * sizeof(O) : 16)));
+  vec_t v;
+};
+
+// NV columns from n on of NR rows m, m + STEP, ... of the residual.  They are not used before linear_finish, so
+// that all rows' loads are in flight together.  VEC: N is a multiple of 8 and the rows of out and residual begin at
+// multiples of 16 bytes; otherwise values are read and stored one by one.
+template <class O, bool VEC, int NR, int STEP, int NV>
+__device__ __forceinline__ void linear_residual(const LinearParams& p, int64_t m, int n, Raw<O, NV> (&r)[NR]) {
+  if (!p.res || n >= p.N) return;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += t[i];
-      }
-      store_floats<float, 4>(static_cast<float*>(p.out) + o, v);
-    } else if (p.out_type == SENGINE_ENC_F16) {
-      if (p.res) {
-        float t[4];
-        load_floats<_Float16, 4>(static_cast<const _Float16*>(p.res) + r, t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += t[i];
-      }
-      store_floats<_Float16, 4>(static_cast<_Float16*>(p.out) + o, v);
+  for (int u = 0; u < NR; ++u) {
+    const int64_t row = m + STEP * u < p.M ? m + STEP * u : p.M - 1;
+    const O* at = static_cast<const O*>(p.res) + row * p.res_stride + n;
+    if constexpr (VEC) {
+      r[u].v = *reinterpret_cast<const typename Raw<O, NV>::vec_t*>(at);
     } else {
-      if (p.res) {
-        float t[4];
-        load_floats<__bf16, 4>(static_cast<const __bf16*>(p.res) + r, t);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += t[i];
-      }
-      store_floats<__bf16, 4>(static_cast<__bf16*>(p.out) + o, v);
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i < cnt) {
-      if (p.res) v[i] += load_as_float(p.res, p.out_type, r + i);
-      if (p.out_type == SENGINE_ENC_F32)
-        static_cast<float*>(p.out)[o + i] = v[i];
-      else if (p.out_type == SENGINE_ENC_F16)
-        static_cast<_Float16*>(p.out)[o + i] = (_Float16)v[i];
-      else
-        static_cast<__bf16*>(p.out)[o + i] = (__bf16)v[i];
+      for (int e = 0; e < NV; ++e)
+        if (n + e < p.N) r[u].v[e] = at[e];
     }
   }
+}
+
+// The columns' coefficients; only 8-bit operands have scales.
+template <class T, int NV>
+struct Columns {
+  static constexpr bool kScaled = sizeof(T) == 1;
+  float w[kScaled ? NV : 1], bias[NV];
+  __device__ __forceinline__ Columns(const LinearParams& p, int n) {
+#pragma unroll
+    for (int e = 0; e < NV; ++e) {
+      const int at = n + e < p.N ? n + e : p.N - 1;
+      if constexpr (kScaled) w[e] = p.w_scale ? p.w_scale[at] : 1.f;
+      bias[e] = p.bias ? load_as_float(p.bias, p.bias_type, at) : 0.f;
+    }
+  }
+};
+
+// The same rows and columns finished from their sums: scales, bias, activation and residual in fp32, one rounding.
+template <class T, class O, bool VEC, int NR, int STEP, int NV>
+__device__ __forceinline__ void linear_finish(const LinearParams& p, int64_t m, int n, float (&v)[NR][NV],
+                                              const Columns<T, NV>& c, const Raw<O, NV> (&r)[NR]) {
+#pragma unroll
+  for (int u = 0; u < NR; ++u) {
+    if constexpr (Columns<T, NV>::kScaled) {
+      const int64_t row = m + STEP * u < p.M ? m + STEP * u : p.M - 1;
+      const float sx = p.x_scale ? p.x_scale[row] : 1.f;
+#pragma unroll
+      for (int e = 0; e < NV; ++e) v[u][e] *= sx * c.w[e];
+    }
+#pragma unroll
+    for (int e = 0; e < NV; ++e) v[u][e] += c.bias[e];
+  }
+  if (p.act != SENGINE_ACT_NONE) {
+    by_activation(p.act, [&](auto act) {
+#pragma unroll
+      for (int u = 0; u < NR; ++u)
+#pragma unroll
+        for (int e = 0; e < NV; ++e) v[u][e] = activate<decltype(act)::value>(v[u][e]);
+    });
+  }
+  if (n >= p.N) return;
+  if (p.res) {
+#pragma unroll
+    for (int u = 0; u < NR; ++u)
+#pragma unroll
+      for (int e = 0; e < NV; ++e) v[u][e] += (float)r[u].v[e];
+  }
+#pragma unroll
+  for (int u = 0; u < NR; ++u) {
+    if (m + STEP * u >= p.M) continue;
+    O* at = static_cast<O*>(p.out) + (m + STEP * u) * p.out_stride + n;
+    if constexpr (VEC) {
+      typename Raw<O, NV>::vec_t x;
+#pragma unroll
+      for (int e = 0; e < NV; ++e) x[e] = (O)v[u][e];
+      *reinterpret_cast<typename Raw<O, NV>::vec_t*>(at) = x;
+    } else {
+#pragma unroll
+      for (int e = 0; e < NV; ++e)
+        if (n + e < p.N) at[e] = (O)v[u][e];
+    }
+  }
+}
+
+// f(O(), Int<VEC>) for the output's type and layout.
+template <class F>
+__device__ __forceinline__ void by_output(const LinearParams& p, F f) {
+  if (p.vec) {
+    if (p.out_type == SENGINE_ENC_F32)
+      f(0.f, Int<1>{});
+    else if (p.out_type == SENGINE_ENC_F16)
+      f((_Float16)0.f, Int<1>{});
+    else
+      f((__bf16)0.f, Int<1>{});
+  } else {
+    if (p.out_type == SENGINE_ENC_F32)
+      f(0.f, Int<0>{});
+    else if (p.out_type == SENGINE_ENC_F16)
+      f((_Float16)0.f, Int<0>{});
+    else
+      f((__bf16)0.f, Int<0>{});
+  }
+}
+
+// The epilogue of TM x TN fragments: value e of fragment acc[i][j] is row m + 16 j, column
+// n + 32 (i / 2) + 4 (i % 2) + e, so that a lane has 8 neighbouring columns of a row.
+template <class T, int TM, int TN>
+__device__ __forceinline__ void linear_epilogue(const LinearParams& p, int64_t m, int n, float4_t (&acc)[TN][TM]) {
+  by_output(p, [&](auto o, auto vec) {
+    using O = decltype(o);
+    constexpr bool VEC = decltype(vec)::value;
+    Raw<O, 8> res[TN / 2][TM];
+#pragma unroll
+    for (int i = 0; i < TN / 2; ++i) linear_residual<O, VEC, TM, 16, 8>(p, m, n + 32 * i, res[i]);
+#pragma unroll
+    for (int i = 0; i < TN / 2; ++i) {
+      const Columns<T, 8> c(p, n + 32 * i);
+      float v[TM][8];
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = acc[2 * i + e / 4][j][e % 4];
+      linear_finish<T, O, VEC, TM, 16, 8>(p, m, n + 32 * i, v, c, res[i]);
+    }
+  });
+}
+
+// Workgroup -> tile.  Workgroups go to the eight XCDs in turn; each XCD takes one contiguous range of
+// an order that walks kLinGroup row tiles before the next column tile, so that what runs on an XCD at
+// a time is a block of tiles whose operands stay in its L2.
+constexpr int kLinGroup = 4;
+__device__ __forceinline__ void linear_tile_of(int id, int ntm, int ntn, int& mt, int& nt) {
+  const int total = ntm * ntn, per = total >> 3, rest = total & 7;
+  const int xcd = id & 7;
+  const int t = xcd * per + (xcd < rest ? xcd : rest) + (id >> 3);
+  const int group = t / (kLinGroup * ntn), first = group * kLinGroup;
+  const int rows = ntm - first < kLinGroup ? ntm - first : kLinGroup;
+  const int at = t - first * ntn;
+  nt = at / rows;
+  mt = first + at - nt * rows;
 }
 
 // Eight e4m3 codes as fp16: exact, every e4m3 value is one.
@@ -119,19 +252,25 @@ __device__ __forceinline__ half8_t widen_e4m3(uint32_t lo, uint32_t hi) {
 // 16-bit outputs take it; an fp32 output is computed from the codes widened to fp16 (E4m3Wide), at half
 // the rate, with sums of 32 bits.
 typedef int int8v_t __attribute__((ext_vector_type(8)));
+
+// One 64-byte half of that step, for the types whose instruction takes it.
+template <class T>
+__device__ __forceinline__ float4_t mma_64b(u32x4_t a, u32x4_t b, float4_t c) {
+  if constexpr (__is_same(T, _Float16)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
+                                                  0, 0);
+  } else if constexpr (__is_same(T, __bf16)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  } else {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen_e4m3(a[0], a[1]), widen_e4m3(b[0], b[1]), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(widen_e4m3(a[2], a[3]), widen_e4m3(b[2], b[3]), c, 0, 0, 0);
+  }
+}
+
 template <class T>
 __device__ __forceinline__ float4_t mma_128b(u32x4_t a0, u32x4_t a1, u32x4_t b0, u32x4_t b1, float4_t c) {
-  if constexpr (__is_same(T, _Float16)) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a0), __builtin_bit_cast(half8_t, b0), c, 0,
-                                               0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a1), __builtin_bit_cast(half8_t, b1), c,
-                                                  0, 0, 0);
-  } else if constexpr (__is_same(T, __bf16)) {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a0), __builtin_bit_cast(bf16x8_t, b0), c,
-                                                0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a1), __builtin_bit_cast(bf16x8_t, b1),
-                                                   c, 0, 0, 0);
-  } else if constexpr (__is_same(T, E4m3)) {
+  if constexpr (__is_same(T, E4m3)) {
     const u32x8_t a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
     const u32x8_t b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
     // both block scales 2^0 (exponent byte 127), both operands e4m3 (format 0)
@@ -139,10 +278,7 @@ __device__ __forceinline__ float4_t mma_128b(u32x4_t a0, u32x4_t a1, u32x4_t b0,
                                                             __builtin_bit_cast(int8v_t, b), c, 0, 0, 0, 0x7f7f7f7f, 0,
                                                             0x7f7f7f7f);
   } else {
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen_e4m3(a0[0], a0[1]), widen_e4m3(b0[0], b0[1]), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen_e4m3(a0[2], a0[3]), widen_e4m3(b0[2], b0[3]), c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen_e4m3(a1[0], a1[1]), widen_e4m3(b1[0], b1[1]), c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(widen_e4m3(a1[2], a1[3]), widen_e4m3(b1[2], b1[3]), c, 0, 0, 0);
+    return mma_64b<T>(a1, b1, mma_64b<T>(a0, b0, c));
   }
 }
 

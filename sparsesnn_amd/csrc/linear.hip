@@ -3,14 +3,14 @@
 //   y[m, n] = act(cx[m] cw[n] sum_k x[m, k] w[n, k] + b[n]) + r[m, n]
 // x and w are both fp16, both bf16 (cx = cw = 1) or both e4m3 with fp32 scales per row.  The sum and
 // the epilogue are fp32 and y is rounded once.
-#include "linear.h"
+#include "linear_rows.h"
+#include "linear_tile.h"
 
 namespace sengine {
 
 // Any strides, any alignment, any K.  Workgroup = 64 rows x 64 columns, four waves of 32 x 32; per
 // 128 bytes of the reduction both operands' rows go through registers into LDS: whole 16-byte pieces
 // by one load of whatever alignment, the row's last piece byte by byte, zeros beyond.
-constexpr int kLinStep = 128;        // bytes of the reduction a step
 constexpr int kLinPitch = 128 + 16;  // LDS row: 16 bytes more, so that 16 rows' pieces spread over the banks
 
 template <class T>
@@ -28,24 +28,13 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
     for (int j = 0; j < 2; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
 
   const int row = tid >> 3, piece = (tid & 7) * 16;  // rows row and row + 32 of each operand
-  const auto fetch = [&](const uint8_t* base, bool valid, int k) {
-    u32x4_t v = u32x4_t{0, 0, 0, 0};
-    if (!valid || k >= p.kbytes) return v;
-    if (k + 16 <= p.kbytes) {
-      __builtin_memcpy(&v, base + k, 16);
-      return v;
-    }
-    uint32_t w[4] = {0, 0, 0, 0};
-    for (int i = 0; k + i < p.kbytes; ++i) w[i >> 2] |= (uint32_t)base[k + i] << (8 * (i & 3));
-    return u32x4_t{w[0], w[1], w[2], w[3]};
-  };
   for (int k = 0; k < p.kbytes; k += kLinStep) {
     u32x4_t xv[2], wv[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = row + 32 * h;
-      xv[h] = fetch(p.x + (m0 + r) * p.x_stride, m0 + r < p.M, k + piece);
-      wv[h] = fetch(p.w + (int64_t)(n0 + r) * p.w_stride, n0 + r < p.N, k + piece);
+      xv[h] = fetch_piece(p.x + (m0 + r) * p.x_stride, k + piece, m0 + r < p.M ? p.kbytes : 0);
+      wv[h] = fetch_piece(p.w + (int64_t)(n0 + r) * p.w_stride, k + piece, n0 + r < p.N ? p.kbytes : 0);
     }
     __syncthreads();  // the previous step's reads are done
 #pragma unroll
@@ -60,7 +49,9 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = 64 * h + (lane >> 4) * 16;
-        a[i][h] = *reinterpret_cast<const u32x4_t*>(sW + (wn + 16 * i + (lane & 15)) * kLinPitch + at);
+        // the epilogue's columns: fragment i's row 4 g + e is weight row 8 g + 4 i + e
+        const int wr = wn + 8 * ((lane >> 2) & 3) + 4 * i + (lane & 3);
+        a[i][h] = *reinterpret_cast<const u32x4_t*>(sW + wr * kLinPitch + at);
         b[i][h] = *reinterpret_cast<const u32x4_t*>(sX + (wm + 16 * i + (lane & 15)) * kLinPitch + at);
       }
 #pragma unroll
@@ -68,28 +59,88 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) acc[i][j] = mma_128b<T>(a[i][0], a[i][1], b[j][0], b[j][1], acc[i][j]);
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      linear_store4(p, m0 + wm + 16 * j + (lane & 15), n0 + wn + 16 * i + 4 * (lane >> 4), acc[i][j]);
+  linear_epilogue<T, 2, 2>(p, m0 + wm + (lane & 15), n0 + wn + 8 * (lane >> 4), acc);
+}
+
+template <class T, int BM, int BN, int WM, int WN, int S, int WGS>
+static hipError_t run_tile(const LinearParams& p, int parts, hipStream_t stream) {
+  const int64_t ntm = (p.M + BM - 1) / BM, ntn = (p.N + BN - 1) / BN;
+  linear_tile_kernel<T, BM, BN, WM, WN, S, WGS>
+      <<<dim3((unsigned)(ntm * ntn), (unsigned)parts), dim3(64 * WM * WN), 0, stream>>>(p, (int)ntm, (int)ntn);
+  return hipGetLastError();
+}
+
+// Which kernel, and in how many parts.  Measured (bf16, us, the kernels as they stand here):
+//   up to 16 token rows     1 x 512 x 8192: rows 13, 64 x 64 tiles 30
+//   256 x 256 tiles, if there is one for every CU and 8 steps: 4096 x 4096 x 512: 28 (128: 35), x 4096: 104 (129);
+//                           with 6 steps, x 384 and GELU on 100352 x 1536: 270 (242)
+//   128 x 128 tiles, if there is one for every CU: 2048 x 2048 x 1024: 18 (64: 21); 3001 x 1000 x 1552: 27 (26);
+//                           1024 x 1024 x 1024: 13 (11)
+//   64 x 64 tiles otherwise, in parts of 12 steps or more up to two workgroups a CU, where the reduction has 48
+//                           steps: 32 x 4096 x 8192: 18 (in one: 31), x 512: 15 (30); 64 x 512 x 2048: 15 (12)
+enum { kLinAny, kLinRows, kLin64, kLin128, kLin256 };
+struct LinearPlan {
+  int kernel, parts, part_steps;
+};
+
+static int64_t tiles_of(const LinearParams& p, int b) { return (p.M + b - 1) / b * ((p.N + b - 1) / b); }
+
+static LinearPlan plan(const LinearParams& p, bool wide) {
+  constexpr int kCUs = 256;
+  const int steps = (p.kbytes + kLinStep - 1) / kLinStep;
+  if (p.M <= 16) return {kLinRows, 1, 0};
+  // LDS copies: whole 16-byte pieces, offsets inside a tile in 31 bits
+  const bool copies = p.kbytes % 16 == 0 && p.x_stride % 16 == 0 && p.w_stride % 16 == 0 &&
+                      (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.w % 16 == 0 && p.kbytes < (1 << 29) &&
+                      p.x_stride < (1 << 22) && p.w_stride < (1 << 22);
+  if (!copies) return {kLinAny, 1, 0};
+  if (!wide && tiles_of(p, 256) >= kCUs && steps >= 8) return {kLin256, 1, 0};
+  if (tiles_of(p, 128) >= kCUs) return {kLin128, 1, 0};
+  const int64_t most = 2 * kCUs / tiles_of(p, 64);
+  const int parts = (int)(most < steps / 12 ? most : steps / 12);
+  if (steps < 48 || parts < 2) return {kLin64, 1, 0};
+  const int part_steps = (steps + parts - 1) / parts;
+  return {kLin64, (steps + part_steps - 1) / part_steps, part_steps};
 }
 
 template <class T>
-static hipError_t run(const LinearParams& p, hipStream_t stream) {
-  const int64_t wgs = (p.M + 63) / 64 * ((p.N + 63) / 64);
-  if (wgs > 0x7fffffffll) return hipErrorInvalidValue;
-  linear_any_kernel<T><<<dim3((unsigned)wgs), dim3(256), 0, stream>>>(p);
-  return hipGetLastError();
+static hipError_t run(LinearParams p, float* workspace, size_t bytes, hipStream_t stream) {
+  const LinearPlan q = plan(p, __is_same(T, E4m3Wide));
+  switch (q.kernel) {
+    case kLinRows:
+      linear_rows_kernel<T, 1, 8, 4><<<dim3((unsigned)((p.N + 15) / 16)), dim3(512), 0, stream>>>(p);
+      return hipGetLastError();
+    case kLin64: {
+      const int64_t tiles = tiles_of(p, 64);
+      if (q.parts > 1 && workspace && bytes >= (size_t)(q.parts * tiles) * 64 * 64 * 4) {
+        p.partial = workspace;
+        p.part_steps = q.part_steps;
+        const hipError_t rc = run_tile<T, 64, 64, 2, 2, 4, 2>(p, q.parts, stream);
+        if (rc != hipSuccess) return rc;
+        linear_join_kernel<T><<<dim3((unsigned)(tiles * 4)), dim3(64), 0, stream>>>(p, (p.N + 63) / 64, (int)tiles, q.parts);
+        return hipGetLastError();
+      }
+      return run_tile<T, 64, 64, 2, 2, 4, 2>(p, 1, stream);
+    }
+    case kLin128:
+      return run_tile<T, 128, 128, 2, 2, 2, 2>(p, 1, stream);
+    case kLin256:
+      if constexpr (!__is_same(T, E4m3Wide)) return run_tile<T, 256, 256, 2, 2, 2, 1>(p, 1, stream);
+      [[fallthrough]];
+    default:
+      linear_any_kernel<T><<<dim3((unsigned)tiles_of(p, 64)), dim3(256), 0, stream>>>(p);
+      return hipGetLastError();
+  }
 }
 
 }  // namespace sengine
 
 using namespace sengine;
 
-extern "C" int sengine_amd_linear(const sengine_linear_desc* d, const void* x, const void* weight,
-                                  const float* x_scale, const float* weight_scale, const void* bias,
-                                  const void* residual, void* out, hipStream_t stream) {
+extern "C" int sengine_amd_linear_ws(const sengine_linear_desc* d, const void* x, const void* weight,
+                                     const float* x_scale, const float* weight_scale, const void* bias,
+                                     const void* residual, void* out, void* workspace, size_t workspace_bytes,
+                                     hipStream_t stream) {
   if (!d) return set_error(-1, "linear: null descriptor");
   if (d->M < 0 || d->N < 1 || d->K < 0) return set_error(-2, "linear: needs M >= 0, N >= 1, K >= 0");
   const bool e4m3 = d->in_type == SENGINE_ENC_E4M3;
@@ -127,15 +178,40 @@ extern "C" int sengine_amd_linear(const sengine_linear_desc* d, const void* x, c
   p.out_type = d->out_type;
   p.bias_type = d->bias_type;
   const auto fits = [&](const void* a, int64_t stride) {
-    return !a || ((uintptr_t)a % (4 * o) == 0 && (stride % 4 == 0 || d->M == 1));
+    return !a || ((uintptr_t)a % 16 == 0 && (stride * o % 16 == 0 || d->M == 1));
   };
-  p.vec = fits(out, d->out_stride) && fits(residual, d->residual_stride);
+  p.vec = d->N % 8 == 0 && fits(out, d->out_stride) && fits(residual, d->residual_stride);
+  if ((uintptr_t)workspace % 16) return set_error(-2, "linear: the workspace must be aligned to 16 bytes");
+  float* ws = static_cast<float*>(workspace);
   hipError_t rc;
   if (e4m3)
-    rc = d->out_type == SENGINE_ENC_F32 ? run<E4m3Wide>(p, stream) : run<E4m3>(p, stream);
+    rc = d->out_type == SENGINE_ENC_F32 ? run<E4m3Wide>(p, ws, workspace_bytes, stream)
+                                        : run<E4m3>(p, ws, workspace_bytes, stream);
   else if (d->in_type == SENGINE_ENC_F16)
-    rc = run<_Float16>(p, stream);
+    rc = run<_Float16>(p, ws, workspace_bytes, stream);
   else
-    rc = run<__bf16>(p, stream);
+    rc = run<__bf16>(p, ws, workspace_bytes, stream);
   return (int)rc;
+}
+
+extern "C" int sengine_amd_linear(const sengine_linear_desc* d, const void* x, const void* weight,
+                                  const float* x_scale, const float* weight_scale, const void* bias,
+                                  const void* residual, void* out, hipStream_t stream) {
+  return sengine_amd_linear_ws(d, x, weight, x_scale, weight_scale, bias, residual, out, nullptr, 0, stream);
+}
+
+extern "C" int sengine_amd_linear_workspace(const sengine_linear_desc* d, size_t* bytes) {
+  if (!d || !bytes) return set_error(-1, "linear_workspace: null argument");
+  *bytes = 0;
+  if (d->M < 1 || d->N < 1 || d->K < 1 || d->K > 0x3fffffff) return 0;
+  const int e = type_bytes(d->in_type);
+  LinearParams p{};
+  p.M = d->M;
+  p.N = d->N;
+  p.kbytes = d->K * e;
+  p.x_stride = d->x_stride * e;
+  p.w_stride = d->weight_stride * e;
+  const LinearPlan q = plan(p, d->in_type == SENGINE_ENC_E4M3 && d->out_type == SENGINE_ENC_F32);
+  if (q.parts > 1) *bytes = (size_t)(q.parts * tiles_of(p, 64)) * 64 * 64 * 4;
+  return 0;
 }

@@ -977,7 +977,10 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
 
 @functools.lru_cache(maxsize=1024)
 def _linear_desc(*fields):
-    return ctypes.byref(LinearDesc(*fields))
+    """(descriptor, bytes of scratch memory) of one problem."""
+    desc, size = ctypes.byref(LinearDesc(*fields)), ctypes.c_size_t()
+    check(_lib.load().sengine_amd_linear_workspace(desc, ctypes.byref(size)), "linear")
+    return desc, size.value
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
@@ -1033,10 +1036,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         out, os_ = torch.empty(shape, dtype=out_dtype, device=dev), N
     else:
         os_ = _token_out(out, shape, out_dtype, "out", dev)
-    check(_lib.load().sengine_amd_linear(
-        _linear_desc(M, xs, wst, rs, os_, N, K, code, ocode, bcode, ACTIVATIONS[activation]), x.data_ptr(),
-        weight.data_ptr(), _ptr(x_scale), _ptr(weight_scale), _ptr(bias), _ptr(residual), out.data_ptr(),
-        _stream(dev)), "linear")
+    desc, size = _linear_desc(M, xs, wst, rs, os_, N, K, code, ocode, bcode, ACTIVATIONS[activation])
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    check(_lib.load().sengine_amd_linear_ws(
+        desc, x.data_ptr(), weight.data_ptr(), _ptr(x_scale), _ptr(weight_scale), _ptr(bias), _ptr(residual),
+        out.data_ptr(), _ptr(ws), size, _stream(dev)), "linear")
     return out
 
 

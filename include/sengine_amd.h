@@ -558,6 +558,15 @@ typedef struct sengine_cross_desc {
 } sengine_cross_desc;
 int sengine_amd_cross_attention(const sengine_cross_desc* d, const void* q, const void* k, const void* v,
                                 const int32_t* key_lengths, const void* key_mask, void* out, hipStream_t stream);
+/*
+ * The same with scratch memory (16-byte aligned, of at least sengine_amd_cross_attention_workspace's bytes; what
+ * it holds before does not matter): few queries of many keys are then computed in parts of the keys, by more
+ * workgroups, and joined in a fixed order.  Without it, or with less, one workgroup goes through all keys.
+ */
+int sengine_amd_cross_attention_workspace(const sengine_cross_desc* d, size_t* bytes);
+int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const void* q, const void* k, const void* v,
+                                   const int32_t* key_lengths, const void* key_mask, void* out, void* workspace,
+                                   size_t workspace_bytes, hipStream_t stream);
 
 /*
  * Peak calibration on the box (the role of the reference's sengine/tuning/hw_calibrate.py:

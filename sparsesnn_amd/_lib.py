@@ -123,6 +123,8 @@ SIGNATURES = {
     "sengine_amd_linear_workspace": (ctypes.c_int, [_LDP, _SZP]),
     "sengine_amd_linear_ws": (ctypes.c_int, [_LDP, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "sengine_amd_cross_attention": (ctypes.c_int, [_CDP, _P, _P, _P, _P, _P, _P, _P]),
+    "sengine_amd_cross_attention_workspace": (ctypes.c_int, [_CDP, _SZP]),
+    "sengine_amd_cross_attention_ws": (ctypes.c_int, [_CDP, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "sengine_amd_pack_spikes": (ctypes.c_int, [_P, _I32, _I64, _I32, _P, _P]),
     "sengine_amd_unpack_spikes": (ctypes.c_int, [_P, _I64, _I32, _P, _I32, _P]),
 }

@@ -4,22 +4,12 @@
 // A query with no such key gets zeros.  What lies in a key or value that does not count is never
 // used, be it infinite or NaN.
 //
-// One wave a query row and head, an online softmax over 64 keys at a time: lane j forms the dot product
-// of key j, then the lanes share the values' columns.
-#include "token_types.h"
+#include "cross_tile.h"
 
 namespace sengine {
 
-struct CrossParams {
-  const void *q, *k, *v;
-  void* out;
-  const int32_t* lengths;
-  const uint8_t* mask;
-  int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h, o_b, o_l, o_h, mask_b;
-  int B, Lq, Lk, Hq, Hkv, d;
-  float scale;
-};
-
+// Any alignment and any strides: one wave a query row and head, an online softmax over 64 keys at a time, lane j
+// forming the dot product of key j, then the lanes sharing the values' columns.
 template <class T>
 __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
   __shared__ float sq[128], sp[64];
@@ -79,13 +69,78 @@ __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
   if (lane + 64 < p.d) out[lane + 64] = (T)(total == 0.f ? 0.f : o1 * inv);
 }
 
+struct CrossPlan {
+  int rows_a_block;  // 0: the row kernel
+  int parts;
+};
+
+static CrossPlan plan(const sengine_cross_desc* d) {
+  const int64_t heads = (int64_t)d->B * d->Hkv, rows = (int64_t)d->Lq * (d->Hq / d->Hkv);
+  CrossPlan q{rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256, 1};
+  const int64_t wgs = heads * ((rows + q.rows_a_block - 1) / q.rows_a_block);
+  const int64_t want = q.rows_a_block == 16 ? 1024 : 512, least = q.rows_a_block == 16 ? 256 : 512;
+  if (wgs * 2 <= want) {
+    int64_t parts = want / wgs;
+    if (parts > d->Lk / least) parts = d->Lk / least;
+    if (parts > 64) parts = 64;
+    if (parts > 1) q.parts = (int)parts;
+  }
+  return q;
+}
+
+static size_t cross_workspace(const sengine_cross_desc* d, int parts) {
+  return (size_t)parts * d->B * d->Lq * d->Hq * (d->d + 2) * sizeof(float);
+}
+
+template <class T, int DV, int NW, int QF, int KT, int S, bool SHARED, int WPE>
+static hipError_t run_tile(CrossParams& p, hipStream_t stream) {
+  p.blocks = (p.rows + (SHARED ? NW : 1) * 16 * QF - 1) / ((SHARED ? NW : 1) * 16 * QF);
+  const int64_t wgs = (int64_t)p.blocks * p.Hkv * p.parts * p.B;
+  if (wgs > 0x7fffffffll) return hipErrorInvalidValue;
+  if (p.mask)
+    cross_tile_kernel<T, DV, NW, QF, KT, S, SHARED, true, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
+  else
+    cross_tile_kernel<T, DV, NW, QF, KT, S, SHARED, false, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+template <class T, int DV>
+static hipError_t by_rows(CrossParams& p, int rows_a_block, hipStream_t stream) {
+  if (rows_a_block == 16) return run_tile<T, DV, 4, 1, 32, 2, false, 1>(p, stream);
+  if (rows_a_block == 64) return run_tile<T, DV, 4, 1, 64, 2, true, 2>(p, stream);
+  if (rows_a_block == 128) return run_tile<T, DV, 4, 2, 64, 2, true, 2>(p, stream);
+  return run_tile<T, DV, 8, 2, 64, 2, true, 2>(p, stream);
+}
+
+template <class T>
+static hipError_t by_width(CrossParams& p, int rows_a_block, hipStream_t stream) {
+  const int dv = (p.d + 15) / 16;
+  hipError_t e;
+  if (dv <= 1)
+    e = by_rows<T, 1>(p, rows_a_block, stream);
+  else if (dv <= 2)
+    e = by_rows<T, 2>(p, rows_a_block, stream);
+  else if (dv <= 3)
+    e = by_rows<T, 3>(p, rows_a_block, stream);
+  else if (dv <= 4)
+    e = by_rows<T, 4>(p, rows_a_block, stream);
+  else if (dv <= 6)
+    e = by_rows<T, 6>(p, rows_a_block, stream);
+  else
+    e = by_rows<T, 8>(p, rows_a_block, stream);
+  if (e != hipSuccess || p.parts == 1) return e;
+  const int64_t rows = (int64_t)p.B * p.Hkv * p.rows;
+  cross_join_kernel<T><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream>>>(p);
+  return hipGetLastError();
+}
+
 }  // namespace sengine
 
 using namespace sengine;
 
-extern "C" int sengine_amd_cross_attention(const sengine_cross_desc* d, const void* q, const void* k, const void* v,
-                                           const int32_t* key_lengths, const void* key_mask, void* out,
-                                           hipStream_t stream) {
+extern "C" int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const void* q, const void* k, const void* v,
+                                              const int32_t* key_lengths, const void* key_mask, void* out,
+                                              void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (!d) return set_error(-1, "cross_attention: null descriptor");
   if (d->B < 0 || d->Lq < 0 || d->Lk < 0 || d->Hq < 1 || d->Hkv < 1)
     return set_error(-2, "cross_attention: needs B, Lq, Lk >= 0 and heads >= 1");
@@ -111,10 +166,43 @@ extern "C" int sengine_amd_cross_attention(const sengine_cross_desc* d, const vo
   p.mask_b = d->mask_stride;
   p.B = d->B, p.Lq = d->Lq, p.Lk = d->Lk, p.Hq = d->Hq, p.Hkv = d->Hkv, p.d = d->d;
   p.scale = d->scale;
+  p.group = d->Hq / d->Hkv;
+  p.rows = d->Lq * p.group;
+  if ((uintptr_t)workspace % 16) return set_error(-2, "cross_attention: the workspace must be aligned to 16 bytes");
+  // the tile kernel: rows of d values that begin at multiples of 16 bytes, offsets in a stretch of keys in 31 bits
+  const auto aligned = [](const void* a, const int64_t* s) {
+    return (uintptr_t)a % 16 == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
+  };
+  const auto near = [](int64_t s) { return s >= 0 && s <= 0x3ffff; };
+  if (aligned(q, d->q_stride) && aligned(k, d->k_stride) && aligned(v, d->v_stride) && aligned(out, d->out_stride) &&
+      near(p.k_l) && near(p.v_l)) {
+    const CrossPlan plan_ = plan(d);
+    p.parts = plan_.parts;
+    if (p.parts > 1 && (!workspace || workspace_bytes < cross_workspace(d, p.parts))) p.parts = 1;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = p.part_o + (int64_t)p.parts * p.B * p.Hkv * p.rows * p.d;
+    return (int)(d->type == SENGINE_ENC_F16 ? by_width<_Float16>(p, plan_.rows_a_block, stream)
+                                            : by_width<__bf16>(p, plan_.rows_a_block, stream));
+  }
   const dim3 grid((unsigned)((int64_t)d->B * d->Lq * d->Hq));
   if (d->type == SENGINE_ENC_F16)
     cross_row_kernel<_Float16><<<grid, dim3(64), 0, stream>>>(p);
   else
     cross_row_kernel<__bf16><<<grid, dim3(64), 0, stream>>>(p);
   return (int)hipGetLastError();
+}
+
+extern "C" int sengine_amd_cross_attention(const sengine_cross_desc* d, const void* q, const void* k, const void* v,
+                                           const int32_t* key_lengths, const void* key_mask, void* out,
+                                           hipStream_t stream) {
+  return sengine_amd_cross_attention_ws(d, q, k, v, key_lengths, key_mask, out, nullptr, 0, stream);
+}
+
+extern "C" int sengine_amd_cross_attention_workspace(const sengine_cross_desc* d, size_t* bytes) {
+  if (!d || !bytes) return set_error(-1, "cross_attention_workspace: null argument");
+  *bytes = 0;
+  if (d->B < 1 || d->Lq < 1 || d->Lk < 1 || d->Hkv < 1 || d->Hq < d->Hkv || d->d < 8) return 0;
+  const int parts = plan(d).parts;
+  if (parts > 1) *bytes = cross_workspace(d, parts);
+  return 0;
 }

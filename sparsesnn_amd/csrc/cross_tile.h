@@ -1,0 +1,409 @@
+// Tile kernel of cross attention (cross_attention.hip).
+//
+// The queries that read one key head form rows: row i * group + h is query i of the group's head h.  A
+// workgroup takes 16 QF rows a wave of one sequence and key head and a range of its keys, KT keys at a time:
+//   S = K Q^T    matrix instructions, keys x rows: a lane has 4 keys a fragment of one row
+//   P            exponentials against the row's reference maximum, which is raised (and the sums rescaled)
+//                only when a score passes it by 2^8: the result does not depend on the reference
+//   O^T += V^T P^T   the P a lane has is the operand as it lies: the order of the reduction's keys over the
+//                lanes is free as long as V's operand, read from LDS transposed, has the same
+// K and V are copied into LDS by buffer loads, S tiles in flight.  SHARED: all waves work on the same tile
+// and meet once a tile; otherwise (few rows) each wave has tiles and LDS of its own, takes every NW-th tile,
+// never meets the others, and their results are joined at the end.
+//
+// A mask is turned into a list of the keys that count, 4096 keys at a time, and only those are fetched: what
+// does not count is neither read nor multiplied.  Places of the last tile past the end are filled with zeros
+// by the buffer's bounds check and score -infinity.
+//
+// LDS: a key's row has PR 16-byte pieces, piece j at place j ^ f(row): 8 lanes that read a piece of 8 rows, and
+// 16 lanes that read 32 bytes of 4 rows, touch every bank once.
+#pragma once
+#include "lds_copy.h"
+#include "token_types.h"
+
+namespace sengine {
+
+struct CrossParams {
+  const void *q, *k, *v;
+  void* out;
+  const int32_t* lengths;
+  const uint8_t* mask;
+  int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h, o_b, o_l, o_h, mask_b;
+  int B, Lq, Lk, Hq, Hkv, d;
+  float scale;
+  int group, rows, blocks;  // rows = Lq * group, in `blocks` row blocks
+  int parts;                // parts of the keys; more than one: partial results for the join
+  float* part_o;            // [part][sequence, key head, row][d], not divided by the sum
+  float* part_ml;           // [part][sequence, key head, row][2]: reference (base 2) and sum
+};
+
+constexpr int kCrossList = 4096;  // keys of a mask at a time
+
+template <class T>
+__device__ __forceinline__ float4_t mma_16(u32x4_t a, u32x4_t b, float4_t c) {
+  if constexpr (__is_same(T, _Float16))
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
+                                                  0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+}
+
+// Largest / sum of the four lanes l, l ^ 16, l ^ 32, l ^ 48.  A swap exchanges one half (32 lanes, or rows of 16)
+// of the first register with the other half of the second, so that of two copies one ends with the lane's own
+// value and the other with its partner's.  It needs two wait states after its operands are written.
+__device__ __forceinline__ float max_of_groups(float x) {
+  float y = x;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  x = fmaxf(x, y);
+  y = x;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  return fmaxf(x, y);
+}
+__device__ __forceinline__ float sum_of_groups(float x) {
+  x += __shfl_xor(x, 32, 64);
+  return x + __shfl_xor(x, 16, 64);
+}
+
+template <class T, int DV, int NW, int QF, int KT, int S, bool SHARED>
+struct CrossTile {
+  static constexpr int DK = (DV + 1) / 2;                       // 32-wide steps of q . k
+  static constexpr int PR = DK <= 1 ? 4 : DK <= 2 ? 8 : 16;     // pieces of a row in LDS
+  static constexpr int kRow = PR * 16, kOperand = KT * kRow, kStage = 2 * kOperand;
+  static constexpr int kAllCopies = 2 * KT * PR / 64;
+  static constexpr int kCopies = SHARED ? kAllCopies / NW : kAllCopies;  // of a wave a tile
+  static constexpr int kLds = (SHARED ? 1 : NW) * S * kStage;
+  static_assert(kAllCopies % (SHARED ? NW : 1) == 0 && KT % 32 == 0, "tile");
+  static_assert(SHARED || NW * 64 * DV * 16 <= kLds, "the waves' results fit");
+};
+
+template <class T, int DV, int NW, int QF, int KT, int S, bool SHARED, bool LIST, int WPE>
+__global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p) {
+  using C = CrossTile<T, DV, NW, QF, KT, S, SHARED>;
+  constexpr int DK = C::DK, PR = C::PR, NK = KT / 16;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[C::kLds];
+  __shared__ uint16_t list[LIST ? kCrossList : 1];
+  __shared__ float joint[SHARED ? 1 : NW][2][16];
+  __shared__ int counts[LIST ? NW : 1];
+  const int lane = (int)threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int g = lane >> 4, c = lane & 15;
+
+  // workgroup -> row block, key head, part, sequence: neighbours on an XCD share a sequence's rows of memory
+  int id = xcd_order((int)blockIdx.x, (int)gridDim.x);
+  const int block = id % p.blocks;
+  id /= p.blocks;
+  const int kh = id % p.Hkv;
+  id /= p.Hkv;
+  const int part = id % p.parts, b = id / p.parts;
+
+  int n = p.Lk;
+  if (p.lengths) {
+    const int len = p.lengths[b];
+    n = len < 0 ? 0 : len < n ? len : n;
+  }
+  const int64_t spans = (n + 63) / 64;  // parts take whole 64-key spans
+  const int k0 = (int)(spans * part / p.parts) * 64;
+  const int64_t kend = spans * (part + 1) / p.parts * 64;
+  const int k1 = kend < n ? (int)kend : n;
+
+  // the rows' queries as matrix operands; a negative scale goes into their sign
+  const int row0 = (block * (SHARED ? NW : 1) + (SHARED ? wave : 0)) * 16 * QF;
+  u32x4_t q[QF][DK];
+  const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+  const float cs = fabsf(p.scale) * 1.4426950408889634f;
+#pragma unroll
+  for (int f = 0; f < QF; ++f) {
+    const int row = row0 + 16 * f + c;
+    const T* at = static_cast<const T*>(p.q) + b * p.q_b + (row / p.group) * p.q_l +
+                  (kh * p.group + row % p.group) * p.q_h;
+#pragma unroll
+    for (int t = 0; t < DK; ++t) {
+      q[f][t] = u32x4_t{0, 0, 0, 0};
+      if (row < p.rows && 32 * t + 8 * g < p.d) {
+        q[f][t] = *reinterpret_cast<const u32x4_t*>(at + 32 * t + 8 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[f][t][i] ^= flip;
+      }
+    }
+  }
+
+  float4_t o[DV][QF];
+  float top[QF], total[QF];
+#pragma unroll
+  for (int f = 0; f < QF; ++f) {
+    top[f] = -INFINITY;
+    total[f] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DV; ++i) o[i][f] = float4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  uint8_t* ring = smem + (SHARED ? 0 : wave * S * C::kStage);
+  const uint32_t ring0 = lds_offset(ring);
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.k) + b * p.k_b + kh * p.k_h);
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.v) + b * p.v_b + kh * p.v_h);
+  const int kst = (int)p.k_l * 2, vst = (int)p.v_l * 2;  // bytes between keys
+  // where this lane reads K fragments and transposed V fragments
+  const int ksw = PR == 4 ? (c >> 1) & 3 : c & 7;
+  int kat[DK], vat[DV < 4 ? DV : 4];
+#pragma unroll
+  for (int t = 0; t < DK; ++t) kat[t] = c * C::kRow + (((4 * t + g) ^ ksw) << 4);
+#pragma unroll
+  for (int f = 0; f < (DV < 4 ? DV : 4); ++f) {
+    const int x = PR == 4 ? (c >> 3) & 1 : c >> 2;
+    vat[f] = C::kOperand + (4 * g + (c >> 2)) * C::kRow + (((2 * f + ((c >> 1) & 1)) ^ (2 * x)) << 4) + (c & 1) * 8;
+  }
+
+  for (int c0 = k0; c0 < k1;) {
+    // the keys of this stretch: a list of those that count, or all
+    int cnt = k1 - c0, cn = cnt;
+    if constexpr (LIST) {
+      constexpr int NG = kCrossList / NW / 64;  // 64-key groups of a wave
+      cn = cn < kCrossList ? cn : kCrossList;
+      const uint8_t* mk = p.mask + b * p.mask_b + c0;
+      uint64_t bits[NG];
+      int mine = 0;
+      __syncthreads();  // the list of the stretch before is no longer read
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        const int key = (wave * NG + i) * 64 + lane;
+        bits[i] = __ballot(key < cn && mk[key < cn ? key : 0] != 0);
+        mine += __popcll(bits[i]);
+      }
+      if (lane == 0) counts[wave] = mine;
+      __syncthreads();
+      int at = 0;
+      cnt = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        at += w < wave ? counts[w] : 0;
+        cnt += counts[w];
+      }
+      cnt = __builtin_amdgcn_readfirstlane(cnt);
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        if (bits[i] >> lane & 1)
+          list[at + __popcll(bits[i] & ((1ull << lane) - 1))] = (uint16_t)((wave * NG + i) * 64 + lane);
+        at += __popcll(bits[i]);
+      }
+      __syncthreads();
+    }
+    const int tiles = (cnt + KT - 1) / KT;
+    // copies of tile t into stage s of the ring; past the last tile they fetch nothing
+    const auto copy = [&](int t, int s) {
+      const int64_t j0 = LIST ? c0 : c0 + (int64_t)t * KT;
+      const uint8_t *ka = kbase + j0 * kst, *va = vbase + j0 * vst;
+      const u32x4_t kr = row_buffer(ka, 0x7fff0000), vr = row_buffer(va, 0x7fff0000);
+#pragma unroll
+      for (int j = 0; j < C::kCopies; ++j) {
+        const int qq = SHARED ? wave * C::kCopies + j : j;
+        const bool isv = qq >= C::kAllCopies / 2;
+        const int qo = isv ? qq - C::kAllCopies / 2 : qq;
+        const int row = qo * (64 / PR) + lane / PR;
+        const int sw = isv ? (PR == 4 ? (row >> 1 & 1) * 2 : (row & 3) * 2) : (PR == 4 ? row >> 1 & 3 : row & 7);
+        const int piece = (lane % PR) ^ sw;
+        const bool in = t * KT + row < cnt && piece * 8 < p.d;
+        int key = row;
+        if constexpr (LIST) key = in ? list[t * KT + row] : 0;
+        const int off = key * (isv ? vst : kst) + piece * 16;
+        u32x4_t r = kr;
+        if constexpr (SHARED) {
+          r[0] = scalar(isv ? vr[0] : kr[0]);
+          r[1] = scalar(isv ? vr[1] : kr[1]);
+        } else {
+          r = isv ? vr : kr;
+        }
+        lds_copy(r, ring0 + s * C::kStage + qq * 1024, in ? off : 0x7fffff00);
+      }
+    };
+    const int step = SHARED ? 1 : NW;
+    int t = SHARED ? 0 : wave;
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) copy(t + s * step, s);
+    int stage = 0;
+    for (; t < tiles; t += step) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"i"((S - 2) * C::kCopies) : "memory");
+      if constexpr (SHARED) {  // every wave's copies of this tile have landed, and none reads the stage before
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      {
+        const int fill = stage == 0 ? S - 1 : stage - 1;
+        copy(t + (S - 1) * step, fill);
+      }
+      const uint8_t* at = ring + stage * C::kStage;
+      stage = stage + 1 == S ? 0 : stage + 1;
+
+      float4_t s[NK][QF];
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+#pragma unroll
+        for (int f = 0; f < QF; ++f) s[i][f] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < DK; ++u) {
+          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(at + i * 16 * C::kRow + kat[u]);
+#pragma unroll
+          for (int f = 0; f < QF; ++f) s[i][f] = mma_16<T>(kf, q[f][u], s[i][f]);
+        }
+      }
+      const int left = cnt - t * KT;
+      if (left < KT) {
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * i + 4 * g + e >= left) {
+#pragma unroll
+              for (int f = 0; f < QF; ++f) s[i][f][e] = -INFINITY;
+            }
+      }
+      float high[QF];
+      bool raise = false;
+#pragma unroll
+      for (int f = 0; f < QF; ++f) {
+        high[f] = fmaxf(fmaxf(s[0][f][0], s[0][f][1]), fmaxf(s[0][f][2], s[0][f][3]));
+#pragma unroll
+        for (int i = 1; i < NK; ++i)
+          high[f] = fmaxf(high[f], fmaxf(fmaxf(s[i][f][0], s[i][f][1]), fmaxf(s[i][f][2], s[i][f][3])));
+        high[f] = max_of_groups(high[f]) * cs;
+        raise |= high[f] > top[f] + 8.f;
+      }
+      if (__any(raise)) {
+#pragma unroll
+        for (int f = 0; f < QF; ++f) {
+          const float t1 = fmaxf(top[f], high[f]);
+          const float back = t1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[f] - t1);
+          top[f] = t1;
+          total[f] *= back;
+#pragma unroll
+          for (int i = 0; i < DV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][f][e] *= back;
+        }
+      }
+      u32x4_t pr[KT / 32][QF];
+#pragma unroll
+      for (int f = 0; f < QF; ++f) {
+        const float ref = top[f] == -INFINITY ? 0.f : -top[f];  // every score so far is -infinity: they weigh nothing
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) {
+          typedef T vec8_t __attribute__((ext_vector_type(8)));
+          vec8_t x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * u + e / 4][f][e % 4], cs, ref));
+            total[f] += w;
+            x[e] = (T)w;
+          }
+          pr[u][f] = __builtin_bit_cast(u32x4_t, x);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < DV; ++i) {
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) {
+          const uint8_t* va = at + vat[i & 3] + (i >> 2) * 128 + u * 32 * C::kRow;
+          const u32x4_t vf = read_transposed(va, va + 16 * C::kRow);
+#pragma unroll
+          for (int f = 0; f < QF; ++f) o[i][f] = mma_16<T>(vf, pr[u][f], o[i][f]);
+        }
+      }
+      // this wave's reads of the stage are done before it may be filled again
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end
+    if constexpr (SHARED) __syncthreads();
+    c0 += cn;
+  }
+
+  if constexpr (!SHARED) {
+    static_assert(QF == 1, "one fragment of rows");
+    // join the waves: a common reference, sums and rows of O added up in the waves' order
+    total[0] = sum_of_groups(total[0]);
+    if (g == 0) {
+      joint[wave][0][c] = top[0];
+      joint[wave][1][c] = total[0];
+    }
+    __syncthreads();
+    float t1 = joint[0][0][c];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) t1 = fmaxf(t1, joint[w][0][c]);
+    const float back = top[0] == -INFINITY ? (total[0] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(top[0] - t1);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float tw = joint[w][0][c];
+      sum += joint[w][1][c] * (tw == -INFINITY ? (joint[w][1][c] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(tw - t1));
+    }
+    top[0] = t1;
+    total[0] = sum;
+    float4_t* mine = reinterpret_cast<float4_t*>(smem) + wave * DV * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < DV; ++i) mine[i * 64] = o[i][0] * back;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < DV; ++i) {
+      if (i % NW != wave) continue;
+      const float4_t* all = reinterpret_cast<const float4_t*>(smem) + i * 64 + lane;
+      o[i][0] = all[0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) o[i][0] += all[w * DV * 64];
+    }
+  } else {
+#pragma unroll
+    for (int f = 0; f < QF; ++f) total[f] = sum_of_groups(total[f]);
+  }
+#pragma unroll
+  for (int f = 0; f < QF; ++f) {
+    const int row = row0 + 16 * f + c;
+    if (row >= p.rows) continue;
+    if (p.parts > 1) {
+      const int64_t r = (((int64_t)part * p.B + b) * p.Hkv + kh) * p.rows + row;
+      if (g == 0 && (SHARED || wave == 0)) {
+        p.part_ml[2 * r] = top[f];
+        p.part_ml[2 * r + 1] = total[f];
+      }
+#pragma unroll
+      for (int i = 0; i < DV; ++i)
+        if ((SHARED || i % NW == wave) && 16 * i + 4 * g < p.d)
+          *reinterpret_cast<float4_t*>(p.part_o + r * p.d + 16 * i + 4 * g) = o[i][f];
+    } else {
+      const float inv = total[f] == 0.f ? 0.f : 1.f / total[f];
+      T* out = static_cast<T*>(p.out) + b * p.o_b + (row / p.group) * p.o_l + (kh * p.group + row % p.group) * p.o_h;
+#pragma unroll
+      for (int i = 0; i < DV; ++i)
+        if ((SHARED || i % NW == wave) && 16 * i + 4 * g < p.d) {
+          const float x[4] = {o[i][f][0] * inv, o[i][f][1] * inv, o[i][f][2] * inv, o[i][f][3] * inv};
+          store_floats<T, 4>(out + 16 * i + 4 * g, x);
+        }
+    }
+  }
+}
+
+// Joins the parts of the rows: 32 lanes a row, 4 columns a lane.
+template <class T>
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossParams p) {
+  const int64_t rows = (int64_t)p.B * p.Hkv * p.rows;
+  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int at = ((int)threadIdx.x & 31) * 4;
+  if (r >= rows || at >= p.d) return;
+  float top = -INFINITY;
+  for (int i = 0; i < p.parts; ++i) top = fmaxf(top, p.part_ml[2 * (i * rows + r)]);
+  float total = 0.f;
+  float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < p.parts; ++i) {
+    const float t = p.part_ml[2 * (i * rows + r)], l = p.part_ml[2 * (i * rows + r) + 1];
+    const float w = t == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(t - top);
+    total += l * w;
+    o += *reinterpret_cast<const float4_t*>(p.part_o + (i * rows + r) * p.d + at) * w;
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const int row = (int)(r % p.rows), kh = (int)(r / p.rows % p.Hkv);
+  const int64_t b = r / p.rows / p.Hkv;
+  const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  store_floats<T, 4>(static_cast<T*>(p.out) + b * p.o_b + (row / p.group) * p.o_l +
+                         (kh * p.group + row % p.group) * p.o_h + at, x);
+}
+
+}  // namespace sengine

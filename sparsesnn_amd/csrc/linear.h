@@ -215,21 +215,6 @@ __device__ __forceinline__ void linear_epilogue(const LinearParams& p, int64_t m
   });
 }
 
-// Workgroup -> tile.  Workgroups go to the eight XCDs in turn; each XCD takes one contiguous range of
-// an order that walks kLinGroup row tiles before the next column tile, so that what runs on an XCD at
-// a time is a block of tiles whose operands stay in its L2.
-constexpr int kLinGroup = 4;
-__device__ __forceinline__ void linear_tile_of(int id, int ntm, int ntn, int& mt, int& nt) {
-  const int total = ntm * ntn, per = total >> 3, rest = total & 7;
-  const int xcd = id & 7;
-  const int t = xcd * per + (xcd < rest ? xcd : rest) + (id >> 3);
-  const int group = t / (kLinGroup * ntn), first = group * kLinGroup;
-  const int rows = ntm - first < kLinGroup ? ntm - first : kLinGroup;
-  const int at = t - first * ntn;
-  nt = at / rows;
-  mt = first + at - nt * rows;
-}
-
 // Eight e4m3 codes as fp16: exact, every e4m3 value is one.
 __device__ __forceinline__ half8_t widen_e4m3(uint32_t lo, uint32_t hi) {
   typedef _Float16 half2_t __attribute__((ext_vector_type(2)));

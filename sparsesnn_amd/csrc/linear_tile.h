@@ -18,29 +18,23 @@
 // 32 LDS rows holds weight row 8 g + 4 b + e, and value e of fragment (b = i % 2) in lane group g is
 // then column 8 g + 4 b + e.
 #pragma once
+#include "lds_copy.h"
 #include "linear.h"
 
 namespace sengine {
 
 constexpr int kLinStep = 128;  // bytes of the reduction a step
 
-// One LDS copy: 64 lanes x 16 bytes from rsrc at each lane's offset to LDS bytes dst..dst + 1023.
-// Written as asm so that later LDS reads do not wait for it: the caller waits (vmcnt) and meets at a
-// barrier.  It returns nothing in registers.
-__device__ __forceinline__ void lds_copy(u32x4_t rsrc, uint32_t dst, int voff) {
-  asm volatile(
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds"
-      :
-      : "s"(dst), "v"(voff), "s"(rsrc)
-      : "memory");
-}
-
-// Buffer of `bytes` bytes from base (both the same in all lanes).
-__device__ __forceinline__ u32x4_t row_buffer(const uint8_t* base, int bytes) {
-  const uint64_t a = (uint64_t)(uintptr_t)base;
-  return u32x4_t{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, (uint32_t)bytes, (uint32_t)kBufferDword3};
+// Workgroup -> tile.  Each XCD walks kLinGroup row tiles before the next column tile, so that what runs on it
+// at a time is a block of tiles whose operands stay in its L2.
+constexpr int kLinGroup = 4;
+__device__ __forceinline__ void linear_tile_of(int id, int ntm, int ntn, int& mt, int& nt) {
+  const int t = xcd_order(id, ntm * ntn);
+  const int group = t / (kLinGroup * ntn), first = group * kLinGroup;
+  const int rows = ntm - first < kLinGroup ? ntm - first : kLinGroup;
+  const int at = t - first * ntn;
+  nt = at / rows;
+  mt = first + at - nt * rows;
 }
 
 // c += a b on one fragment, in place.  As asm the sums stay in the accumulation registers they have:
@@ -95,7 +89,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   int mt, nt;
-  linear_tile_of(blockIdx.x, ntm, ntn, mt, nt);
+  linear_tile_of((int)blockIdx.x, ntm, ntn, mt, nt);
   const int64_t m0 = (int64_t)mt * BM;
   const int n0 = nt * BN;
 
@@ -117,7 +111,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
     const int n = (r & ~31) + ((r >> 2) & 3) * 8 + ((r >> 4) & 1) * 4 + (r & 3);
     voff[C::kXCopies + j] = n * (int)p.w_stride + piece;
   }
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  const uint32_t lds0 = lds_offset(smem);
   // 64 fragments a wave fill the accumulation registers: there the loop is the only way through the steps
   // (two at a time, an odd last one followed by one of zeros), since sums that arrive by several ways would
   // have to be moved, through scratch memory.

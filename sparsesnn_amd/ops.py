@@ -1046,8 +1046,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
 @functools.lru_cache(maxsize=1024)
 def _cross_desc(qs, ks, vs, os_, *fields):
+    """(descriptor, bytes of scratch memory) of one problem."""
     s3 = ctypes.c_int64 * 3
-    return ctypes.byref(CrossDesc(s3(*qs[:3]), s3(*ks[:3]), s3(*vs[:3]), s3(*os_[:3]), *fields))
+    desc, size = ctypes.byref(CrossDesc(s3(*qs[:3]), s3(*ks[:3]), s3(*vs[:3]), s3(*os_[:3]), *fields)), ctypes.c_size_t()
+    check(_lib.load().sengine_amd_cross_attention_workspace(desc, ctypes.byref(size)), "cross_attention")
+    return desc, size.value
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float] = None,
@@ -1101,8 +1104,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
             raise SEngineError(f"key_mask: expected torch.bool ({B}, {Lk}) with contiguous rows, got "
                                f"{key_mask.dtype} {tuple(key_mask.shape)}")
         ms = key_mask.stride(0)
-    check(_lib.load().sengine_amd_cross_attention(
-        _cross_desc(*st, ms, B, Lq, Lk, Hq, Hkv, d, code, 1.0 / math.sqrt(d) if scale is None else scale),
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths), _ptr(key_mask), out.data_ptr(),
-        _stream(dev)), "cross_attention")
+    desc, size = _cross_desc(*st, ms, B, Lq, Lk, Hq, Hkv, d, code, 1.0 / math.sqrt(d) if scale is None else scale)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    check(_lib.load().sengine_amd_cross_attention_ws(
+        desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths), _ptr(key_mask), out.data_ptr(), _ptr(ws),
+        size, _stream(dev)), "cross_attention")
     return out

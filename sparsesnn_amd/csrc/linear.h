@@ -110,12 +110,13 @@ __device__ __forceinline__ void linear_residual(const LinearParams& p, int64_t m
   }
 }
 
-// The columns' coefficients; only 8-bit operands have scales.
+// The coefficients of NV columns and NR rows STEP apart; only 8-bit operands have scales.  Tile kernels load them
+// before their products, so that the epilogue does not wait for them.
 template <class T, int NV>
 struct Columns {
   static constexpr bool kScaled = sizeof(T) == 1;
   float w[kScaled ? NV : 1], bias[NV];
-  __device__ __forceinline__ Columns(const LinearParams& p, int n) {
+  __device__ __forceinline__ void load(const LinearParams& p, int n) {
 #pragma unroll
     for (int e = 0; e < NV; ++e) {
       const int at = n + e < p.N ? n + e : p.N - 1;
@@ -124,18 +125,31 @@ struct Columns {
     }
   }
 };
+template <class T, int NR, int STEP>
+struct RowScales {
+  static constexpr bool kScaled = sizeof(T) == 1;
+  float x[kScaled ? NR : 1];
+  __device__ __forceinline__ void load(const LinearParams& p, int64_t m) {
+    if constexpr (kScaled) {
+#pragma unroll
+      for (int u = 0; u < NR; ++u) {
+        const int64_t row = m + STEP * u < p.M ? m + STEP * u : p.M - 1;
+        x[u] = p.x_scale ? p.x_scale[row] : 1.f;
+      }
+    }
+  }
+};
 
 // The same rows and columns finished from their sums: scales, bias, activation and residual in fp32, one rounding.
 template <class T, class O, bool VEC, int NR, int STEP, int NV>
 __device__ __forceinline__ void linear_finish(const LinearParams& p, int64_t m, int n, float (&v)[NR][NV],
-                                              const Columns<T, NV>& c, const Raw<O, NV> (&r)[NR]) {
+                                              const Columns<T, NV>& c, const RowScales<T, NR, STEP>& rs,
+                                              const Raw<O, NV> (&r)[NR]) {
 #pragma unroll
   for (int u = 0; u < NR; ++u) {
     if constexpr (Columns<T, NV>::kScaled) {
-      const int64_t row = m + STEP * u < p.M ? m + STEP * u : p.M - 1;
-      const float sx = p.x_scale ? p.x_scale[row] : 1.f;
 #pragma unroll
-      for (int e = 0; e < NV; ++e) v[u][e] *= sx * c.w[e];
+      for (int e = 0; e < NV; ++e) v[u][e] *= rs.x[u] * c.w[e];
     }
 #pragma unroll
     for (int e = 0; e < NV; ++e) v[u][e] += c.bias[e];
@@ -193,24 +207,26 @@ __device__ __forceinline__ void by_output(const LinearParams& p, F f) {
 }
 
 // The epilogue of TM x TN fragments: value e of fragment acc[i][j] is row m + 16 j, column
-// n + 32 (i / 2) + 4 (i % 2) + e, so that a lane has 8 neighbouring columns of a row.
+// n + 32 (i / 2) + 4 (i % 2) + e, so that a lane has 8 neighbouring columns of a row.  c and rs are those
+// columns' and rows' coefficients.
 template <class T, int TM, int TN>
-__device__ __forceinline__ void linear_epilogue(const LinearParams& p, int64_t m, int n, float4_t (&acc)[TN][TM]) {
+__device__ __forceinline__ void linear_epilogue(const LinearParams& p, int64_t m, int n, float4_t (&acc)[TN][TM],
+                                                const Columns<T, 8> (&c)[TN / 2], const RowScales<T, TM, 16>& rs) {
   by_output(p, [&](auto o, auto vec) {
     using O = decltype(o);
     constexpr bool VEC = decltype(vec)::value;
-    Raw<O, 8> res[TN / 2][TM];
-#pragma unroll
-    for (int i = 0; i < TN / 2; ++i) linear_residual<O, VEC, TM, 16, 8>(p, m, n + 32 * i, res[i]);
+    Raw<O, 8> res[2][TM];  // those of the next columns are in flight while these are finished
+    linear_residual<O, VEC, TM, 16, 8>(p, m, n, res[0]);
 #pragma unroll
     for (int i = 0; i < TN / 2; ++i) {
-      const Columns<T, 8> c(p, n + 32 * i);
+      if (i + 1 < TN / 2) linear_residual<O, VEC, TM, 16, 8>(p, m, n + 32 * (i + 1), res[(i + 1) % 2]);
       float v[TM][8];
 #pragma unroll
       for (int j = 0; j < TM; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[j][e] = acc[2 * i + e / 4][j][e % 4];
-      linear_finish<T, O, VEC, TM, 16, 8>(p, m, n + 32 * i, v, c, res[i]);
+      linear_finish<T, O, VEC, TM, 16, 8>(p, m, n + 32 * i, v, c[i], rs, res[i % 2]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   });
 }

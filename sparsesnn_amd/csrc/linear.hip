@@ -8,6 +8,8 @@
 
 namespace sengine {
 
+constexpr int kLinStep = 128;  // bytes of the reduction that plans count in
+
 // Any strides, any alignment, any K.  Workgroup = 64 rows x 64 columns, four waves of 32 x 32; per
 // 128 bytes of the reduction both operands' rows go through registers into LDS: whole 16-byte pieces
 // by one load of whatever alignment, the row's last piece byte by byte, zeros beyond.
@@ -59,13 +61,17 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) acc[i][j] = mma_128b<T>(a[i][0], a[i][1], b[j][0], b[j][1], acc[i][j]);
   }
-  linear_epilogue<T, 2, 2>(p, m0 + wm + (lane & 15), n0 + wn + 8 * (lane >> 4), acc);
+  Columns<T, 8> cols[1];
+  RowScales<T, 2, 16> rscales;
+  cols[0].load(p, n0 + wn + 8 * (lane >> 4));
+  rscales.load(p, m0 + wm + (lane & 15));
+  linear_epilogue<T, 2, 2>(p, m0 + wm + (lane & 15), n0 + wn + 8 * (lane >> 4), acc, cols, rscales);
 }
 
-template <class T, int BM, int BN, int WM, int WN, int S, int WGS>
+template <class T, int HB, int BM, int BN, int WM, int WN, int S, int WGS>
 static hipError_t run_tile(const LinearParams& p, int parts, hipStream_t stream) {
   const int64_t ntm = (p.M + BM - 1) / BM, ntn = (p.N + BN - 1) / BN;
-  linear_tile_kernel<T, BM, BN, WM, WN, S, WGS>
+  linear_tile_kernel<T, HB, BM, BN, WM, WN, S, WGS>
       <<<dim3((unsigned)(ntm * ntn), (unsigned)parts), dim3(64 * WM * WN), 0, stream>>>(p, (int)ntm, (int)ntn);
   return hipGetLastError();
 }
@@ -115,17 +121,17 @@ static hipError_t run(LinearParams p, float* workspace, size_t bytes, hipStream_
       if (q.parts > 1 && workspace && bytes >= (size_t)(q.parts * tiles) * 64 * 64 * 4) {
         p.partial = workspace;
         p.part_steps = q.part_steps;
-        const hipError_t rc = run_tile<T, 64, 64, 2, 2, 4, 2>(p, q.parts, stream);
+        const hipError_t rc = run_tile<T, 128, 64, 64, 2, 2, 4, 2>(p, q.parts, stream);
         if (rc != hipSuccess) return rc;
         linear_join_kernel<T><<<dim3((unsigned)(tiles * 4)), dim3(64), 0, stream>>>(p, (p.N + 63) / 64, (int)tiles, q.parts);
         return hipGetLastError();
       }
-      return run_tile<T, 64, 64, 2, 2, 4, 2>(p, 1, stream);
+      return run_tile<T, 128, 64, 64, 2, 2, 4, 2>(p, 1, stream);
     }
     case kLin128:
-      return run_tile<T, 128, 128, 2, 2, 2, 2>(p, 1, stream);
+      return run_tile<T, 128, 128, 128, 2, 2, 2, 2>(p, 1, stream);
     case kLin256:
-      if constexpr (!__is_same(T, E4m3Wide)) return run_tile<T, 256, 256, 2, 2, 2, 1>(p, 1, stream);
+      if constexpr (!__is_same(T, E4m3Wide)) return run_tile<T, 128, 256, 256, 2, 2, 2, 1>(p, 1, stream);
       [[fallthrough]];
     default:
       linear_any_kernel<T><<<dim3((unsigned)tiles_of(p, 64)), dim3(256), 0, stream>>>(p);

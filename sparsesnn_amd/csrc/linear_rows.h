@@ -102,12 +102,15 @@ __global__ __launch_bounds__(64 * W) void linear_rows_kernel(LinearParams p) {
     constexpr bool VEC = decltype(vec)::value;
     Raw<O, 4> res[1];
     linear_residual<O, VEC, 1, 1, 4>(p, m, col, res);
-    const Columns<T, 4> c(p, col);
+    Columns<T, 4> c;
+    RowScales<T, 1, 1> rs;
+    c.load(p, col);
+    rs.load(p, m);
     float4_t sum = part[0][wave][lane];
 #pragma unroll
     for (int w = 1; w < W; ++w) sum += part[w][wave][lane];
     float v[1][4] = {{sum[0], sum[1], sum[2], sum[3]}};
-    linear_finish<T, O, VEC, 1, 1, 4>(p, m, col, v, c, res);
+    linear_finish<T, O, VEC, 1, 1, 4>(p, m, col, v, c, rs, res);
   });
 }
 

@@ -23,7 +23,6 @@
 
 namespace sengine {
 
-constexpr int kLinStep = 128;  // bytes of the reduction a step
 
 // Workgroup -> tile.  Each XCD walks kLinGroup row tiles before the next column tile, so that what runs on it
 // at a time is a block of tiles whose operands stay in its L2.
@@ -62,27 +61,47 @@ __device__ __forceinline__ void mma_inplace(u32x8_t a, u32x8_t b, float4_t& c) {
 }
 __device__ __forceinline__ void mma_drain() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
-__device__ __forceinline__ u32x4_t get_half(u32x8_t v, int h) {
-  return h ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3);
-}
-__device__ __forceinline__ void set_half(u32x8_t& v, int h, u32x4_t x) {
+// A lane's share of a fragment in one step: 16 bytes of each 64-byte half of its row.
+template <int HB>
+struct Fragment;
+template <>
+struct Fragment<64> {
+  u32x4_t v;
+  __device__ __forceinline__ void set(int, u32x4_t x) { v = x; }
+  __device__ __forceinline__ u32x4_t half(int) const { return v; }
+};
+template <>
+struct Fragment<128> {
+  u32x8_t v;
+  __device__ __forceinline__ void set(int h, u32x4_t x) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[4 * h + i] = x[i];
+    for (int i = 0; i < 4; ++i) v[4 * h + i] = x[i];
+  }
+  __device__ __forceinline__ u32x4_t half(int h) const {
+    return h ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3);
+  }
+};
+
+// Piece j of LDS row r lies at place j ^ lin_place(r).
+template <int PR>
+__device__ __forceinline__ int lin_place(int r) {
+  return PR == 4 ? r >> 1 & 3 : r & 7;
 }
 
-template <class T, int BM, int BN, int WM, int WN, int S>
+template <class T, int HB, int BM, int BN, int WM, int WN, int S>
 struct LinearTile {
   static constexpr int kWaves = WM * WN;
   static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  static constexpr int kStage = (BM + BN) * kLinStep;
-  static constexpr int kXCopies = BM / 8 / kWaves, kWCopies = BN / 8 / kWaves;  // LDS copies of a wave a stage
+  static constexpr int kStage = (BM + BN) * HB;
+  static constexpr int kXCopies = BM * HB / 1024 / kWaves, kWCopies = BN * HB / 1024 / kWaves;  // of a wave a stage
   static constexpr int kCopies = kXCopies + kWCopies;
-  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && TM % 2 == 0 && TN % 2 == 0, "tile");
+  static_assert(BM * HB % (1024 * kWaves) == 0 && BN * HB % (1024 * kWaves) == 0 && TM % 2 == 0 && TN % 2 == 0, "tile");
 };
 
-template <class T, int BM, int BN, int WM, int WN, int S, int WGS>
+template <class T, int HB, int BM, int BN, int WM, int WN, int S, int WGS>
 __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_tile_kernel(LinearParams p, int ntm, int ntn) {
-  using C = LinearTile<T, BM, BN, WM, WN, S>;
+  using C = LinearTile<T, HB, BM, BN, WM, WN, S>;
+  constexpr int PR = HB / 16;  // 16-byte pieces of a row in a stage
   constexpr int TM = C::TM, TN = C::TN;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[S * C::kStage];
   const int lane = (int)threadIdx.x & 63;
@@ -100,14 +119,15 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
   const uint8_t* wb = p.w + (int64_t)n0 * p.w_stride;
   const int xbytes = (mrows - 1) * (int)p.x_stride + p.kbytes;
   const int wbytes = (nrows - 1) * (int)p.w_stride + p.kbytes;
-  const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
+  // this lane's row and piece of each copy of 1024 bytes
+  const int lrow = lane / PR, piece = ((lane % PR) ^ lin_place<PR>(lrow)) * 16;
   int voff[C::kCopies];
 #pragma unroll
   for (int j = 0; j < C::kXCopies; ++j)
-    voff[j] = (8 * (wave * C::kXCopies + j) + (lane >> 3)) * (int)p.x_stride + piece;
+    voff[j] = (64 / PR * (wave * C::kXCopies + j) + lrow) * (int)p.x_stride + piece;
 #pragma unroll
   for (int j = 0; j < C::kWCopies; ++j) {
-    const int r = 8 * (wave * C::kWCopies + j) + (lane >> 3);  // LDS row; its weight row:
+    const int r = 64 / PR * (wave * C::kWCopies + j) + lrow;  // LDS row; its weight row:
     const int n = (r & ~31) + ((r >> 2) & 3) * 8 + ((r >> 4) & 1) * 4 + (r & 3);
     voff[C::kXCopies + j] = n * (int)p.w_stride + piece;
   }
@@ -116,7 +136,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
   // (two at a time, an odd last one followed by one of zeros), since sums that arrive by several ways would
   // have to be moved, through scratch memory.
   constexpr bool PAIRS = TM * TN >= 64;
-  const int total = (p.kbytes + kLinStep - 1) / kLinStep;
+  const int total = (p.kbytes + HB - 1) / HB;
   // a part of the reduction (blockIdx.y) or all of it
   const int first = p.partial ? (int)blockIdx.y * p.part_steps : 0;
   const int wanted = p.partial && total - first > p.part_steps ? p.part_steps : total - first;
@@ -126,11 +146,11 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
   u32x4_t xr, wr;
   uint32_t dst;
   const auto copies_of = [&](int step, int stage) {
-    const int k = (first + step) * kLinStep, left = step < wanted ? p.kbytes - k : 0;
+    const int k = (first + step) * HB, left = step < wanted ? p.kbytes - k : 0;
     xr = row_buffer(xb + k, left > 0 ? xbytes - k : 0);
     wr = row_buffer(wb + k, left > 0 ? wbytes - k : 0);
     dst = lds0 + stage * C::kStage;
-    if (left < kLinStep) {  // the tail: pieces past the row's end are out of range
+    if (left < HB) {  // the tail: pieces past the row's end are out of range
 #pragma unroll
       for (int j = 0; j < C::kCopies; ++j) voff[j] = piece < left ? voff[j] : 0x7fffff00;
     }
@@ -139,39 +159,53 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
     if (j < C::kXCopies)
       lds_copy(xr, dst + (wave * C::kXCopies + j) * 1024, voff[j]);
     else
-      lds_copy(wr, dst + BM * kLinStep + (wave * C::kWCopies + j - C::kXCopies) * 1024, voff[j]);
+      lds_copy(wr, dst + BM * HB + (wave * C::kWCopies + j - C::kXCopies) * 1024, voff[j]);
   };
+
+  // what the epilogue needs of the columns and rows that this lane finishes
+  constexpr int NV = PAIRS ? 4 : 8, NC = PAIRS ? 1 : TN / 2;
+  const int64_t em = m0 + wm * TM * 16 + (PAIRS ? lane >> 5 : lane & 15);
+  const int en = n0 + wn * TN * 16 + (PAIRS ? (lane & 31) * 4 : (lane >> 4) * 8);
+  Columns<T, NV> cols[NC];
+  RowScales<T, TM, 16> rscales;
+  if (!p.partial) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) cols[i].load(p, en + 32 * i);
+    if constexpr (!PAIRS) rscales.load(p, em);
+  }
 
   float4_t acc[TN][TM];
 #pragma unroll
   for (int i = 0; i < TN; ++i)
 #pragma unroll
     for (int j = 0; j < TM; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
-  u32x8_t a[TN], b[TM];  // 32 bytes of a row: both 64-byte halves of a step
-  // this lane's 16 bytes of fragment row lane % 16: pieces lane / 16 and 4 + lane / 16
-  const int fr = (lane & 15) * kLinStep, sw = lane & 7;
+  Fragment<HB> a[TN], b[TM];
+  // this lane's 16 bytes of fragment row lane % 16 in either half of the step: pieces lane / 16 and 4 + lane / 16
+  const int fr = (lane & 15) * HB, sw = lin_place<PR>(lane & 15);
   const int at0 = fr + (((lane >> 4) ^ sw) << 4), at1 = fr + (((4 + (lane >> 4)) ^ sw) << 4);
-  const int xat = wm * TM * 16 * kLinStep, wat = BM * kLinStep + wn * TN * 16 * kLinStep;
+  const int xat = wm * TM * 16 * HB, wat = BM * HB + wn * TN * 16 * HB;
   const auto read_a = [&](int stage_at, int i, int h) {
-    set_half(a[i], h, *reinterpret_cast<const u32x4_t*>(smem + stage_at + wat + i * 16 * kLinStep + (h ? at1 : at0)));
+    a[i].set(h, *reinterpret_cast<const u32x4_t*>(smem + stage_at + wat + i * 16 * HB + (h ? at1 : at0)));
   };
   const auto read_b = [&](int stage_at, int j, int h) {
-    set_half(b[j], h, *reinterpret_cast<const u32x4_t*>(smem + stage_at + xat + j * 16 * kLinStep + (h ? at1 : at0)));
+    b[j].set(h, *reinterpret_cast<const u32x4_t*>(smem + stage_at + xat + j * 16 * HB + (h ? at1 : at0)));
   };
   // Products FROM..TO-1 of the NM of quarter (i0, j0), with hook(n) before product n.
-  constexpr int NH = __is_same(T, E4m3) ? 1 : 2;  // 64-byte halves of a step that are products of their own
+  constexpr int LH = HB / 64;                      // 64-byte halves of a step
+  constexpr int NH = __is_same(T, E4m3) ? 1 : LH;  // those that are products of their own
+  static_assert(!__is_same(T, E4m3) || HB == 128, "8-bit products take 128 bytes");
   constexpr int NM = NH * (TN / 2) * (TM / 2);
   const auto quarter = [&](int i0, int j0, int from, int to, auto hook) {
 #pragma unroll
     for (int n = from; n < to; ++n) {
       const int h = n / (TN / 2 * (TM / 2)), i = i0 + n / (TM / 2) % (TN / 2), j = j0 + n % (TM / 2);
       hook(n);
-      if constexpr (NH == 1)
-        mma_inplace<PAIRS>(a[i], b[j], acc[i][j]);
+      if constexpr (__is_same(T, E4m3))
+        mma_inplace<PAIRS>(a[i].v, b[j].v, acc[i][j]);
       else if constexpr (__is_same(T, E4m3Wide))
-        acc[i][j] = mma_64b<T>(get_half(a[i], h), get_half(b[j], h), acc[i][j]);
+        acc[i][j] = mma_64b<T>(a[i].half(h), b[j].half(h), acc[i][j]);
       else
-        mma_inplace<T, PAIRS>(get_half(a[i], h), get_half(b[j], h), acc[i][j]);
+        mma_inplace<T, PAIRS>(a[i].half(h), b[j].half(h), acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -193,7 +227,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < LH; ++h) {
 #pragma unroll
       for (int i = 0; i < TN / 2; ++i) read_a(0, i, h);
 #pragma unroll
@@ -207,10 +241,10 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
       const int nstage = stage + 1 == S ? 0 : stage + 1;
       const int nxt = nstage * C::kStage;
       quarter(0, F, 0, NM, [&](int n) {
-        spread(n, TM, NM, [&](int r) { read_b(cur, G + r % (TM / 2), r / (TM / 2)); });
+        spread(n, LH * TM / 2, NM, [&](int r) { read_b(cur, G + r % (TM / 2), r / (TM / 2)); });
       });
       quarter(0, G, 0, NM, [&](int n) {
-        spread(n, TN, NM, [&](int r) { read_a(cur, TN / 2 + r % (TN / 2), r / (TN / 2)); });
+        spread(n, LH * TN / 2, NM, [&](int r) { read_a(cur, TN / 2 + r % (TN / 2), r / (TN / 2)); });
       });
       quarter(TN / 2, G, 0, SPLIT, [&](int) {});
       // this wave has read the stage (lgkmcnt) and its copies of the next one have landed (vmcnt)
@@ -221,12 +255,12 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
       __builtin_amdgcn_sched_barrier(0);
       // the rest of the step: the next one's first operands and the copies
       const auto rest = [&](int n) {
-        spread(n, TN + TM, REST, [&](int r) {
-          if constexpr (NH == 1) {  // a fragment's halves are one operand: B's only after its last use
-            if (r < TN)
+        spread(n, LH * (TN + TM) / 2, REST, [&](int r) {
+          if constexpr (NH == 1) {  // a fragment is one operand: B's only after its last use
+            if (r < LH * TN / 2)
               read_a(nxt, r % (TN / 2), r / (TN / 2));
             else
-              read_b(nxt, G + (r - TN) % (TM / 2), (r - TN) / (TM / 2));
+              read_b(nxt, G + (r - LH * TN / 2) % (TM / 2), (r - LH * TN / 2) / (TM / 2));
           } else {
             const int h = r / (TN / 2 + TM / 2), q = r % (TN / 2 + TM / 2);
             if (q < TN / 2)
@@ -270,8 +304,8 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
       return;
     }
   }
-  if constexpr (TM * TN < 64) {
-    linear_epilogue<T, TM, TN>(p, m0 + wm * TM * 16 + (lane & 15), n0 + wn * TN * 16 + (lane >> 4) * 8, acc);
+  if constexpr (!PAIRS) {
+    linear_epilogue<T, TM, TN>(p, em, en, acc, cols, rscales);
   } else {
     // 64 fragments: the code that finishes them would be too long laid out one after the other.  The sums
     // go through the wave's part of LDS (once the last copies have landed), TM / RJ fragment rows a round, in
@@ -282,15 +316,14 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
     static_assert(PR == 32 && TM * 16 * PR * 16 * C::kWaves <= RJ * S * C::kStage, "sums of a round fit");
     __syncthreads();
     uint8_t* part = smem + wave * (S * C::kStage / C::kWaves);
-    const int col = n0 + wn * TN * 16 + 4 * (lane & 31);
     by_output(p, [&](auto o, auto vec) {
       using O = decltype(o);
       constexpr bool VEC = decltype(vec)::value;
       constexpr int U = 8, RR = TM / RJ * 16;  // rows of a lane at a time (two rows apart), rows a round
-      const int64_t m = m0 + wm * TM * 16 + (lane >> 5);
-      const Columns<T, 4> c(p, col);
       Raw<O, 4> next[U];
-      linear_residual<O, VEC, U, 2, 4>(p, m, col, next);
+      RowScales<T, U, 2> nrs;
+      linear_residual<O, VEC, U, 2, 4>(p, em, en, next);
+      nrs.load(p, em);
 #pragma unroll
       for (int q = 0; q < RJ; ++q) {
 #pragma unroll
@@ -303,9 +336,11 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
           }
         for (int r0 = 0; r0 < RR; r0 += 2 * U) {
           Raw<O, 4> res[U];
+          const RowScales<T, U, 2> rs = nrs;
 #pragma unroll
           for (int u = 0; u < U; ++u) res[u] = next[u];
-          linear_residual<O, VEC, U, 2, 4>(p, m + q * RR + r0 + 2 * U, col, next);  // clamped past the last row
+          linear_residual<O, VEC, U, 2, 4>(p, em + q * RR + r0 + 2 * U, en, next);  // clamped past the last row
+          nrs.load(p, em + q * RR + r0 + 2 * U);
           float v[U][4];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
@@ -314,7 +349,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[u][e] = x[e];
           }
-          linear_finish<T, O, VEC, U, 2, 4>(p, m + q * RR + r0, col, v, c, res);
+          linear_finish<T, O, VEC, U, 2, 4>(p, em + q * RR + r0, en, v, cols[0], rs, res);
         }
       }
     });
@@ -326,6 +361,12 @@ template <class T>
 __global__ __launch_bounds__(64) void linear_join_kernel(LinearParams p, int ntn, int tiles, int parts) {
   const int lane = (int)threadIdx.x, tile = (int)blockIdx.x >> 2, wave = (int)blockIdx.x & 3;
   const float4_t* at = reinterpret_cast<const float4_t*>(p.partial) + (int64_t)blockIdx.x * 256 + lane;
+  const int64_t m = (int64_t)(tile / ntn) * 64 + (wave >> 1) * 32 + (lane & 15);
+  const int n = tile % ntn * 64 + (wave & 1) * 32 + (lane >> 4) * 8;
+  Columns<T, 8> cols[1];
+  RowScales<T, 2, 16> rscales;
+  cols[0].load(p, n);
+  rscales.load(p, m);
   float4_t acc[2][2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i / 2][i % 2] = at[i * 64];
@@ -335,8 +376,7 @@ __global__ __launch_bounds__(64) void linear_join_kernel(LinearParams p, int ntn
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i / 2][i % 2] += at[i * 64];
   }
-  linear_epilogue<T, 2, 2>(p, (int64_t)(tile / ntn) * 64 + (wave >> 1) * 32 + (lane & 15),
-                           tile % ntn * 64 + (wave & 1) * 32 + (lane >> 4) * 8, acc);
+  linear_epilogue<T, 2, 2>(p, m, n, acc, cols, rscales);
 }
 
 }  // namespace sengine

@@ -8,7 +8,6 @@ pointers and cannot check buffer sizes itself).
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 import os
 from dataclasses import dataclass, replace
@@ -17,8 +16,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import (ACTIVATIONS, ENC_BF16, ENC_BITS, ENC_E4M3, ENC_F16, ENC_F32, NEURON_IF, NEURON_LIF, NEURON_MS, WLAYOUT_HWIO, WLAYOUT_OIHW,
-                   ConvLifDesc, CrossDesc, LinearDesc, RmsNormDesc, SEngineError, check)
+from ._lib import (ACTIVATIONS, ENC_BF16, ENC_BITS, ENC_E4M3, ENC_F16, ENC_F32, NEURON_IF, NEURON_LIF, NEURON_MS,
+                   WLAYOUT_HWIO, WLAYOUT_OIHW, ConvLifDesc, CrossDesc, LinearDesc, RmsNormDesc, SEngineError, check)
 
 __all__ = [
     "ConvSpec", "make_desc", "geometry", "set_fused_kernel", "compress_2_4", "pack_dense_weights", "pack_spikes",
@@ -912,22 +911,25 @@ def _token_out(t, shape, dtype, name: str, device):
     return _token_rows(t, name)[1]
 
 
-@functools.lru_cache(maxsize=1024)
-def _rms_norm_desc(*fields):
-    return ctypes.byref(RmsNormDesc(*fields))
+# What a call's checks come to depends on its tensors' types, shapes, strides and devices only; it is kept under them,
+# so that the calls of a decoding loop do not pay for the checks again (they take longer than a small kernel).
+_TOKEN_PLANS: dict = {}
 
 
-def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
-             eps: float = 1e-6, out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
-             stream_out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
-    """Root-mean-square norm of rows x (..., D) with the residual's addition: s = x + residual,
-    y = s / sqrt(mean(s^2) + eps) * weight, in fp32, y formed from the unrounded s.
+def _remember(key, plan):
+    if key is not None:
+        if len(_TOKEN_PLANS) >= 4096:
+            _TOKEN_PLANS.clear()
+        _TOKEN_PLANS[key] = plan
+    return plan
 
-    x is fp16, bf16 or fp32; residual and stream have its shape and type; weight (D,) its type or
-    fp32.  Returns (y, stream) with y in x's type, or with out_dtype=torch.float8_e4m3fn
-    (y, stream, scale): y's codes and one fp32 scale a row (shape x.shape[:-1]), y ~ codes * scale.
-    stream is s rounded to x's type, None without a residual.  `out`, `stream_out` (which may be
-    `residual`, updated in place) and `scale` take the results where given."""
+
+def _layout(t):
+    return None if t is None else (t.dtype, t.shape, t.stride(), t.device)
+
+
+def _rms_norm_plan(key, x, weight, residual, eps, out_dtype, out, stream_out, scale):
+    """(descriptor, output's type, whether that is e4m3, rows' shape, device, whether x is dense) of a checked call."""
     _token_input(x, "x")
     dev, code = x.device, _type_code(x, (torch.float16, torch.bfloat16, torch.float32), "x")
     if x.dim() == 0:
@@ -951,51 +953,53 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
         out_dtype = x.dtype
     elif out_dtype is not x.dtype and not eight:
         raise SEngineError(f"out_dtype: expected {x.dtype} or torch.float8_e4m3fn, got {out_dtype}")
+    os_ = D if out is None else _token_out(out, shape, out_dtype, "out", dev)
+    ss = D if stream_out is None else _token_out(stream_out, shape, x.dtype, "stream_out", dev)
+    if scale is not None:
+        if not eight:
+            raise SEngineError("scale goes with out_dtype=torch.float8_e4m3fn")
+        _token_vector(scale, rows, "scale", dev)
+        _type_code(scale, (torch.float32,), "scale")
+    desc = ctypes.byref(RmsNormDesc(rows, xs, rs, os_, ss, D, code, ws, _TOKEN_TYPES[out_dtype], eps))
+    return _remember(key, (desc, out_dtype, eight, shape, dev, x.is_contiguous()))
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+             eps: float = 1e-6, out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
+             stream_out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
+    """Root-mean-square norm of rows x (..., D) with the residual's addition: s = x + residual,
+    y = s / sqrt(mean(s^2) + eps) * weight, in fp32, y formed from the unrounded s.
+
+    x is fp16, bf16 or fp32; residual and stream have its shape and type; weight (D,) its type or
+    fp32.  Returns (y, stream) with y in x's type, or with out_dtype=torch.float8_e4m3fn
+    (y, stream, scale): y's codes and one fp32 scale a row (shape x.shape[:-1]), y ~ codes * scale.
+    stream is s rounded to x's type, None without a residual.  `out`, `stream_out` (which may be
+    `residual`, updated in place) and `scale` take the results where given."""
+    key = None
+    if out is None and stream_out is None and scale is None:
+        try:
+            key = ("norm", x.dtype, x.shape, x.stride(), x.device, eps, out_dtype, _layout(weight), _layout(residual))
+        except AttributeError:
+            pass  # not a tensor: the checks say so
+    plan = _TOKEN_PLANS.get(key)
+    if plan is None or (torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad)
+            or (residual is not None and residual.requires_grad))):
+        plan = _rms_norm_plan(key, x, weight, residual, eps, out_dtype, out, stream_out, scale)
+    desc, out_dtype, eight, shape, dev, dense = plan
     if out is None:
-        out, os_ = torch.empty(shape, dtype=out_dtype, device=dev), D
-    else:
-        os_ = _token_out(out, shape, out_dtype, "out", dev)
-    ss = D
-    if residual is not None:
-        if stream_out is None:
-            stream_out = torch.empty(shape, dtype=x.dtype, device=dev)
-        else:
-            ss = _token_out(stream_out, shape, x.dtype, "stream_out", dev)
-    if eight:
-        if scale is None:
-            scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
-        else:
-            _token_vector(scale, rows, "scale", dev)
-            _type_code(scale, (torch.float32,), "scale")
-    elif scale is not None:
-        raise SEngineError("scale goes with out_dtype=torch.float8_e4m3fn")
-    check(_lib.load().sengine_amd_rms_norm(
-        _rms_norm_desc(rows, xs, rs, os_, ss, D, code, ws, _TOKEN_TYPES[out_dtype], eps), x.data_ptr(),
-        _ptr(residual), _ptr(weight), out.data_ptr(), _ptr(stream_out), _ptr(scale), _stream(dev)), "rms_norm")
+        out = torch.empty(shape, dtype=out_dtype, device=dev) if eight or not dense else torch.empty_like(x)
+    if residual is not None and stream_out is None:
+        stream_out = torch.empty_like(x) if dense else torch.empty(shape, dtype=x.dtype, device=dev)
+    if eight and scale is None:
+        scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    check(_lib.load().sengine_amd_rms_norm(desc, x.data_ptr(), _ptr(residual), _ptr(weight), out.data_ptr(),
+                                           _ptr(stream_out), _ptr(scale), _stream(dev)), "rms_norm")
     return (out, stream_out, scale) if eight else (out, stream_out)
 
 
-@functools.lru_cache(maxsize=1024)
-def _linear_desc(*fields):
-    """(descriptor, bytes of scratch memory) of one problem."""
-    desc, size = ctypes.byref(LinearDesc(*fields)), ctypes.c_size_t()
-    check(_lib.load().sengine_amd_linear_workspace(desc, ctypes.byref(size)), "linear")
-    return desc, size.value
-
-
-def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
-           residual: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None,
-           weight_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
-           out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """act(x weight^T + bias) + residual of token rows x (..., K) with weight (N, K), nn.Linear's
-    layout; activation 'none' | 'relu' | 'gelu' (by the error function) | 'gelu_tanh' | 'silu'.
-
-    x and weight are both fp16, both bf16, or both float8_e4m3fn with fp32 scales of x's rows
-    (x_scale, as rms_norm returns it) and of weight's rows (weight_scale, (N,)).  The sums and what
-    follows them are fp32 (the 8-bit matrix instructions keep about 16 bits of a sum, which a 16-bit
-    result hides; an fp32 result of e4m3 operands takes the 16-bit ones at half the rate); the result is rounded once to out_dtype (fp16, bf16 or fp32; x's type,
-    for e4m3 bf16, by default).  residual (..., N) has out_dtype, bias (N,) fp16, bf16 or fp32;
-    `out` may be `residual`."""
+def _linear_plan(key, x, weight, bias, activation, residual, x_scale, weight_scale, out_dtype, out):
+    """(descriptor, bytes of scratch memory, output's shape and type, device) of a checked call."""
     _token_input(x, "x")
     dev = x.device
     code = _type_code(x, (torch.float16, torch.bfloat16, torch.float8_e4m3fn), "x")
@@ -1032,11 +1036,44 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
             raise SEngineError(f"residual: expected {out_dtype} {shape}, got {residual.dtype} "
                                f"{tuple(residual.shape)}")
         rs = _token_rows(residual, "residual")[1]
+    os_ = N if out is None else _token_out(out, shape, out_dtype, "out", dev)
+    desc = ctypes.byref(LinearDesc(M, xs, wst, rs, os_, N, K, code, ocode, bcode, ACTIVATIONS[activation]))
+    size = ctypes.c_size_t()
+    check(_lib.load().sengine_amd_linear_workspace(desc, ctypes.byref(size)), "linear")
+    return _remember(key, (desc, size.value, shape, out_dtype, dev))
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+           residual: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None,
+           weight_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x weight^T + bias) + residual of token rows x (..., K) with weight (N, K), nn.Linear's
+    layout; activation 'none' | 'relu' | 'gelu' (by the error function) | 'gelu_tanh' | 'silu'.
+
+    x and weight are both fp16, both bf16, or both float8_e4m3fn with fp32 scales of x's rows
+    (x_scale, as rms_norm returns it) and of weight's rows (weight_scale, (N,)).  The sums and what
+    follows them are fp32 (the 8-bit matrix instructions keep about 16 bits of a sum, which a 16-bit
+    result hides; an fp32 result of e4m3 operands takes the 16-bit ones at half the rate); the result
+    is rounded once to out_dtype (fp16, bf16 or fp32; x's type, for e4m3 bf16, by default).  residual
+    (..., N) has out_dtype, bias (N,) fp16, bf16 or fp32; `out` may be `residual`.  A long reduction
+    with few results is computed in parts through scratch memory of torch's allocator, the parts
+    added in a fixed order."""
+    key = None
     if out is None:
-        out, os_ = torch.empty(shape, dtype=out_dtype, device=dev), N
-    else:
-        os_ = _token_out(out, shape, out_dtype, "out", dev)
-    desc, size = _linear_desc(M, xs, wst, rs, os_, N, K, code, ocode, bcode, ACTIVATIONS[activation])
+        try:
+            key = ("linear", x.dtype, x.shape, x.stride(), x.device, weight.dtype, weight.shape, weight.stride(),
+                   weight.device, activation, out_dtype, _layout(bias), _layout(residual), _layout(x_scale),
+                   _layout(weight_scale))
+        except AttributeError:
+            pass  # not a tensor: the checks say so
+    plan = _TOKEN_PLANS.get(key)
+    if plan is None or (torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad
+            or any(t is not None and t.requires_grad for t in (bias, residual, x_scale, weight_scale)))):
+        plan = _linear_plan(key, x, weight, bias, activation, residual, x_scale, weight_scale, out_dtype, out)
+    desc, size, shape, out_dtype, dev = plan
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=dev)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     check(_lib.load().sengine_amd_linear_ws(
         desc, x.data_ptr(), weight.data_ptr(), _ptr(x_scale), _ptr(weight_scale), _ptr(bias), _ptr(residual),
@@ -1044,27 +1081,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     return out
 
 
-@functools.lru_cache(maxsize=1024)
-def _cross_desc(qs, ks, vs, os_, *fields):
-    """(descriptor, bytes of scratch memory) of one problem."""
-    s3 = ctypes.c_int64 * 3
-    desc, size = ctypes.byref(CrossDesc(s3(*qs[:3]), s3(*ks[:3]), s3(*vs[:3]), s3(*os_[:3]), *fields)), ctypes.c_size_t()
-    check(_lib.load().sengine_amd_cross_attention_workspace(desc, ctypes.byref(size)), "cross_attention")
-    return desc, size.value
-
-
-def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float] = None,
-                    key_lengths: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None,
-                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Attention of q (B, Lq, Hq, d) to an encoder's states k, v (B, Lk, Hkv, d), Hq a multiple of
-    Hkv (query head h reads key head h // (Hq // Hkv)), d a multiple of 8 up to 128; fp16 or bf16;
-    scale 1 / sqrt(d) by default.  Returns (B, Lq, Hq, d) in q's type.
-
-    key_lengths (B,) int32: the keys of each sequence that count (clamped to 0..Lk); key_mask
-    (B, Lk) bool: True where a key counts.  A query with no key that counts gets zeros; what lies
-    in the others is never used.  Any strides whose rows of d values are contiguous and begin at
-    multiples of 16 bytes; k and v expanded over the batch (one encoder pass, many queries) are read
-    as they are."""
+def _cross_plan(key, q, k, v, scale, key_lengths, key_mask, out):
+    """(descriptor, bytes of scratch memory, device) of a checked call."""
     _token_input(q, "q")
     dev, code = q.device, _type_code(q, (torch.float16, torch.bfloat16), "q")
     for t, name in ((k, "k"), (v, "v")):
@@ -1076,9 +1094,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
                            f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, Lq, Hq, d = q.shape
     Lk, Hkv = k.shape[1], k.shape[2]
-    if out is None:
-        out = torch.empty((B, Lq, Hq, d), dtype=q.dtype, device=dev)
-    else:
+    if out is not None:
         if not isinstance(out, torch.Tensor):
             raise TypeError("out must be a torch.Tensor")
         if out.device != dev or out.dtype != q.dtype or out.shape != q.shape:
@@ -1086,11 +1102,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
                                f"{tuple(out.shape)} on {out.device}")
         if out.requires_grad and torch.is_grad_enabled():
             raise SEngineError("out requires a gradient: the token operators are inference only")
-    st = [t.stride() for t in (q, k, v, out)]
-    for t, s, name in zip((q, k, v, out), st, ("q", "k", "v", "out")):
-        if (s[3] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and s[2] % 8 == 0 and t.data_ptr() % 16 == 0) or not t.numel():
-            continue
-        if s[3] != 1 or t.data_ptr() % 16 or any(n > 1 and x % 8 for n, x in zip(t.shape, s[:3])):
+    st = [t.stride() for t in (q, k, v)]
+    st.append(out.stride() if out is not None else (Lq * Hq * d, Hq * d, d, 1))
+    for t, s, name in zip((q, k, v, q if out is None else out), st, ("q", "k", "v", "out")):
+        if t.numel() and ((s[3] != 1 and d > 1) or any(n > 1 and x % 8 for n, x in zip(t.shape, s[:3]))):
             raise SEngineError(f"{name}: rows of d values must be contiguous and begin at multiples of 16 bytes "
                                f"(strides {s})")
     if key_lengths is not None:
@@ -1104,9 +1119,48 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
             raise SEngineError(f"key_mask: expected torch.bool ({B}, {Lk}) with contiguous rows, got "
                                f"{key_mask.dtype} {tuple(key_mask.shape)}")
         ms = key_mask.stride(0)
-    desc, size = _cross_desc(*st, ms, B, Lq, Lk, Hq, Hkv, d, code, 1.0 / math.sqrt(d) if scale is None else scale)
+    s3 = ctypes.c_int64 * 3
+    # a stride over a single element is never taken: 0 keeps it from looking unaligned
+    st = [s3(*(x if n > 1 else 0 for n, x in zip(t.shape[:3], s))) for t, s in zip((q, k, v, q), st)]
+    desc = ctypes.byref(CrossDesc(*st, ms, B, Lq, Lk, Hq, Hkv, d, code, 1.0 / math.sqrt(d) if scale is None else scale))
+    size = ctypes.c_size_t()
+    check(_lib.load().sengine_amd_cross_attention_workspace(desc, ctypes.byref(size)), "cross_attention")
+    return _remember(key, (desc, size.value, dev))
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float] = None,
+                    key_lengths: Optional[torch.Tensor] = None, key_mask: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q (B, Lq, Hq, d) to an encoder's states k, v (B, Lk, Hkv, d), Hq a multiple of
+    Hkv (query head h reads key head h // (Hq // Hkv)), d a multiple of 8 up to 128; fp16 or bf16;
+    scale 1 / sqrt(d) by default.  Returns (B, Lq, Hq, d) in q's type.
+
+    key_lengths (B,) int32: the keys of each sequence that count (clamped to 0..Lk); key_mask
+    (B, Lk) bool: True where a key counts.  A query with no key that counts gets zeros; what lies
+    in the others is never used.  Any strides whose rows of d values are contiguous and begin at
+    multiples of 16 bytes; k and v expanded over the batch (one encoder pass, many queries) are read
+    as they are.  Scores, their maximum and sums are fp32; the weights are rounded to q's type for
+    the product with v.  Few queries of many keys are computed in parts of the keys through scratch
+    memory of torch's allocator, the parts joined in a fixed order."""
+    key = None
+    if out is None:
+        try:
+            key = ("cross", q.dtype, q.shape, q.stride(), q.device, k.dtype, k.shape, k.stride(), k.device, v.dtype,
+                   v.shape, v.stride(), v.device, scale, _layout(key_lengths), _layout(key_mask))
+        except AttributeError:
+            pass  # not a tensor: the checks say so
+    plan = _TOKEN_PLANS.get(key)
+    if plan is None or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        plan = _cross_plan(key, q, k, v, scale, key_lengths, key_mask, out)
+    desc, size, dev = plan
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    if (qp | kp | vp | op) & 15:
+        for p, t, name in ((qp, q, "q"), (kp, k, "k"), (vp, v, "v"), (op, out, "out")):
+            if p & 15 and t.numel():
+                raise SEngineError(f"{name}: must begin at a multiple of 16 bytes")
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     check(_lib.load().sengine_amd_cross_attention_ws(
-        desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(key_lengths), _ptr(key_mask), out.data_ptr(), _ptr(ws),
-        size, _stream(dev)), "cross_attention")
+        desc, qp, kp, vp, _ptr(key_lengths), _ptr(key_mask), op, _ptr(ws), size, _stream(dev)), "cross_attention")
     return out

@@ -92,24 +92,31 @@ static size_t cross_workspace(const sengine_cross_desc* d, int parts) {
   return (size_t)parts * d->B * d->Lq * d->Hq * (d->d + 2) * sizeof(float);
 }
 
-template <class T, int DV, int NW, int QF, int KT, int S, bool SHARED, int WPE>
+template <class T, int DV, int NW, int QF, int KT, bool SHARED, int WPE>
 static hipError_t run_tile(CrossParams& p, hipStream_t stream) {
   p.blocks = (p.rows + (SHARED ? NW : 1) * 16 * QF - 1) / ((SHARED ? NW : 1) * 16 * QF);
-  const int64_t wgs = (int64_t)p.blocks * p.Hkv * p.parts * p.B;
+  // units of all key heads where there are enough of them (heads of 48 values share cache lines), else of one;
+  // in turn over the XCDs unless that would leave some with less (2.5 units against 3 and the like)
+  p.unit_heads = (int64_t)p.B * p.parts >= 32 ? p.Hkv : 1;
+  p.inner = p.blocks * p.unit_heads;
+  const int64_t units = (int64_t)p.B * p.parts * (p.Hkv / p.unit_heads);
+  p.spread = units % 8 == 0 || units >= 64;
+  p.units = (int)units;
+  const int64_t wgs = (p.spread ? (units + 7) / 8 * 8 : units) * p.inner;
   if (wgs > 0x7fffffffll) return hipErrorInvalidValue;
   if (p.mask)
-    cross_tile_kernel<T, DV, NW, QF, KT, S, SHARED, true, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
+    cross_tile_kernel<T, DV, NW, QF, KT, SHARED, true, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
   else
-    cross_tile_kernel<T, DV, NW, QF, KT, S, SHARED, false, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
+    cross_tile_kernel<T, DV, NW, QF, KT, SHARED, false, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
   return hipGetLastError();
 }
 
 template <class T, int DV>
 static hipError_t by_rows(CrossParams& p, int rows_a_block, hipStream_t stream) {
-  if (rows_a_block == 16) return run_tile<T, DV, 4, 1, 32, 2, false, 1>(p, stream);
-  if (rows_a_block == 64) return run_tile<T, DV, 4, 1, 64, 2, true, 2>(p, stream);
-  if (rows_a_block == 128) return run_tile<T, DV, 4, 2, 64, 2, true, 2>(p, stream);
-  return run_tile<T, DV, 8, 2, 64, 2, true, 2>(p, stream);
+  if (rows_a_block == 16) return run_tile<T, DV, 4, 1, 32, false, 1>(p, stream);
+  if (rows_a_block == 64) return run_tile<T, DV, 4, 1, 64, true, 2>(p, stream);
+  if (rows_a_block == 128) return run_tile<T, DV, 4, 2, 64, true, 2>(p, stream);
+  return run_tile<T, DV, 8, 2, 64, true, 2>(p, stream);
 }
 
 template <class T>

@@ -18,10 +18,15 @@
 // LDS: a key's row has PR 16-byte pieces, piece j at place j ^ f(row): 8 lanes that read a piece of 8 rows, and
 // 16 lanes that read 32 bytes of 4 rows, touch every bank once.
 #pragma once
+#include <type_traits>
+
 #include "lds_copy.h"
 #include "token_types.h"
 
 namespace sengine {
+
+using Yes = std::integral_constant<bool, true>;
+using No = std::integral_constant<bool, false>;
 
 struct CrossParams {
   const void *q, *k, *v;
@@ -32,6 +37,7 @@ struct CrossParams {
   int B, Lq, Lk, Hq, Hkv, d;
   float scale;
   int group, rows, blocks;  // rows = Lq * group, in `blocks` row blocks
+  int units, inner, unit_heads, spread;  // the order of the workgroups (cross_tile_kernel)
   int parts;                // parts of the keys; more than one: partial results for the join
   float* part_o;            // [part][sequence, key head, row][d], not divided by the sum
   float* part_ml;           // [part][sequence, key head, row][2]: reference (base 2) and sum
@@ -49,7 +55,7 @@ __device__ __forceinline__ float4_t mma_16(u32x4_t a, u32x4_t b, float4_t c) {
                                                    0, 0, 0);
 }
 
-// Largest / sum of the four lanes l, l ^ 16, l ^ 32, l ^ 48.  A swap exchanges one half (32 lanes, or rows of 16)
+// Largest of the four lanes l, l ^ 16, l ^ 32, l ^ 48.  A swap exchanges one half (32 lanes, or rows of 16)
 // of the first register with the other half of the second, so that of two copies one ends with the lane's own
 // value and the other with its partner's.  It needs two wait states after its operands are written.
 __device__ __forceinline__ float max_of_groups(float x) {
@@ -60,26 +66,21 @@ __device__ __forceinline__ float max_of_groups(float x) {
   asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
   return fmaxf(x, y);
 }
-__device__ __forceinline__ float sum_of_groups(float x) {
-  x += __shfl_xor(x, 32, 64);
-  return x + __shfl_xor(x, 16, 64);
-}
-
-template <class T, int DV, int NW, int QF, int KT, int S, bool SHARED>
+template <class T, int DV, int NW, int QF, int KT, bool SHARED>
 struct CrossTile {
   static constexpr int DK = (DV + 1) / 2;                       // 32-wide steps of q . k
   static constexpr int PR = DK <= 1 ? 4 : DK <= 2 ? 8 : 16;     // pieces of a row in LDS
   static constexpr int kRow = PR * 16, kOperand = KT * kRow, kStage = 2 * kOperand;
   static constexpr int kAllCopies = 2 * KT * PR / 64;
   static constexpr int kCopies = SHARED ? kAllCopies / NW : kAllCopies;  // of a wave a tile
-  static constexpr int kLds = (SHARED ? 1 : NW) * S * kStage;
+  static constexpr int kLds = (SHARED ? 1 : NW) * 2 * kStage;
   static_assert(kAllCopies % (SHARED ? NW : 1) == 0 && KT % 32 == 0, "tile");
   static_assert(SHARED || NW * 64 * DV * 16 <= kLds, "the waves' results fit");
 };
 
-template <class T, int DV, int NW, int QF, int KT, int S, bool SHARED, bool LIST, int WPE>
+template <class T, int DV, int NW, int QF, int KT, bool SHARED, bool LIST, int WPE>
 __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p) {
-  using C = CrossTile<T, DV, NW, QF, KT, S, SHARED>;
+  using C = CrossTile<T, DV, NW, QF, KT, SHARED>;
   constexpr int DK = C::DK, PR = C::PR, NK = KT / 16;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[C::kLds];
   __shared__ uint16_t list[LIST ? kCrossList : 1];
@@ -89,13 +90,26 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
 
-  // workgroup -> row block, key head, part, sequence: neighbours on an XCD share a sequence's rows of memory
-  int id = xcd_order((int)blockIdx.x, (int)gridDim.x);
-  const int block = id % p.blocks;
-  id /= p.blocks;
-  const int kh = id % p.Hkv;
-  id /= p.Hkv;
-  const int part = id % p.parts, b = id / p.parts;
+  // workgroup -> unit (sequence, part of the keys, one key head or all) and place in it (row block, key head).
+  // Workgroups go to the eight XCDs in turn: a unit stays on one, whose L2 then holds what its workgroups share,
+  // and neighbouring units, which are of one sequence and so of one length, go to different ones.
+  int unit, in;
+  if (p.spread) {
+    const int local = (int)blockIdx.x >> 3;
+    unit = ((int)blockIdx.x & 7) + 8 * (local / p.inner);
+    in = local % p.inner;
+    if (unit >= p.units) return;
+  } else {
+    unit = (int)blockIdx.x / p.inner;
+    in = (int)blockIdx.x % p.inner;
+  }
+  const int block = in % p.blocks;
+  int kh = in / p.blocks;
+  if (p.unit_heads == 1) {
+    kh = unit % p.Hkv;
+    unit /= p.Hkv;
+  }
+  const int part = unit % p.parts, b = unit / p.parts;
 
   int n = p.Lk;
   if (p.lengths) {
@@ -129,16 +143,19 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
   }
 
   float4_t o[DV][QF];
-  float top[QF], total[QF];
+  float top[QF];
+  float4_t total[QF];  // the sum of the weights, the same in all four, from a product with ones: of what V is multiplied by
 #pragma unroll
   for (int f = 0; f < QF; ++f) {
     top[f] = -INFINITY;
-    total[f] = 0.f;
+    total[f] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < DV; ++i) o[i][f] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  uint8_t* ring = smem + (SHARED ? 0 : wave * S * C::kStage);
+  const uint32_t one2 = __is_same(T, _Float16) ? 0x3c003c00u : 0x3f803f80u;
+  const u32x4_t ones = u32x4_t{one2, one2, one2, one2};
+  uint8_t* ring = smem + (SHARED ? 0 : wave * 2 * C::kStage);
   const uint32_t ring0 = lds_offset(ring);
   const uint8_t* kbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.k) + b * p.k_b + kh * p.k_h);
   const uint8_t* vbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.v) + b * p.v_b + kh * p.v_h);
@@ -154,6 +171,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
     vat[f] = C::kOperand + (4 * g + (c >> 2)) * C::kRow + (((2 * f + ((c >> 1) & 1)) ^ (2 * x)) << 4) + (c & 1) * 8;
   }
 
+  // All keys.  LATE waves do a tile's exponentials before its neighbour's products, the others after.
+  const auto run = [&](auto late) {
+  constexpr bool LATE = decltype(late)::value;
   for (int c0 = k0; c0 < k1;) {
     // the keys of this stretch: a list of those that count, or all
     int cnt = k1 - c0, cn = cnt;
@@ -189,63 +209,95 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
       __syncthreads();
     }
     const int tiles = (cnt + KT - 1) / KT;
-    // copies of tile t into stage s of the ring; past the last tile they fetch nothing
-    const auto copy = [&](int t, int s) {
-      const int64_t j0 = LIST ? c0 : c0 + (int64_t)t * KT;
-      const uint8_t *ka = kbase + j0 * kst, *va = vbase + j0 * vst;
+    // This wave's copies: K of tile tk and V of tile tv, into the stages of
+    // parity sk and sv.  Places past the
+    // last key, and tiles past the last, fetch nothing.
+    int off[C::kCopies];
+    const auto is_v = [&](int j) { return (SHARED ? wave * C::kCopies + j : j) >= C::kAllCopies / 2; };
+    const auto locate = [&](int tk, int tv) {
+#pragma unroll
+      for (int j = 0; j < C::kCopies; ++j) {
+        const int qq = SHARED ? wave * C::kCopies + j : j;
+        const bool v = is_v(j);
+        const int row = (v ? qq - C::kAllCopies / 2 : qq) * (64 / PR) + lane / PR;
+        const int sw = v ? (PR == 4 ? (row >> 1 & 1) * 2 : (row & 3) * 2) : (PR == 4 ? row >> 1 & 3 : row & 7);
+        const int piece = (lane % PR) ^ sw, at = (v ? tv : tk) * KT + row;
+        const bool in = at < cnt && piece * 8 < p.d;
+        int key = row;
+        if constexpr (LIST) key = in ? list[at] : 0;
+        off[j] = in ? key * (v ? vst : kst) + piece * 16 : 0x7fffff00;
+      }
+    };
+    const auto copy = [&](int tk, int tv, int sk, int sv) {
+      const uint8_t* ka = kbase + (LIST ? c0 : c0 + (int64_t)tk * KT) * kst;
+      const uint8_t* va = vbase + (LIST ? c0 : c0 + (int64_t)tv * KT) * vst;
       const u32x4_t kr = row_buffer(ka, 0x7fff0000), vr = row_buffer(va, 0x7fff0000);
 #pragma unroll
       for (int j = 0; j < C::kCopies; ++j) {
         const int qq = SHARED ? wave * C::kCopies + j : j;
-        const bool isv = qq >= C::kAllCopies / 2;
-        const int qo = isv ? qq - C::kAllCopies / 2 : qq;
-        const int row = qo * (64 / PR) + lane / PR;
-        const int sw = isv ? (PR == 4 ? (row >> 1 & 1) * 2 : (row & 3) * 2) : (PR == 4 ? row >> 1 & 3 : row & 7);
-        const int piece = (lane % PR) ^ sw;
-        const bool in = t * KT + row < cnt && piece * 8 < p.d;
-        int key = row;
-        if constexpr (LIST) key = in ? list[t * KT + row] : 0;
-        const int off = key * (isv ? vst : kst) + piece * 16;
+        const bool v = is_v(j);
         u32x4_t r = kr;
         if constexpr (SHARED) {
-          r[0] = scalar(isv ? vr[0] : kr[0]);
-          r[1] = scalar(isv ? vr[1] : kr[1]);
+          r[0] = scalar(v ? vr[0] : kr[0]);
+          r[1] = scalar(v ? vr[1] : kr[1]);
         } else {
-          r = isv ? vr : kr;
+          r = v ? vr : kr;
         }
-        lds_copy(r, ring0 + s * C::kStage + qq * 1024, in ? off : 0x7fffff00);
+        lds_copy(r, ring0 + ((v ? sv : sk) & 1) * C::kStage + qq * 1024, off[j]);
       }
     };
-    const int step = SHARED ? 1 : NW;
-    int t = SHARED ? 0 : wave;
+    float4_t s[NK][QF];
+    u32x4_t pr[KT / 32][QF];
+    // O and the sum take on tile tv's weights and values (V), then the scores of tile tk are formed (K); either may be
+    // left out.  Each fragment's operand is read while the products of the one before are made, and no earlier: read
+    // further ahead they would not fit the registers.
+    const auto products = [&](auto V, int tv, auto K, int tk) {
+      constexpr int NVG = decltype(V)::value ? DV : 0, NG = NVG + (decltype(K)::value ? NK : 0);
+      const uint8_t *va = ring + (tv & 1) * C::kStage, *ka = ring + (tk & 1) * C::kStage;
+      u32x4_t vf[2][KT / 32], kf[2][DK];
+      const auto read = [&](int n) {
+        if (n < NVG) {
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) copy(t + s * step, s);
-    int stage = 0;
-    for (; t < tiles; t += step) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"i"((S - 2) * C::kCopies) : "memory");
-      if constexpr (SHARED) {  // every wave's copies of this tile have landed, and none reads the stage before
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-      }
-      {
-        const int fill = stage == 0 ? S - 1 : stage - 1;
-        copy(t + (S - 1) * step, fill);
-      }
-      const uint8_t* at = ring + stage * C::kStage;
-      stage = stage + 1 == S ? 0 : stage + 1;
-
-      float4_t s[NK][QF];
+          for (int u = 0; u < KT / 32; ++u) {
+            const uint8_t* at = va + vat[n & 3] + (n >> 2) * 128 + u * 32 * C::kRow;
+            vf[n & 1][u] = read_transposed(at, at + 16 * C::kRow);
+          }
+        } else if (n < NG) {
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-#pragma unroll
-        for (int f = 0; f < QF; ++f) s[i][f] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < DK; ++u) {
-          const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(at + i * 16 * C::kRow + kat[u]);
-#pragma unroll
-          for (int f = 0; f < QF; ++f) s[i][f] = mma_16<T>(kf, q[f][u], s[i][f]);
+          for (int u = 0; u < DK; ++u)
+            kf[n & 1][u] = *reinterpret_cast<const u32x4_t*>(ka + (n - NVG) * 16 * C::kRow + kat[u]);
         }
+      };
+      read(0);
+      if constexpr (NVG > 0) {
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+          for (int f = 0; f < QF; ++f) total[f] = mma_16<T>(ones, pr[u][f], total[f]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        read(n + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (n < NVG) {
+#pragma unroll
+          for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+            for (int f = 0; f < QF; ++f) o[n][f] = mma_16<T>(vf[n & 1][u], pr[u][f], o[n][f]);
+        } else {
+          const int i = n - NVG;
+#pragma unroll
+          for (int f = 0; f < QF; ++f) s[i][f] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int u = 0; u < DK; ++u)
+#pragma unroll
+            for (int f = 0; f < QF; ++f) s[i][f] = mma_16<T>(kf[n & 1][u], q[f][u], s[i][f]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    const auto weights = [&](int t) {
       const int left = cnt - t * KT;
       if (left < KT) {
 #pragma unroll
@@ -261,10 +313,18 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
       bool raise = false;
 #pragma unroll
       for (int f = 0; f < QF; ++f) {
-        high[f] = fmaxf(fmaxf(s[0][f][0], s[0][f][1]), fmaxf(s[0][f][2], s[0][f][3]));
-#pragma unroll
-        for (int i = 1; i < NK; ++i)
-          high[f] = fmaxf(high[f], fmaxf(fmaxf(s[i][f][0], s[i][f][1]), fmaxf(s[i][f][2], s[i][f][3])));
+        high[f] = fmaxf(fmaxf(s[0][f][0], s[0][f][1]), s[0][f][2]);  // three at a time
+        high[f] = fmaxf(fmaxf(s[0][f][3], s[1][f][0]), high[f]);
+        high[f] = fmaxf(fmaxf(s[1][f][1], s[1][f][2]), high[f]);
+        if constexpr (NK == 2) {
+          high[f] = fmaxf(s[1][f][3], high[f]);
+        } else {
+          high[f] = fmaxf(fmaxf(s[1][f][3], s[2][f][0]), high[f]);
+          high[f] = fmaxf(fmaxf(s[2][f][1], s[2][f][2]), high[f]);
+          high[f] = fmaxf(fmaxf(s[2][f][3], s[3][f][0]), high[f]);
+          high[f] = fmaxf(fmaxf(s[3][f][1], s[3][f][2]), high[f]);
+          high[f] = fmaxf(s[3][f][3], high[f]);
+        }
         high[f] = max_of_groups(high[f]) * cs;
         raise |= high[f] > top[f] + 8.f;
       }
@@ -281,7 +341,6 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
             for (int e = 0; e < 4; ++e) o[i][f][e] *= back;
         }
       }
-      u32x4_t pr[KT / 32][QF];
 #pragma unroll
       for (int f = 0; f < QF; ++f) {
         const float ref = top[f] == -INFINITY ? 0.f : -top[f];  // every score so far is -infinity: they weigh nothing
@@ -290,45 +349,81 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
           typedef T vec8_t __attribute__((ext_vector_type(8)));
           vec8_t x;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * u + e / 4][f][e % 4], cs, ref));
-            total[f] += w;
-            x[e] = (T)w;
-          }
+          for (int e = 0; e < 8; ++e)
+            x[e] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * u + e / 4][f][e % 4], cs, ref));
           pr[u][f] = __builtin_bit_cast(u32x4_t, x);
         }
       }
-#pragma unroll
-      for (int i = 0; i < DV; ++i) {
-#pragma unroll
-        for (int u = 0; u < KT / 32; ++u) {
-          const uint8_t* va = at + vat[i & 3] + (i >> 2) * 128 + u * 32 * C::kRow;
-          const u32x4_t vf = read_transposed(va, va + 16 * C::kRow);
-#pragma unroll
-          for (int f = 0; f < QF; ++f) o[i][f] = mma_16<T>(vf, pr[u][f], o[i][f]);
+    };
+    if constexpr (SHARED) {
+      // Between meetings t and t + 1 the waves need K of tile t and V of tile t - 1, which meeting t finds landed,
+      // and K of t + 1 and V of t are on their way.  The later half of eight waves, which share the SIMDs with the
+      // earlier half, does its exponentials first and its products after, so that one half's vector work goes with
+      // the other's matrix work.
+      const auto meet = [&](int t) {
+        locate(t + 1, t);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        copy(t + 1, t, t + 1, t);
+      };
+      if (tiles > 0) {
+        locate(0, tiles);
+        copy(0, tiles, 0, 1);  // no V yet: a tile past the last
+        meet(0);
+        products(No{}, 0, Yes{}, 0);
+        if (!LATE) weights(0);
+        for (int t = 1; t < tiles; ++t) {
+          meet(t);
+          if (LATE) weights(t - 1);
+          products(Yes{}, t - 1, Yes{}, t);
+          if (!LATE) weights(t);
         }
+        meet(tiles);
+        if (LATE) weights(tiles - 1);
+        products(Yes{}, tiles - 1, No{}, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end
       }
-      // this wave's reads of the stage are done before it may be filled again
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __syncthreads();
+    } else {
+      // tile i of this wave is tile wave + i * NW of the stretch
+      const int own = (tiles - wave + NW - 1) / NW;
+      const auto fetch = [&](int i) {
+        locate(wave + i * NW, wave + i * NW);
+        copy(wave + i * NW, wave + i * NW, i, i);
+      };
+      if (own > 0) fetch(0);
+      for (int i = 0; i < own; ++i) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        fetch(i + 1);
+        products(No{}, 0, Yes{}, i);
+        weights(wave + i * NW);
+        products(Yes{}, i, No{}, 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is read before it is filled again
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end
-    if constexpr (SHARED) __syncthreads();
     c0 += cn;
   }
+  };
+  // (code of its own for each half: branches inside the loop would move the sums between registers)
+  if (SHARED && NW == 8 && wave >= 4)
+    run(Yes{});
+  else
+    run(No{});
 
   if constexpr (!SHARED) {
     static_assert(QF == 1, "one fragment of rows");
     // join the waves: a common reference, sums and rows of O added up in the waves' order
-    total[0] = sum_of_groups(total[0]);
     if (g == 0) {
       joint[wave][0][c] = top[0];
-      joint[wave][1][c] = total[0];
+      joint[wave][1][c] = total[0][0];
     }
     __syncthreads();
     float t1 = joint[0][0][c];
 #pragma unroll
     for (int w = 1; w < NW; ++w) t1 = fmaxf(t1, joint[w][0][c]);
-    const float back = top[0] == -INFINITY ? (total[0] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(top[0] - t1);
+    const float back = top[0] == -INFINITY ? (total[0][0] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(top[0] - t1);
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
@@ -336,7 +431,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
       sum += joint[w][1][c] * (tw == -INFINITY ? (joint[w][1][c] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(tw - t1));
     }
     top[0] = t1;
-    total[0] = sum;
+    total[0][0] = sum;
     float4_t* mine = reinterpret_cast<float4_t*>(smem) + wave * DV * 64 + lane;
 #pragma unroll
     for (int i = 0; i < DV; ++i) mine[i * 64] = o[i][0] * back;
@@ -349,9 +444,6 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
 #pragma unroll
       for (int w = 1; w < NW; ++w) o[i][0] += all[w * DV * 64];
     }
-  } else {
-#pragma unroll
-    for (int f = 0; f < QF; ++f) total[f] = sum_of_groups(total[f]);
   }
 #pragma unroll
   for (int f = 0; f < QF; ++f) {
@@ -361,14 +453,14 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
       const int64_t r = (((int64_t)part * p.B + b) * p.Hkv + kh) * p.rows + row;
       if (g == 0 && (SHARED || wave == 0)) {
         p.part_ml[2 * r] = top[f];
-        p.part_ml[2 * r + 1] = total[f];
+        p.part_ml[2 * r + 1] = total[f][0];
       }
 #pragma unroll
       for (int i = 0; i < DV; ++i)
         if ((SHARED || i % NW == wave) && 16 * i + 4 * g < p.d)
           *reinterpret_cast<float4_t*>(p.part_o + r * p.d + 16 * i + 4 * g) = o[i][f];
     } else {
-      const float inv = total[f] == 0.f ? 0.f : 1.f / total[f];
+      const float inv = total[f][0] == 0.f ? 0.f : 1.f / total[f][0];
       T* out = static_cast<T*>(p.out) + b * p.o_b + (row / p.group) * p.o_l + (kh * p.group + row % p.group) * p.o_h;
 #pragma unroll
       for (int i = 0; i < DV; ++i)

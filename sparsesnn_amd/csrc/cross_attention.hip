@@ -70,19 +70,21 @@ __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
 }
 
 struct CrossPlan {
-  int rows_a_block;  // 0: the row kernel
+  int rows_a_block;
+  int heads;  // key heads of a workgroup
   int parts;
 };
 
 static CrossPlan plan(const sengine_cross_desc* d) {
-  const int64_t heads = (int64_t)d->B * d->Hkv, rows = (int64_t)d->Lq * (d->Hq / d->Hkv);
-  CrossPlan q{rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256, 1};
-  const int64_t wgs = heads * ((rows + q.rows_a_block - 1) / q.rows_a_block);
+  const int64_t rows = (int64_t)d->Lq * (d->Hq / d->Hkv);
+  CrossPlan q{rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256, 1, 1};
+  if (rows <= 64 && d->d <= 48 && d->d % 16 == 0 && d->Hkv % 4 == 0 && d->k_stride[2] == d->d && d->v_stride[2] == d->d) q.heads = 4;
+  const int64_t wgs = (int64_t)d->B * (d->Hkv / q.heads) * ((rows + q.rows_a_block - 1) / q.rows_a_block);
   const int64_t want = q.rows_a_block == 16 ? 1024 : 512, least = q.rows_a_block == 16 ? 256 : 512;
   if (wgs * 2 <= want) {
     int64_t parts = want / wgs;
     if (parts > d->Lk / least) parts = d->Lk / least;
-    if (parts > 64) parts = 64;
+    if (parts > kCrossParts) parts = kCrossParts;
     if (parts > 1) q.parts = (int)parts;
   }
   return q;
@@ -92,52 +94,57 @@ static size_t cross_workspace(const sengine_cross_desc* d, int parts) {
   return (size_t)parts * d->B * d->Lq * d->Hq * (d->d + 2) * sizeof(float);
 }
 
-template <class T, int DV, int NW, int QF, int KT, bool SHARED, int WPE>
+template <class T, int DV, int NW, int QF, int KT, int S, int HPW, bool SHARED, int WPE>
 static hipError_t run_tile(CrossParams& p, hipStream_t stream) {
-  p.blocks = (p.rows + (SHARED ? NW : 1) * 16 * QF - 1) / ((SHARED ? NW : 1) * 16 * QF);
+  constexpr int R = (SHARED ? NW / HPW : 1) * 16 * QF;
+  p.blocks = (p.rows + R - 1) / R;
   // units of all key heads where there are enough of them (heads of 48 values share cache lines), else of one;
   // in turn over the XCDs unless that would leave some with less (2.5 units against 3 and the like)
-  p.unit_heads = (int64_t)p.B * p.parts >= 32 ? p.Hkv : 1;
+  p.unit_heads = (int64_t)p.B * p.parts >= 32 ? p.Hkv / HPW : 1;
   p.inner = p.blocks * p.unit_heads;
-  const int64_t units = (int64_t)p.B * p.parts * (p.Hkv / p.unit_heads);
+  const int64_t units = (int64_t)p.B * p.parts * (p.Hkv / HPW / p.unit_heads);
   p.spread = units % 8 == 0 || units >= 64;
   p.units = (int)units;
   const int64_t wgs = (p.spread ? (units + 7) / 8 * 8 : units) * p.inner;
   if (wgs > 0x7fffffffll) return hipErrorInvalidValue;
   if (p.mask)
-    cross_tile_kernel<T, DV, NW, QF, KT, SHARED, true, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
+    cross_tile_kernel<T, DV, NW, QF, KT, S, HPW, SHARED, true, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
   else
-    cross_tile_kernel<T, DV, NW, QF, KT, SHARED, false, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
+    cross_tile_kernel<T, DV, NW, QF, KT, S, HPW, SHARED, false, WPE><<<dim3((unsigned)wgs), dim3(64 * NW), 0, stream>>>(p);
   return hipGetLastError();
 }
 
 template <class T, int DV>
-static hipError_t by_rows(CrossParams& p, int rows_a_block, hipStream_t stream) {
-  if (rows_a_block == 16) return run_tile<T, DV, 4, 1, 32, false, 1>(p, stream);
-  if (rows_a_block == 64) return run_tile<T, DV, 4, 1, 64, true, 2>(p, stream);
-  if (rows_a_block == 128) return run_tile<T, DV, 4, 2, 64, true, 2>(p, stream);
-  return run_tile<T, DV, 8, 2, 64, true, 2>(p, stream);
+static hipError_t by_rows(CrossParams& p, const CrossPlan& q, hipStream_t stream) {
+  if constexpr (DV < 4) {
+    if (q.heads == 4 && q.rows_a_block == 16) return run_tile<T, DV, 4, 1, 32, 3, 4, true, 1>(p, stream);
+    if (q.heads == 4) return run_tile<T, DV, 8, 2, 32, 3, 4, true, 2>(p, stream);
+  }
+  if (q.rows_a_block == 16) return run_tile<T, DV, 4, 1, 32, 2, 1, false, 1>(p, stream);
+  if (q.rows_a_block == 64) return run_tile<T, DV, 4, 1, 64, 2, 1, true, 2>(p, stream);
+  if (q.rows_a_block == 128) return run_tile<T, DV, 4, 2, 64, 2, 1, true, 2>(p, stream);
+  return run_tile<T, DV, 8, 2, 64, 2, 1, true, 2>(p, stream);
 }
 
 template <class T>
-static hipError_t by_width(CrossParams& p, int rows_a_block, hipStream_t stream) {
+static hipError_t by_width(CrossParams& p, const CrossPlan& q, hipStream_t stream) {
   const int dv = (p.d + 15) / 16;
   hipError_t e;
   if (dv <= 1)
-    e = by_rows<T, 1>(p, rows_a_block, stream);
+    e = by_rows<T, 1>(p, q, stream);
   else if (dv <= 2)
-    e = by_rows<T, 2>(p, rows_a_block, stream);
+    e = by_rows<T, 2>(p, q, stream);
   else if (dv <= 3)
-    e = by_rows<T, 3>(p, rows_a_block, stream);
+    e = by_rows<T, 3>(p, q, stream);
   else if (dv <= 4)
-    e = by_rows<T, 4>(p, rows_a_block, stream);
+    e = by_rows<T, 4>(p, q, stream);
   else if (dv <= 6)
-    e = by_rows<T, 6>(p, rows_a_block, stream);
+    e = by_rows<T, 6>(p, q, stream);
   else
-    e = by_rows<T, 8>(p, rows_a_block, stream);
+    e = by_rows<T, 8>(p, q, stream);
   if (e != hipSuccess || p.parts == 1) return e;
   const int64_t rows = (int64_t)p.B * p.Hkv * p.rows;
-  cross_join_kernel<T><<<dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, stream>>>(p);
+  cross_join_kernel<T><<<dim3((unsigned)rows), dim3(64), 0, stream>>>(p);
   return hipGetLastError();
 }
 
@@ -188,8 +195,8 @@ extern "C" int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const
     if (p.parts > 1 && (!workspace || workspace_bytes < cross_workspace(d, p.parts))) p.parts = 1;
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + (int64_t)p.parts * p.B * p.Hkv * p.rows * p.d;
-    return (int)(d->type == SENGINE_ENC_F16 ? by_width<_Float16>(p, plan_.rows_a_block, stream)
-                                            : by_width<__bf16>(p, plan_.rows_a_block, stream));
+    return (int)(d->type == SENGINE_ENC_F16 ? by_width<_Float16>(p, plan_, stream)
+                                            : by_width<__bf16>(p, plan_, stream));
   }
   const dim3 grid((unsigned)((int64_t)d->B * d->Lq * d->Hq));
   if (d->type == SENGINE_ENC_F16)

@@ -9,7 +9,9 @@
 //                lanes is free as long as V's operand, read from LDS transposed, has the same
 // K and V are copied into LDS by buffer loads, S tiles in flight.  SHARED: all waves work on the same tile
 // and meet once a tile; otherwise (few rows) each wave has tiles and LDS of its own, takes every NW-th tile,
-// never meets the others, and their results are joined at the end.
+// never meets the others, and their results are joined at the end.  Where a head's row is not whole cache lines and the
+// heads lie side by side, HPW key heads share a workgroup and their rows are copied as one: a line that two heads
+// share is fetched once (alone they fetched 1.67 times the bytes at d = 48).
 //
 // A mask is turned into a list of the keys that count, 4096 keys at a time, and only those are fetched: what
 // does not count is neither read nor multiplied.  Places of the last tile past the end are filled with zeros
@@ -66,21 +68,24 @@ __device__ __forceinline__ float max_of_groups(float x) {
   asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(x), "+v"(y));
   return fmaxf(x, y);
 }
-template <class T, int DV, int NW, int QF, int KT, bool SHARED>
+template <class T, int DV, int NW, int QF, int KT, int S, int HPW, bool SHARED>
 struct CrossTile {
   static constexpr int DK = (DV + 1) / 2;                       // 32-wide steps of q . k
-  static constexpr int PR = DK <= 1 ? 4 : DK <= 2 ? 8 : 16;     // pieces of a row in LDS
+  static constexpr bool MERGED = HPW > 1;                       // a row is that of HPW neighbouring heads, d = 16 DV
+  static constexpr int PR = MERGED ? HPW * DV * 2 : DK <= 1 ? 4 : DK <= 2 ? 8 : 16;  // pieces of a row in LDS
   static constexpr int kRow = PR * 16, kOperand = KT * kRow, kStage = 2 * kOperand;
   static constexpr int kAllCopies = 2 * KT * PR / 64;
+  static constexpr int WPH = SHARED ? NW / HPW : 1;  // waves, each with rows of its own, of a key head
   static constexpr int kCopies = SHARED ? kAllCopies / NW : kAllCopies;  // of a wave a tile
-  static constexpr int kLds = (SHARED ? 1 : NW) * 2 * kStage;
-  static_assert(kAllCopies % (SHARED ? NW : 1) == 0 && KT % 32 == 0, "tile");
-  static_assert(SHARED || NW * 64 * DV * 16 <= kLds, "the waves' results fit");
+  static constexpr int kLds = (SHARED ? 1 : NW) * S * kStage;
+  static_assert(kAllCopies % (SHARED ? NW : 1) == 0 && KT % 32 == 0 && KT * PR % 64 == 0, "tile");
+  static_assert(!MERGED || (PR % 8 == 0 && DV <= 4), "merged rows");
+  static_assert(SHARED || (HPW == 1 && NW * 64 * DV * 16 <= kLds), "the waves' results fit");
 };
 
-template <class T, int DV, int NW, int QF, int KT, bool SHARED, bool LIST, int WPE>
+template <class T, int DV, int NW, int QF, int KT, int S, int HPW, bool SHARED, bool LIST, int WPE>
 __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p) {
-  using C = CrossTile<T, DV, NW, QF, KT, SHARED>;
+  using C = CrossTile<T, DV, NW, QF, KT, S, HPW, SHARED>;
   constexpr int DK = C::DK, PR = C::PR, NK = KT / 16;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[C::kLds];
   __shared__ uint16_t list[LIST ? kCrossList : 1];
@@ -106,9 +111,11 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
   const int block = in % p.blocks;
   int kh = in / p.blocks;
   if (p.unit_heads == 1) {
-    kh = unit % p.Hkv;
-    unit /= p.Hkv;
+    kh = unit % (p.Hkv / HPW);
+    unit /= p.Hkv / HPW;
   }
+  const int kh0 = kh * HPW, hw = SHARED ? wave / C::WPH : 0;  // the workgroup's first key head, the wave's place
+  kh = kh0 + hw;
   const int part = unit % p.parts, b = unit / p.parts;
 
   int n = p.Lk;
@@ -122,7 +129,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
   const int k1 = kend < n ? (int)kend : n;
 
   // the rows' queries as matrix operands; a negative scale goes into their sign
-  const int row0 = (block * (SHARED ? NW : 1) + (SHARED ? wave : 0)) * 16 * QF;
+  const int row0 = (block * C::WPH + (SHARED ? wave % C::WPH : 0)) * 16 * QF;
   u32x4_t q[QF][DK];
   const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
   const float cs = fabsf(p.scale) * 1.4426950408889634f;
@@ -155,20 +162,22 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
 
   const uint32_t one2 = __is_same(T, _Float16) ? 0x3c003c00u : 0x3f803f80u;
   const u32x4_t ones = u32x4_t{one2, one2, one2, one2};
-  uint8_t* ring = smem + (SHARED ? 0 : wave * 2 * C::kStage);
+  uint8_t* ring = smem + (SHARED ? 0 : wave * S * C::kStage);
   const uint32_t ring0 = lds_offset(ring);
-  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.k) + b * p.k_b + kh * p.k_h);
-  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.v) + b * p.v_b + kh * p.v_h);
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.k) + b * p.k_b + kh0 * p.k_h);
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.v) + b * p.v_b + kh0 * p.v_h);
   const int kst = (int)p.k_l * 2, vst = (int)p.v_l * 2;  // bytes between keys
   // where this lane reads K fragments and transposed V fragments
-  const int ksw = PR == 4 ? (c >> 1) & 3 : c & 7;
+  const int ksw = PR == 4 ? (c >> 1) & 3 : c & 7, hp = C::MERGED ? hw * DV * 2 : 0;  // hp: the head's first piece
+  constexpr bool HALF = C::MERGED && DV % 2 == 1;  // the last step of q . k has 16 values: the rest is another head's
   int kat[DK], vat[DV < 4 ? DV : 4];
 #pragma unroll
-  for (int t = 0; t < DK; ++t) kat[t] = c * C::kRow + (((4 * t + g) ^ ksw) << 4);
+  for (int t = 0; t < DK; ++t)
+    kat[t] = c * C::kRow + (((hp + 4 * t + (HALF && t == DK - 1 ? g & 1 : g)) ^ ksw) << 4);
 #pragma unroll
   for (int f = 0; f < (DV < 4 ? DV : 4); ++f) {
     const int x = PR == 4 ? (c >> 3) & 1 : c >> 2;
-    vat[f] = C::kOperand + (4 * g + (c >> 2)) * C::kRow + (((2 * f + ((c >> 1) & 1)) ^ (2 * x)) << 4) + (c & 1) * 8;
+    vat[f] = C::kOperand + (4 * g + (c >> 2)) * C::kRow + (((hp + 2 * f + ((c >> 1) & 1)) ^ (2 * x)) << 4) + (c & 1) * 8;
   }
 
   // All keys.  LATE waves do a tile's exponentials before its neighbour's products, the others after.
@@ -209,20 +218,19 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
       __syncthreads();
     }
     const int tiles = (cnt + KT - 1) / KT;
-    // This wave's copies: K of tile tk and V of tile tv, into the stages of
-    // parity sk and sv.  Places past the
-    // last key, and tiles past the last, fetch nothing.
+    // This wave's copies: K of tile tk and V of tile tv, into stages sk and sv.  Places past the last key, and tiles
+    // past the last or before the first, fetch nothing.
     int off[C::kCopies];
-    const auto is_v = [&](int j) { return (SHARED ? wave * C::kCopies + j : j) >= C::kAllCopies / 2; };
+    const auto number = [&](int j) { return SHARED ? wave * C::kCopies + j : j; };
+    const auto is_v = [&](int j) { return number(j) >= C::kAllCopies / 2; };
     const auto locate = [&](int tk, int tv) {
 #pragma unroll
       for (int j = 0; j < C::kCopies; ++j) {
-        const int qq = SHARED ? wave * C::kCopies + j : j;
         const bool v = is_v(j);
-        const int row = (v ? qq - C::kAllCopies / 2 : qq) * (64 / PR) + lane / PR;
+        const int place = number(j) % (C::kAllCopies / 2) * 64 + lane, row = place / PR;
         const int sw = v ? (PR == 4 ? (row >> 1 & 1) * 2 : (row & 3) * 2) : (PR == 4 ? row >> 1 & 3 : row & 7);
-        const int piece = (lane % PR) ^ sw, at = (v ? tv : tk) * KT + row;
-        const bool in = at < cnt && piece * 8 < p.d;
+        const int piece = (place % PR) ^ sw, at = (v ? tv : tk) * KT + row;
+        const bool in = (unsigned)at < (unsigned)cnt && (C::MERGED || piece * 8 < p.d);
         int key = row;
         if constexpr (LIST) key = in ? list[at] : 0;
         off[j] = in ? key * (v ? vst : kst) + piece * 16 : 0x7fffff00;
@@ -231,29 +239,21 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
     const auto copy = [&](int tk, int tv, int sk, int sv) {
       const uint8_t* ka = kbase + (LIST ? c0 : c0 + (int64_t)tk * KT) * kst;
       const uint8_t* va = vbase + (LIST ? c0 : c0 + (int64_t)tv * KT) * vst;
-      const u32x4_t kr = row_buffer(ka, 0x7fff0000), vr = row_buffer(va, 0x7fff0000);
 #pragma unroll
       for (int j = 0; j < C::kCopies; ++j) {
-        const int qq = SHARED ? wave * C::kCopies + j : j;
         const bool v = is_v(j);
-        u32x4_t r = kr;
-        if constexpr (SHARED) {
-          r[0] = scalar(v ? vr[0] : kr[0]);
-          r[1] = scalar(v ? vr[1] : kr[1]);
-        } else {
-          r = v ? vr : kr;
-        }
-        lds_copy(r, ring0 + ((v ? sv : sk) & 1) * C::kStage + qq * 1024, off[j]);
+        const u32x4_t r = row_buffer(v ? va : ka, 0x7fff0000);
+        lds_copy(r, scalar(ring0 + (v ? sv : sk) * C::kStage + number(j) * 1024), off[j]);
       }
     };
     float4_t s[NK][QF];
     u32x4_t pr[KT / 32][QF];
-    // O and the sum take on tile tv's weights and values (V), then the scores of tile tk are formed (K); either may be
+    // O and the sum take on the weights and stage sv's values (V), then the scores of stage sk are formed (K); either may be
     // left out.  Each fragment's operand is read while the products of the one before are made, and no earlier: read
     // further ahead they would not fit the registers.
-    const auto products = [&](auto V, int tv, auto K, int tk) {
+    const auto products = [&](auto V, int sv, auto K, int sk) {
       constexpr int NVG = decltype(V)::value ? DV : 0, NG = NVG + (decltype(K)::value ? NK : 0);
-      const uint8_t *va = ring + (tv & 1) * C::kStage, *ka = ring + (tk & 1) * C::kStage;
+      const uint8_t *va = ring + sv * C::kStage, *ka = ring + sk * C::kStage;
       u32x4_t vf[2][KT / 32], kf[2][DK];
       const auto read = [&](int n) {
         if (n < NVG) {
@@ -287,6 +287,10 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
             for (int f = 0; f < QF; ++f) o[n][f] = mma_16<T>(vf[n & 1][u], pr[u][f], o[n][f]);
         } else {
           const int i = n - NVG;
+          if constexpr (HALF) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) kf[n & 1][DK - 1][e] = g < 2 ? kf[n & 1][DK - 1][e] : 0;
+          }
 #pragma unroll
           for (int f = 0; f < QF; ++f) s[i][f] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -356,50 +360,63 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
       }
     };
     if constexpr (SHARED) {
-      // Between meetings t and t + 1 the waves need K of tile t and V of tile t - 1, which meeting t finds landed,
-      // and K of t + 1 and V of t are on their way.  The later half of eight waves, which share the SIMDs with the
-      // earlier half, does its exponentials first and its products after, so that one half's vector work goes with
-      // the other's matrix work.
+      // Between meetings t and t + 1 the waves need K of tile t and V of tile t - 1, which meeting t finds landed;
+      // K up to t + S - 1 and V up to t + S - 2 are on their way.  The later half of eight waves, which share the
+      // SIMDs with the earlier half, does its exponentials first and its products after, so that one half's vector
+      // work goes with the other's matrix work.
+      int sk = 0, sv = S - 1;  // stages of K of tile t and of V of tile t - 1
       const auto meet = [&](int t) {
-        locate(t + 1, t);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        locate(t + S - 1, t + S - 2);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((S - 2) * C::kCopies) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        copy(t + 1, t, t + 1, t);
+        copy(t + S - 1, t + S - 2, sv, sv == 0 ? S - 1 : sv - 1);
+      };
+      const auto next = [&] {
+        sv = sk;
+        sk = sk + 1 == S ? 0 : sk + 1;
       };
       if (tiles > 0) {
-        locate(0, tiles);
-        copy(0, tiles, 0, 1);  // no V yet: a tile past the last
+#pragma unroll
+        for (int u = 0; u < S - 1; ++u) {
+          locate(u, u - 1);
+          copy(u, u - 1, u, u == 0 ? S - 1 : u - 1);
+        }
         meet(0);
         products(No{}, 0, Yes{}, 0);
         if (!LATE) weights(0);
         for (int t = 1; t < tiles; ++t) {
+          next();
           meet(t);
           if (LATE) weights(t - 1);
-          products(Yes{}, t - 1, Yes{}, t);
+          products(Yes{}, sv, Yes{}, sk);
           if (!LATE) weights(t);
         }
+        next();
         meet(tiles);
         if (LATE) weights(tiles - 1);
-        products(Yes{}, tiles - 1, No{}, 0);
+        products(Yes{}, sv, No{}, 0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end
       }
       __syncthreads();
     } else {
       // tile i of this wave is tile wave + i * NW of the stretch
       const int own = (tiles - wave + NW - 1) / NW;
-      const auto fetch = [&](int i) {
+      const auto fetch = [&](int i, int stage) {
         locate(wave + i * NW, wave + i * NW);
-        copy(wave + i * NW, wave + i * NW, i, i);
+        copy(wave + i * NW, wave + i * NW, stage, stage);
       };
-      if (own > 0) fetch(0);
+      int stage = 0;
+#pragma unroll
+      for (int i = 0; i < S - 1; ++i) fetch(i, i);
       for (int i = 0; i < own; ++i) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        fetch(i + 1);
-        products(No{}, 0, Yes{}, i);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"((S - 2) * C::kCopies) : "memory");
+        fetch(i + S - 1, stage == 0 ? S - 1 : stage - 1);
+        products(No{}, 0, Yes{}, stage);
         weights(wave + i * NW);
-        products(Yes{}, i, No{}, 0);
+        products(Yes{}, stage, No{}, 0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is read before it is filled again
+        stage = stage + 1 == S ? 0 : stage + 1;
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end
     }
@@ -472,24 +489,35 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
   }
 }
 
-// Joins the parts of the rows: 32 lanes a row, 4 columns a lane.
+// Joins the parts of a row, one wave each: lane i has part i's reference and sum, then 32 lanes take 4 columns each of
+// every second part.
+constexpr int kCrossParts = 64;
 template <class T>
-__global__ __launch_bounds__(256) void cross_join_kernel(CrossParams p) {
-  const int64_t rows = (int64_t)p.B * p.Hkv * p.rows;
-  const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int at = ((int)threadIdx.x & 31) * 4;
-  if (r >= rows || at >= p.d) return;
-  float top = -INFINITY;
-  for (int i = 0; i < p.parts; ++i) top = fmaxf(top, p.part_ml[2 * (i * rows + r)]);
-  float total = 0.f;
-  float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = 0; i < p.parts; ++i) {
-    const float t = p.part_ml[2 * (i * rows + r)], l = p.part_ml[2 * (i * rows + r) + 1];
-    const float w = t == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(t - top);
-    total += l * w;
-    o += *reinterpret_cast<const float4_t*>(p.part_o + (i * rows + r) * p.d + at) * w;
+__global__ __launch_bounds__(64) void cross_join_kernel(CrossParams p) {
+  const int64_t rows = (int64_t)p.B * p.Hkv * p.rows, r = blockIdx.x;
+  const int lane = (int)threadIdx.x, at = (lane & 31) * 4;
+  float t = -INFINITY, l = 0.f;
+  if (lane < p.parts) {
+    t = p.part_ml[2 * (lane * rows + r)];
+    l = p.part_ml[2 * (lane * rows + r) + 1];
   }
+  float top = t;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+  const float w = t == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(t - top);
+  float total = l * w;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) total += __shfl_xor(total, x, 64);
+  float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int i0 = 0; i0 < p.parts; i0 += 2) {
+    const int i = i0 + (lane >> 5);
+    const float wi = __shfl(w, i & 63, 64);
+    if (i < p.parts && at < p.d) o += *reinterpret_cast<const float4_t*>(p.part_o + (i * rows + r) * p.d + at) * wi;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], 32, 64);
+  if (lane >= 32 || at >= p.d) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const int row = (int)(r % p.rows), kh = (int)(r / p.rows % p.Hkv);
   const int64_t b = r / p.rows / p.Hkv;

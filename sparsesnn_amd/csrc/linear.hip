@@ -121,12 +121,12 @@ static hipError_t run(LinearParams p, float* workspace, size_t bytes, hipStream_
       if (q.parts > 1 && workspace && bytes >= (size_t)(q.parts * tiles) * 64 * 64 * 4) {
         p.partial = workspace;
         p.part_steps = q.part_steps;
-        const hipError_t rc = run_tile<T, 128, 64, 64, 2, 2, 4, 2>(p, q.parts, stream);
+        const hipError_t rc = run_tile<T, 128, 64, 64, 2, 2, 3, 3>(p, q.parts, stream);
         if (rc != hipSuccess) return rc;
         linear_join_kernel<T><<<dim3((unsigned)(tiles * 4)), dim3(64), 0, stream>>>(p, (p.N + 63) / 64, (int)tiles, q.parts);
         return hipGetLastError();
       }
-      return run_tile<T, 128, 64, 64, 2, 2, 4, 2>(p, 1, stream);
+      return run_tile<T, 128, 64, 64, 2, 2, 3, 3>(p, 1, stream);
     }
     case kLin128:
       return run_tile<T, 128, 128, 128, 2, 2, 2, 2>(p, 1, stream);

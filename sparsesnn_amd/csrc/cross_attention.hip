@@ -69,6 +69,14 @@ __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
   if (lane + 64 < p.d) out[lane + 64] = (T)(total == 0.f ? 0.f : o1 * inv);
 }
 
+// Which form, and in how many parts (us, measured as they stand here).
+//   rows of a workgroup (rows: the queries of a key head's group) 16 on waves with tiles of their own; 64, 128, 256
+//     where that many are left to share a tile: 4 x 4096 x 4001, 16 heads x 128: 256 rows 535, 128 rows 668;
+//     4 x 4096 x 4096 x 64: 256 rows 360, 128 rows 340
+//   four key heads together where a head's row is not whole cache lines, up to 48 values: 64 x 3136, 128 sequences,
+//     8 heads x 48: 147 (alone 166); with heads of 128 bytes side by side already there is nothing to share
+//   parts of the keys up to two workgroups a CU, of 256 keys or more (512 with 64 rows or more): one query of up to
+//     16384 keys, 8 sequences of unequal lengths, 8 key heads x 128: in 8 parts 62, in 16 71, in 12 68
 struct CrossPlan {
   int rows_a_block;
   int heads;  // key heads of a workgroup
@@ -80,9 +88,10 @@ static CrossPlan plan(const sengine_cross_desc* d) {
   CrossPlan q{rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256, 1, 1};
   if (rows <= 64 && d->d <= 48 && d->d % 16 == 0 && d->Hkv % 4 == 0 && d->k_stride[2] == d->d && d->v_stride[2] == d->d) q.heads = 4;
   const int64_t wgs = (int64_t)d->B * (d->Hkv / q.heads) * ((rows + q.rows_a_block - 1) / q.rows_a_block);
-  const int64_t want = q.rows_a_block == 16 ? 1024 : 512, least = q.rows_a_block == 16 ? 256 : 512;
-  if (wgs * 2 <= want) {
-    int64_t parts = want / wgs;
+  constexpr int64_t kWant = 512;  // workgroups: two a CU
+  const int64_t least = q.rows_a_block == 16 ? 256 : 512;  // keys of a part
+  if (wgs * 2 <= kWant) {
+    int64_t parts = kWant / wgs;
     if (parts > d->Lk / least) parts = d->Lk / least;
     if (parts > kCrossParts) parts = kCrossParts;
     if (parts > 1) q.parts = (int)parts;

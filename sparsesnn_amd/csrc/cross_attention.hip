@@ -70,13 +70,15 @@ __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
 }
 
 // Which form, and in how many parts (us, measured as they stand here).
-//   rows of a workgroup (rows: the queries of a key head's group) 16 on waves with tiles of their own; 64, 128, 256
-//     where that many are left to share a tile: 4 x 4096 x 4001, 16 heads x 128: 256 rows 535, 128 rows 668;
-//     4 x 4096 x 4096 x 64: 256 rows 360, 128 rows 340
+//   rows of a workgroup (rows: the queries of a key head's group): 16, on waves with tiles of their own, where there
+//     are no more; else the most of 256, 128, 64 that leave a workgroup for every CU, 256 for heads over 64 values
+//     only: 4 x 4096 x 4001, 16 heads x 128: 256 rows 535, 128 rows 668; 4 x 4096 x 4096 x 64: 398 and 384;
+//     1000 x 1000, 8 heads x 64: 26, 21 and with 64 rows 18
 //   four key heads together where a head's row is not whole cache lines, up to 48 values: 64 x 3136, 128 sequences,
 //     8 heads x 48: 147 (alone 166); with heads of 128 bytes side by side already there is nothing to share
 //   parts of the keys up to two workgroups a CU, of 256 keys or more (512 with 64 rows or more): one query of up to
 //     16384 keys, 8 sequences of unequal lengths, 8 key heads x 128: in 8 parts 62, in 16 71, in 12 68
+constexpr int kCUs = 256;
 struct CrossPlan {
   int rows_a_block;
   int heads;  // key heads of a workgroup
@@ -85,10 +87,17 @@ struct CrossPlan {
 
 static CrossPlan plan(const sengine_cross_desc* d) {
   const int64_t rows = (int64_t)d->Lq * (d->Hq / d->Hkv);
-  CrossPlan q{rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256, 1, 1};
+  const auto wgs_of = [&](int r) { return (int64_t)d->B * d->Hkv * ((rows + r - 1) / r); };
+  CrossPlan q{16, 1, 1};
+  if (rows > 128 && d->d > 64 && wgs_of(256) >= kCUs)
+    q.rows_a_block = 256;
+  else if (rows > 64 && wgs_of(128) >= kCUs)
+    q.rows_a_block = 128;
+  else if (rows > 16)
+    q.rows_a_block = 64;
   if (rows <= 64 && d->d <= 48 && d->d % 16 == 0 && d->Hkv % 4 == 0 && d->k_stride[2] == d->d && d->v_stride[2] == d->d) q.heads = 4;
   const int64_t wgs = (int64_t)d->B * (d->Hkv / q.heads) * ((rows + q.rows_a_block - 1) / q.rows_a_block);
-  constexpr int64_t kWant = 512;  // workgroups: two a CU
+  constexpr int64_t kWant = 2 * kCUs;  // workgroups
   const int64_t least = q.rows_a_block == 16 ? 256 : 512;  // keys of a part
   if (wgs * 2 <= kWant) {
     int64_t parts = kWant / wgs;
@@ -172,6 +181,7 @@ extern "C" int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const
     return set_error(-2, "cross_attention: the head size must be a multiple of 8 up to 128");
   if (d->type != SENGINE_ENC_F16 && d->type != SENGINE_ENC_BF16)
     return set_error(-2, "cross_attention: q, k and v must be fp16 or bf16");
+  if (d->Lk > 0x3fffffff) return set_error(-2, "cross_attention: more than 2^30 keys");
   if ((int64_t)d->B * d->Lq * d->Hq > 0x7fffffffll) return set_error(-2, "cross_attention: too many query rows");
   if (d->B == 0 || d->Lq == 0) return 0;
   if (!q || !out || (d->Lk > 0 && (!k || !v))) return set_error(-1, "cross_attention: null q, k, v or out");

@@ -74,9 +74,10 @@ __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
 //     are no more; else the most of 256, 128, 64 that leave a workgroup for every CU, 256 for heads over 64 values
 //     only: 4 x 4096 x 4001, 16 heads x 128: 256 rows 535, 128 rows 668; 4 x 4096 x 4096 x 64: 398 and 384;
 //     1000 x 1000, 8 heads x 64: 26, 21 and with 64 rows 18
-//   four key heads together where a head's row is not whole cache lines, up to 48 values: 64 x 3136, 128 sequences,
-//     8 heads x 48: 147 (alone 166); with heads of 128 bytes side by side already there is nothing to share
-//   parts of the keys up to two workgroups a CU, of 256 keys or more (512 with 64 rows or more): one query of up to
+//   four key heads together where a head's row is not whole cache lines, up to 48 values, and the time is that of
+//     reading K and V (they pass 64 MB): 64 x 3136, 128 sequences, 8 heads x 48: 113 (alone 166); one query of 196
+//     keys, 4 sequences: 9.4 (alone, with waves of their own: 8)
+//   parts of the keys where there are fewer workgroups than CUs, up to two a CU, of 256 keys or more (512 with 64 rows or more): one query of up to
 //     16384 keys, 8 sequences of unequal lengths, 8 key heads x 128: in 8 parts 62, in 16 71, in 12 68
 constexpr int kCUs = 256;
 struct CrossPlan {
@@ -95,11 +96,13 @@ static CrossPlan plan(const sengine_cross_desc* d) {
     q.rows_a_block = 128;
   else if (rows > 16)
     q.rows_a_block = 64;
-  if (rows <= 64 && d->d <= 48 && d->d % 16 == 0 && d->Hkv % 4 == 0 && d->k_stride[2] == d->d && d->v_stride[2] == d->d) q.heads = 4;
+  if (rows <= 64 && d->d <= 48 && d->d % 16 == 0 && d->Hkv % 4 == 0 && d->k_stride[2] == d->d &&
+      d->v_stride[2] == d->d && (int64_t)d->B * d->Lk * d->Hkv * d->d >= 1 << 24)
+    q.heads = 4;
   const int64_t wgs = (int64_t)d->B * (d->Hkv / q.heads) * ((rows + q.rows_a_block - 1) / q.rows_a_block);
   constexpr int64_t kWant = 2 * kCUs;  // workgroups
   const int64_t least = q.rows_a_block == 16 ? 256 : 512;  // keys of a part
-  if (wgs * 2 <= kWant) {
+  if (wgs < kCUs) {
     int64_t parts = kWant / wgs;
     if (parts > d->Lk / least) parts = d->Lk / least;
     if (parts > kCrossParts) parts = kCrossParts;

@@ -123,7 +123,7 @@ static hipError_t run(LinearParams p, float* workspace, size_t bytes, hipStream_
         p.part_steps = q.part_steps;
         const hipError_t rc = run_tile<T, 128, 64, 64, 2, 2, 3, 3>(p, q.parts, stream);
         if (rc != hipSuccess) return rc;
-        linear_join_kernel<T><<<dim3((unsigned)(tiles * 4)), dim3(64), 0, stream>>>(p, (p.N + 63) / 64, (int)tiles, q.parts);
+        linear_join_kernel<T><<<dim3((unsigned)(tiles * 8)), dim3(64), 0, stream>>>(p, (p.N + 63) / 64, (int)tiles, q.parts);
         return hipGetLastError();
       }
       return run_tile<T, 128, 64, 64, 2, 2, 3, 3>(p, 1, stream);

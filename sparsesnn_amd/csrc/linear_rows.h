@@ -51,11 +51,11 @@ __global__ __launch_bounds__(64 * W) void linear_rows_kernel(LinearParams p) {
     __builtin_memcpy(&v, q, 16);
     return v;
   };
-  const auto load = [&](Batch& b, int s) {  // steps s, s + W, .. of the whole ones; the last is repeated past the end
+  const auto load = [&](Batch& b, int s) {  // the whole steps among s, s + W, ..
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int at = s + u * W < full ? s + u * W : full - 1;
-      const int64_t k = (int64_t)at * 128;
+      if (s + u * W >= full) break;
+      const int64_t k = (int64_t)(s + u * W) * 128;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         b.w[u][h] = load16(wp + k + 64 * h);

@@ -356,27 +356,25 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
   }
 }
 
-// Joins the parts of a split reduction, one wave per 32 x 32 block of a 64 x 64 tile, and finishes it.
+// Joins the parts of a split reduction, one wave per 16 x 32 block of a 64 x 64 tile, and finishes it.
 template <class T>
 __global__ __launch_bounds__(64) void linear_join_kernel(LinearParams p, int ntn, int tiles, int parts) {
-  const int lane = (int)threadIdx.x, tile = (int)blockIdx.x >> 2, wave = (int)blockIdx.x & 3;
-  const float4_t* at = reinterpret_cast<const float4_t*>(p.partial) + (int64_t)blockIdx.x * 256 + lane;
-  const int64_t m = (int64_t)(tile / ntn) * 64 + (wave >> 1) * 32 + (lane & 15);
+  const int lane = (int)threadIdx.x, tile = (int)blockIdx.x >> 3, wave = (int)blockIdx.x >> 1 & 3, j = (int)blockIdx.x & 1;
+  const float4_t* at = reinterpret_cast<const float4_t*>(p.partial) + (int64_t)(tile * 4 + wave) * 256 + j * 64 + lane;
+  const int64_t m = (int64_t)(tile / ntn) * 64 + (wave >> 1) * 32 + j * 16 + (lane & 15);
   const int n = tile % ntn * 64 + (wave & 1) * 32 + (lane >> 4) * 8;
   Columns<T, 8> cols[1];
-  RowScales<T, 2, 16> rscales;
+  RowScales<T, 1, 16> rscales;
   cols[0].load(p, n);
   rscales.load(p, m);
-  float4_t acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) acc[i / 2][i % 2] = at[i * 64];
-#pragma unroll 4
+  float4_t acc[2][1] = {{at[0]}, {at[128]}};
+#pragma unroll 8
   for (int q = 1; q < parts; ++q) {
-    at += (int64_t)tiles * 4 * 256;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i / 2][i % 2] += at[i * 64];
+    const float4_t* part = at + (int64_t)q * tiles * 4 * 256;
+    acc[0][0] += part[0];
+    acc[1][0] += part[128];
   }
-  linear_epilogue<T, 2, 2>(p, m, n, acc, cols, rscales);
+  linear_epilogue<T, 1, 2>(p, m, n, acc, cols, rscales);
 }
 
 }  // namespace sengine

@@ -17,6 +17,11 @@
 // does not count is neither read nor multiplied.  Places of the last tile past the end are filled with zeros
 // by the buffer's bounds check and score -infinity.
 //
+// Bound by, as measured: 4 x 4096 queries x 4001 keys, 16 heads x 128, bf16: 500 to 535 us without a mask (1.0 to 1.1
+// PFLOP/s), 340 with a fifth of the keys and one sequence masked; matrix cores 42 %, vector unit 44 % (the
+// exponentials), LDS reads as long as the products.  One query of up to 16384 keys (8 sequences, 8 key heads x 128)
+// 57 us and 64 queries of 3136 keys (128 sequences, 8 heads x 48) 113 us: bandwidth, 4.9 and 5.5 TB/s.
+//
 // LDS: a key's row has PR 16-byte pieces, piece j at place j ^ f(row): 8 lanes that read a piece of 8 rows, and
 // 16 lanes that read 32 bytes of 4 rows, touch every bank once.
 #pragma once
@@ -151,7 +156,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
 
   float4_t o[DV][QF];
   float top[QF];
-  float4_t total[QF];  // the sum of the weights, the same in all four, from a product with ones: of what V is multiplied by
+  float4_t total[QF];  // the sum of the weights (all four the same) from a product with ones: of what V is multiplied by
 #pragma unroll
   for (int f = 0; f < QF; ++f) {
     top[f] = -INFINITY;
@@ -177,251 +182,252 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
 #pragma unroll
   for (int f = 0; f < (DV < 4 ? DV : 4); ++f) {
     const int x = PR == 4 ? (c >> 3) & 1 : c >> 2;
-    vat[f] = C::kOperand + (4 * g + (c >> 2)) * C::kRow + (((hp + 2 * f + ((c >> 1) & 1)) ^ (2 * x)) << 4) + (c & 1) * 8;
+    vat[f] = C::kOperand + (4 * g + (c >> 2)) * C::kRow + (((hp + 2 * f + ((c >> 1) & 1)) ^ (2 * x)) << 4) +
+             (c & 1) * 8;
   }
 
   // All keys.  LATE waves do a tile's exponentials before its neighbour's products, the others after.
   const auto run = [&](auto late) {
-  constexpr bool LATE = decltype(late)::value;
-  for (int c0 = k0; c0 < k1;) {
-    // the keys of this stretch: a list of those that count, or all
-    int cnt = k1 - c0, cn = cnt;
-    if constexpr (LIST) {
-      constexpr int NG = kCrossList / NW / 64;  // 64-key groups of a wave
-      cn = cn < kCrossList ? cn : kCrossList;
-      const uint8_t* mk = p.mask + b * p.mask_b + c0;
-      uint64_t bits[NG];
-      int mine = 0;
-      __syncthreads();  // the list of the stretch before is no longer read
+    constexpr bool LATE = decltype(late)::value;
+    for (int c0 = k0; c0 < k1;) {
+      // the keys of this stretch: a list of those that count, or all
+      int cnt = k1 - c0, cn = cnt;
+      if constexpr (LIST) {
+        constexpr int NG = kCrossList / NW / 64;  // 64-key groups of a wave
+        cn = cn < kCrossList ? cn : kCrossList;
+        const uint8_t* mk = p.mask + b * p.mask_b + c0;
+        uint64_t bits[NG];
+        int mine = 0;
+        __syncthreads();  // the list of the stretch before is no longer read
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        const int key = (wave * NG + i) * 64 + lane;
-        bits[i] = __ballot(key < cn && mk[key < cn ? key : 0] != 0);
-        mine += __popcll(bits[i]);
+        for (int i = 0; i < NG; ++i) {
+          const int key = (wave * NG + i) * 64 + lane;
+          bits[i] = __ballot(key < cn && mk[key < cn ? key : 0] != 0);
+          mine += __popcll(bits[i]);
+        }
+        if (lane == 0) counts[wave] = mine;
+        __syncthreads();
+        int at = 0;
+        cnt = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          at += w < wave ? counts[w] : 0;
+          cnt += counts[w];
+        }
+        cnt = __builtin_amdgcn_readfirstlane(cnt);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          if (bits[i] >> lane & 1)
+            list[at + __popcll(bits[i] & ((1ull << lane) - 1))] = (uint16_t)((wave * NG + i) * 64 + lane);
+          at += __popcll(bits[i]);
+        }
+        __syncthreads();
       }
-      if (lane == 0) counts[wave] = mine;
-      __syncthreads();
-      int at = 0;
-      cnt = 0;
+      const int tiles = (cnt + KT - 1) / KT;
+      // This wave's copies: K of tile tk and V of tile tv, into stages sk and sv.  Places past the last key, and tiles
+      // past the last or before the first, fetch nothing.
+      int off[C::kCopies];
+      const auto number = [&](int j) { return SHARED ? wave * C::kCopies + j : j; };
+      const auto is_v = [&](int j) { return number(j) >= C::kAllCopies / 2; };
+      const auto locate = [&](int tk, int tv) {
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        at += w < wave ? counts[w] : 0;
-        cnt += counts[w];
-      }
-      cnt = __builtin_amdgcn_readfirstlane(cnt);
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        if (bits[i] >> lane & 1)
-          list[at + __popcll(bits[i] & ((1ull << lane) - 1))] = (uint16_t)((wave * NG + i) * 64 + lane);
-        at += __popcll(bits[i]);
-      }
-      __syncthreads();
-    }
-    const int tiles = (cnt + KT - 1) / KT;
-    // This wave's copies: K of tile tk and V of tile tv, into stages sk and sv.  Places past the last key, and tiles
-    // past the last or before the first, fetch nothing.
-    int off[C::kCopies];
-    const auto number = [&](int j) { return SHARED ? wave * C::kCopies + j : j; };
-    const auto is_v = [&](int j) { return number(j) >= C::kAllCopies / 2; };
-    const auto locate = [&](int tk, int tv) {
-#pragma unroll
-      for (int j = 0; j < C::kCopies; ++j) {
-        const bool v = is_v(j);
-        const int place = number(j) % (C::kAllCopies / 2) * 64 + lane, row = place / PR;
-        const int sw = v ? (PR == 4 ? (row >> 1 & 1) * 2 : (row & 3) * 2) : (PR == 4 ? row >> 1 & 3 : row & 7);
-        const int piece = (place % PR) ^ sw, at = (v ? tv : tk) * KT + row;
-        const bool in = (unsigned)at < (unsigned)cnt && (C::MERGED || piece * 8 < p.d);
-        int key = row;
-        if constexpr (LIST) key = in ? list[at] : 0;
-        off[j] = in ? key * (v ? vst : kst) + piece * 16 : 0x7fffff00;
-      }
-    };
-    const auto copy = [&](int tk, int tv, int sk, int sv) {
-      const uint8_t* ka = kbase + (LIST ? c0 : c0 + (int64_t)tk * KT) * kst;
-      const uint8_t* va = vbase + (LIST ? c0 : c0 + (int64_t)tv * KT) * vst;
-#pragma unroll
-      for (int j = 0; j < C::kCopies; ++j) {
-        const bool v = is_v(j);
-        const u32x4_t r = row_buffer(v ? va : ka, 0x7fff0000);
-        lds_copy(r, scalar(ring0 + (v ? sv : sk) * C::kStage + number(j) * 1024), off[j]);
-      }
-    };
-    float4_t s[NK][QF];
-    u32x4_t pr[KT / 32][QF];
-    // O and the sum take on the weights and stage sv's values (V), then the scores of stage sk are formed (K); either may be
-    // left out.  Each fragment's operand is read while the products of the one before are made, and no earlier: read
-    // further ahead they would not fit the registers.
-    const auto products = [&](auto V, int sv, auto K, int sk) {
-      constexpr int NVG = decltype(V)::value ? DV : 0, NG = NVG + (decltype(K)::value ? NK : 0);
-      const uint8_t *va = ring + sv * C::kStage, *ka = ring + sk * C::kStage;
-      u32x4_t vf[2][KT / 32], kf[2][DK];
-      const auto read = [&](int n) {
-        if (n < NVG) {
-#pragma unroll
-          for (int u = 0; u < KT / 32; ++u) {
-            const uint8_t* at = va + vat[n & 3] + (n >> 2) * 128 + u * 32 * C::kRow;
-            vf[n & 1][u] = read_transposed(at, at + 16 * C::kRow);
-          }
-        } else if (n < NG) {
-#pragma unroll
-          for (int u = 0; u < DK; ++u)
-            kf[n & 1][u] = *reinterpret_cast<const u32x4_t*>(ka + (n - NVG) * 16 * C::kRow + kat[u]);
+        for (int j = 0; j < C::kCopies; ++j) {
+          const bool v = is_v(j);
+          const int place = number(j) % (C::kAllCopies / 2) * 64 + lane, row = place / PR;
+          const int sw = v ? (PR == 4 ? (row >> 1 & 1) * 2 : (row & 3) * 2) : (PR == 4 ? row >> 1 & 3 : row & 7);
+          const int piece = (place % PR) ^ sw, at = (v ? tv : tk) * KT + row;
+          const bool in = (unsigned)at < (unsigned)cnt && (C::MERGED || piece * 8 < p.d);
+          int key = row;
+          if constexpr (LIST) key = in ? list[at] : 0;
+          off[j] = in ? key * (v ? vst : kst) + piece * 16 : 0x7fffff00;
         }
       };
-      read(0);
-      if constexpr (NVG > 0) {
+      const auto copy = [&](int tk, int tv, int sk, int sv) {
+        const uint8_t* ka = kbase + (LIST ? c0 : c0 + (int64_t)tk * KT) * kst;
+        const uint8_t* va = vbase + (LIST ? c0 : c0 + (int64_t)tv * KT) * vst;
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u)
+        for (int j = 0; j < C::kCopies; ++j) {
+          const bool v = is_v(j);
+          const u32x4_t r = row_buffer(v ? va : ka, 0x7fff0000);
+          lds_copy(r, scalar(ring0 + (v ? sv : sk) * C::kStage + number(j) * 1024), off[j]);
+        }
+      };
+      float4_t s[NK][QF];
+      u32x4_t pr[KT / 32][QF];
+      // O and the sum take on the weights and stage sv's values (V), then the scores of stage sk are formed (K); either may be
+      // left out.  Each fragment's operand is read while the products of the one before are made, and no earlier: read
+      // further ahead they would not fit the registers.
+      const auto products = [&](auto V, int sv, auto K, int sk) {
+        constexpr int NVG = decltype(V)::value ? DV : 0, NG = NVG + (decltype(K)::value ? NK : 0);
+        const uint8_t *va = ring + sv * C::kStage, *ka = ring + sk * C::kStage;
+        u32x4_t vf[2][KT / 32], kf[2][DK];
+        const auto read = [&](int n) {
+          if (n < NVG) {
 #pragma unroll
-          for (int f = 0; f < QF; ++f) total[f] = mma_16<T>(ones, pr[u][f], total[f]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+            for (int u = 0; u < KT / 32; ++u) {
+              const uint8_t* at = va + vat[n & 3] + (n >> 2) * 128 + u * 32 * C::kRow;
+              vf[n & 1][u] = read_transposed(at, at + 16 * C::kRow);
+            }
+          } else if (n < NG) {
 #pragma unroll
-      for (int n = 0; n < NG; ++n) {
-        read(n + 1);
-        __builtin_amdgcn_sched_barrier(0);
-        if (n < NVG) {
+            for (int u = 0; u < DK; ++u)
+              kf[n & 1][u] = *reinterpret_cast<const u32x4_t*>(ka + (n - NVG) * 16 * C::kRow + kat[u]);
+          }
+        };
+        read(0);
+        if constexpr (NVG > 0) {
 #pragma unroll
           for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-            for (int f = 0; f < QF; ++f) o[n][f] = mma_16<T>(vf[n & 1][u], pr[u][f], o[n][f]);
-        } else {
-          const int i = n - NVG;
-          if constexpr (HALF) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) kf[n & 1][DK - 1][e] = g < 2 ? kf[n & 1][DK - 1][e] : 0;
-          }
-#pragma unroll
-          for (int f = 0; f < QF; ++f) s[i][f] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int u = 0; u < DK; ++u)
-#pragma unroll
-            for (int f = 0; f < QF; ++f) s[i][f] = mma_16<T>(kf[n & 1][u], q[f][u], s[i][f]);
+            for (int f = 0; f < QF; ++f) total[f] = mma_16<T>(ones, pr[u][f], total[f]);
         }
         __builtin_amdgcn_sched_barrier(0);
-      }
-    };
-    const auto weights = [&](int t) {
-      const int left = cnt - t * KT;
-      if (left < KT) {
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+        for (int n = 0; n < NG; ++n) {
+          read(n + 1);
+          __builtin_amdgcn_sched_barrier(0);
+          if (n < NVG) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (16 * i + 4 * g + e >= left) {
+            for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-              for (int f = 0; f < QF; ++f) s[i][f][e] = -INFINITY;
+              for (int f = 0; f < QF; ++f) o[n][f] = mma_16<T>(vf[n & 1][u], pr[u][f], o[n][f]);
+          } else {
+            const int i = n - NVG;
+            if constexpr (HALF) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) kf[n & 1][DK - 1][e] = g < 2 ? kf[n & 1][DK - 1][e] : 0;
             }
-      }
-      float high[QF];
-      bool raise = false;
 #pragma unroll
-      for (int f = 0; f < QF; ++f) {
-        high[f] = fmaxf(fmaxf(s[0][f][0], s[0][f][1]), s[0][f][2]);  // three at a time
-        high[f] = fmaxf(fmaxf(s[0][f][3], s[1][f][0]), high[f]);
-        high[f] = fmaxf(fmaxf(s[1][f][1], s[1][f][2]), high[f]);
-        if constexpr (NK == 2) {
-          high[f] = fmaxf(s[1][f][3], high[f]);
-        } else {
-          high[f] = fmaxf(fmaxf(s[1][f][3], s[2][f][0]), high[f]);
-          high[f] = fmaxf(fmaxf(s[2][f][1], s[2][f][2]), high[f]);
-          high[f] = fmaxf(fmaxf(s[2][f][3], s[3][f][0]), high[f]);
-          high[f] = fmaxf(fmaxf(s[3][f][1], s[3][f][2]), high[f]);
-          high[f] = fmaxf(s[3][f][3], high[f]);
+            for (int f = 0; f < QF; ++f) s[i][f] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < DK; ++u)
+#pragma unroll
+              for (int f = 0; f < QF; ++f) s[i][f] = mma_16<T>(kf[n & 1][u], q[f][u], s[i][f]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        high[f] = max_of_groups(high[f]) * cs;
-        raise |= high[f] > top[f] + 8.f;
-      }
-      if (__any(raise)) {
+      };
+      const auto weights = [&](int t) {
+        const int left = cnt - t * KT;
+        if (left < KT) {
+#pragma unroll
+          for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (16 * i + 4 * g + e >= left) {
+#pragma unroll
+                for (int f = 0; f < QF; ++f) s[i][f][e] = -INFINITY;
+              }
+        }
+        float high[QF];
+        bool raise = false;
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
-          const float t1 = fmaxf(top[f], high[f]);
-          const float back = t1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[f] - t1);
-          top[f] = t1;
-          total[f] *= back;
-#pragma unroll
-          for (int i = 0; i < DV; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][f][e] *= back;
+          high[f] = fmaxf(fmaxf(s[0][f][0], s[0][f][1]), s[0][f][2]);  // three at a time
+          high[f] = fmaxf(fmaxf(s[0][f][3], s[1][f][0]), high[f]);
+          high[f] = fmaxf(fmaxf(s[1][f][1], s[1][f][2]), high[f]);
+          if constexpr (NK == 2) {
+            high[f] = fmaxf(s[1][f][3], high[f]);
+          } else {
+            high[f] = fmaxf(fmaxf(s[1][f][3], s[2][f][0]), high[f]);
+            high[f] = fmaxf(fmaxf(s[2][f][1], s[2][f][2]), high[f]);
+            high[f] = fmaxf(fmaxf(s[2][f][3], s[3][f][0]), high[f]);
+            high[f] = fmaxf(fmaxf(s[3][f][1], s[3][f][2]), high[f]);
+            high[f] = fmaxf(s[3][f][3], high[f]);
+          }
+          high[f] = max_of_groups(high[f]) * cs;
+          raise |= high[f] > top[f] + 8.f;
         }
-      }
+        if (__any(raise)) {
 #pragma unroll
-      for (int f = 0; f < QF; ++f) {
-        const float ref = top[f] == -INFINITY ? 0.f : -top[f];  // every score so far is -infinity: they weigh nothing
+          for (int f = 0; f < QF; ++f) {
+            const float t1 = fmaxf(top[f], high[f]);
+            const float back = t1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[f] - t1);
+            top[f] = t1;
+            total[f] *= back;
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u) {
-          typedef T vec8_t __attribute__((ext_vector_type(8)));
-          vec8_t x;
+            for (int i = 0; i < DV; ++i)
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * u + e / 4][f][e % 4], cs, ref));
-          pr[u][f] = __builtin_bit_cast(u32x4_t, x);
+              for (int e = 0; e < 4; ++e) o[i][f][e] *= back;
+          }
         }
-      }
-    };
-    if constexpr (SHARED) {
-      // Between meetings t and t + 1 the waves need K of tile t and V of tile t - 1, which meeting t finds landed;
-      // K up to t + S - 1 and V up to t + S - 2 are on their way.  The later half of eight waves, which share the
-      // SIMDs with the earlier half, does its exponentials first and its products after, so that one half's vector
-      // work goes with the other's matrix work.
-      int sk = 0, sv = S - 1;  // stages of K of tile t and of V of tile t - 1
-      const auto meet = [&](int t) {
-        locate(t + S - 1, t + S - 2);
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((S - 2) * C::kCopies) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        copy(t + S - 1, t + S - 2, sv, sv == 0 ? S - 1 : sv - 1);
+#pragma unroll
+        for (int f = 0; f < QF; ++f) {
+          const float ref = top[f] == -INFINITY ? 0.f : -top[f];  // every score so far is -infinity: they weigh nothing
+#pragma unroll
+          for (int u = 0; u < KT / 32; ++u) {
+            typedef T vec8_t __attribute__((ext_vector_type(8)));
+            vec8_t x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              x[e] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * u + e / 4][f][e % 4], cs, ref));
+            pr[u][f] = __builtin_bit_cast(u32x4_t, x);
+          }
+        }
       };
-      const auto next = [&] {
-        sv = sk;
-        sk = sk + 1 == S ? 0 : sk + 1;
-      };
-      if (tiles > 0) {
+      if constexpr (SHARED) {
+        // Between meetings t and t + 1 the waves need K of tile t and V of tile t - 1, which meeting t finds landed;
+        // K up to t + S - 1 and V up to t + S - 2 are on their way.  The later half of eight waves, which share the
+        // SIMDs with the earlier half, does its exponentials first and its products after, so that one half's vector
+        // work goes with the other's matrix work.
+        int sk = 0, sv = S - 1;  // stages of K of tile t and of V of tile t - 1
+        const auto meet = [&](int t) {
+          locate(t + S - 1, t + S - 2);
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((S - 2) * C::kCopies) : "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          copy(t + S - 1, t + S - 2, sv, sv == 0 ? S - 1 : sv - 1);
+        };
+        const auto next = [&] {
+          sv = sk;
+          sk = sk + 1 == S ? 0 : sk + 1;
+        };
+        if (tiles > 0) {
 #pragma unroll
-        for (int u = 0; u < S - 1; ++u) {
-          locate(u, u - 1);
-          copy(u, u - 1, u, u == 0 ? S - 1 : u - 1);
-        }
-        meet(0);
-        products(No{}, 0, Yes{}, 0);
-        if (!LATE) weights(0);
-        for (int t = 1; t < tiles; ++t) {
+          for (int u = 0; u < S - 1; ++u) {
+            locate(u, u - 1);
+            copy(u, u - 1, u, u == 0 ? S - 1 : u - 1);
+          }
+          meet(0);
+          products(No{}, 0, Yes{}, 0);
+          if (!LATE) weights(0);
+          for (int t = 1; t < tiles; ++t) {
+            next();
+            meet(t);
+            if (LATE) weights(t - 1);
+            products(Yes{}, sv, Yes{}, sk);
+            if (!LATE) weights(t);
+          }
           next();
-          meet(t);
-          if (LATE) weights(t - 1);
-          products(Yes{}, sv, Yes{}, sk);
-          if (!LATE) weights(t);
+          meet(tiles);
+          if (LATE) weights(tiles - 1);
+          products(Yes{}, sv, No{}, 0);
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end
         }
-        next();
-        meet(tiles);
-        if (LATE) weights(tiles - 1);
-        products(Yes{}, sv, No{}, 0);
+        __syncthreads();
+      } else {
+        // tile i of this wave is tile wave + i * NW of the stretch
+        const int own = (tiles - wave + NW - 1) / NW;
+        const auto fetch = [&](int i, int stage) {
+          locate(wave + i * NW, wave + i * NW);
+          copy(wave + i * NW, wave + i * NW, stage, stage);
+        };
+        int stage = 0;
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) fetch(i, i);
+        for (int i = 0; i < own; ++i) {
+          asm volatile("s_waitcnt vmcnt(%0)" ::"i"((S - 2) * C::kCopies) : "memory");
+          fetch(i + S - 1, stage == 0 ? S - 1 : stage - 1);
+          products(No{}, 0, Yes{}, stage);
+          weights(wave + i * NW);
+          products(Yes{}, stage, No{}, 0);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is read before it is filled again
+          stage = stage + 1 == S ? 0 : stage + 1;
+        }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end
       }
-      __syncthreads();
-    } else {
-      // tile i of this wave is tile wave + i * NW of the stretch
-      const int own = (tiles - wave + NW - 1) / NW;
-      const auto fetch = [&](int i, int stage) {
-        locate(wave + i * NW, wave + i * NW);
-        copy(wave + i * NW, wave + i * NW, stage, stage);
-      };
-      int stage = 0;
-#pragma unroll
-      for (int i = 0; i < S - 1; ++i) fetch(i, i);
-      for (int i = 0; i < own; ++i) {
-        asm volatile("s_waitcnt vmcnt(%0)" ::"i"((S - 2) * C::kCopies) : "memory");
-        fetch(i + S - 1, stage == 0 ? S - 1 : stage - 1);
-        products(No{}, 0, Yes{}, stage);
-        weights(wave + i * NW);
-        products(Yes{}, stage, No{}, 0);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is read before it is filled again
-        stage = stage + 1 == S ? 0 : stage + 1;
-      }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies past the end
+      c0 += cn;
     }
-    c0 += cn;
-  }
   };
   // (code of its own for each half: branches inside the loop would move the sums between registers)
   if (SHARED && NW == 8 && wave >= 4)
@@ -489,8 +495,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
   }
 }
 
-// Joins the parts of a row, one wave each: lane i has part i's reference and sum, then 32 lanes take 4 columns each of
-// every second part.
+// Joins the parts of a row, one wave each: lane i has part i's reference and sum, then 32 lanes take 4 columns each
+// of every second part.  256 rows of 8 parts of 128 values: 4.9 us.
 constexpr int kCrossParts = 64;
 template <class T>
 __global__ __launch_bounds__(64) void cross_join_kernel(CrossParams p) {

@@ -8,8 +8,6 @@
 
 namespace sengine {
 
-constexpr int kLinStep = 128;  // bytes of the reduction that plans count in
-
 // Any strides, any alignment, any K.  Workgroup = 64 rows x 64 columns, four waves of 32 x 32; per
 // 128 bytes of the reduction both operands' rows go through registers into LDS: whole 16-byte pieces
 // by one load of whatever alignment, the row's last piece byte by byte, zeros beyond.
@@ -68,10 +66,10 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
   linear_epilogue<T, 2, 2>(p, m0 + wm + (lane & 15), n0 + wn + 8 * (lane >> 4), acc, cols, rscales);
 }
 
-template <class T, int HB, int BM, int BN, int WM, int WN, int S, int WGS>
+template <class T, int BM, int BN, int WM, int WN, int S, int WGS>
 static hipError_t run_tile(const LinearParams& p, int parts, hipStream_t stream) {
   const int64_t ntm = (p.M + BM - 1) / BM, ntn = (p.N + BN - 1) / BN;
-  linear_tile_kernel<T, HB, BM, BN, WM, WN, S, WGS>
+  linear_tile_kernel<T, BM, BN, WM, WN, S, WGS>
       <<<dim3((unsigned)(ntm * ntn), (unsigned)parts), dim3(64 * WM * WN), 0, stream>>>(p, (int)ntm, (int)ntn);
   return hipGetLastError();
 }
@@ -114,24 +112,25 @@ static hipError_t run(LinearParams p, float* workspace, size_t bytes, hipStream_
   const LinearPlan q = plan(p, __is_same(T, E4m3Wide));
   switch (q.kernel) {
     case kLinRows:
-      linear_rows_kernel<T, 1, 8, 4><<<dim3((unsigned)((p.N + 15) / 16)), dim3(512), 0, stream>>>(p);
+      linear_rows_kernel<T, 8, 4><<<dim3((unsigned)((p.N + 15) / 16)), dim3(512), 0, stream>>>(p);
       return hipGetLastError();
     case kLin64: {
       const int64_t tiles = tiles_of(p, 64);
       if (q.parts > 1 && workspace && bytes >= (size_t)(q.parts * tiles) * 64 * 64 * 4) {
         p.partial = workspace;
         p.part_steps = q.part_steps;
-        const hipError_t rc = run_tile<T, 128, 64, 64, 2, 2, 3, 3>(p, q.parts, stream);
+        const hipError_t rc = run_tile<T, 64, 64, 2, 2, 3, 3>(p, q.parts, stream);
         if (rc != hipSuccess) return rc;
-        linear_join_kernel<T><<<dim3((unsigned)(tiles * 8)), dim3(64), 0, stream>>>(p, (p.N + 63) / 64, (int)tiles, q.parts);
+        linear_join_kernel<T>
+            <<<dim3((unsigned)(tiles * 8)), dim3(64), 0, stream>>>(p, (p.N + 63) / 64, (int)tiles, q.parts);
         return hipGetLastError();
       }
-      return run_tile<T, 128, 64, 64, 2, 2, 3, 3>(p, 1, stream);
+      return run_tile<T, 64, 64, 2, 2, 3, 3>(p, 1, stream);
     }
     case kLin128:
-      return run_tile<T, 128, 128, 128, 2, 2, 2, 2>(p, 1, stream);
+      return run_tile<T, 128, 128, 2, 2, 2, 2>(p, 1, stream);
     case kLin256:
-      if constexpr (!__is_same(T, E4m3Wide)) return run_tile<T, 128, 256, 256, 2, 2, 2, 1>(p, 1, stream);
+      if constexpr (!__is_same(T, E4m3Wide)) return run_tile<T, 256, 256, 2, 2, 2, 1>(p, 1, stream);
       [[fallthrough]];
     default:
       linear_any_kernel<T><<<dim3((unsigned)tiles_of(p, 64)), dim3(256), 0, stream>>>(p);

@@ -4,15 +4,22 @@
 // Per 128 bytes of the reduction both operands' rows are copied into one of S LDS stages by
 // buffer_load ... lds, 16 bytes a lane; out-of-range lanes (rows past the end, the reduction's tail)
 // receive zeros from the buffer's bounds check.  LDS row r keeps its 16-byte piece j at place
-// j ^ (r % 8): eight lanes copy one row's 128 bytes and the 16 lanes that read piece j of 16 rows touch
-// every bank evenly.
+// j ^ (r % 8): eight lanes copy one row's 128 bytes and the 16 lanes that read piece j of
+// 16 rows touch every bank evenly.
 //
 // The stage's rows of a wave are read in four quarters, A = weight rows, B = token rows, each halved:
 //   A-lo B-first | A-lo B-second | A-hi B-second | A-hi B-first
 // so that each quarter's products need only one new half, which is read during the quarter before it.
-// All reads of a stage are done by the end of the second quarter: there the workgroup meets once, the
-// freed stage is refilled, and the third quarter already reads the next stage.  The second half of B
-// becomes the first of the next step.
+// In the middle of the third quarter all reads of the stage are done: there the workgroup meets once, and
+// beside the rest of the step's products the freed stage is refilled and the next stage's first operands
+// are read.  The second half of B becomes the first of the next step.
+//
+// Bound by, as measured: 256 x 256 tiles: 8192 x 4096 x 8192 bf16 416 us (1.32 PFLOP/s), 8192^3 e4m3 453
+// (2.43): matrix cores and the clock that they leave; without the copies 8192^3 bf16 takes 757 of 857 us.
+// A wave of 128 x 128 needs two thirds of the LDS reads of eight waves of 128 x 64.  128 x 128 tiles:
+// 100352 x 1536 x 384 fp16 with GELU 249 us, 22 a step and 130 for the starts, epilogues and stores of 9408
+// tiles.  64 x 64 tiles: 0.2 us a step, three workgroups a CU.  Stages of 64 bytes, twice as many, are
+// slower everywhere (8192^3 bf16 974 us): twice the meetings, half lines.
 //
 // Weight rows are placed so that a lane ends with 8 consecutive output columns: row 16 b + 4 g + e of
 // 32 LDS rows holds weight row 8 g + 4 b + e, and value e of fragment (b = i % 2) in lane group g is
@@ -22,6 +29,8 @@
 #include "linear.h"
 
 namespace sengine {
+
+constexpr int kLinStep = 128;  // bytes of the reduction a step
 
 
 // Workgroup -> tile.  Each XCD walks kLinGroup row tiles before the next column tile, so that what runs on it
@@ -62,16 +71,7 @@ __device__ __forceinline__ void mma_inplace(u32x8_t a, u32x8_t b, float4_t& c) {
 __device__ __forceinline__ void mma_drain() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 // A lane's share of a fragment in one step: 16 bytes of each 64-byte half of its row.
-template <int HB>
-struct Fragment;
-template <>
-struct Fragment<64> {
-  u32x4_t v;
-  __device__ __forceinline__ void set(int, u32x4_t x) { v = x; }
-  __device__ __forceinline__ u32x4_t half(int) const { return v; }
-};
-template <>
-struct Fragment<128> {
+struct Fragment {
   u32x8_t v;
   __device__ __forceinline__ void set(int h, u32x4_t x) {
 #pragma unroll
@@ -82,26 +82,20 @@ struct Fragment<128> {
   }
 };
 
-// Piece j of LDS row r lies at place j ^ lin_place(r).
-template <int PR>
-__device__ __forceinline__ int lin_place(int r) {
-  return PR == 4 ? r >> 1 & 3 : r & 7;
-}
-
-template <class T, int HB, int BM, int BN, int WM, int WN, int S>
+template <class T, int BM, int BN, int WM, int WN, int S>
 struct LinearTile {
   static constexpr int kWaves = WM * WN;
   static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  static constexpr int kStage = (BM + BN) * HB;
-  static constexpr int kXCopies = BM * HB / 1024 / kWaves, kWCopies = BN * HB / 1024 / kWaves;  // of a wave a stage
+  static constexpr int kStage = (BM + BN) * kLinStep;
+  static constexpr int kXCopies = BM * kLinStep / 1024 / kWaves, kWCopies = BN * kLinStep / 1024 / kWaves;  // of a wave a stage
   static constexpr int kCopies = kXCopies + kWCopies;
-  static_assert(BM * HB % (1024 * kWaves) == 0 && BN * HB % (1024 * kWaves) == 0 && TM % 2 == 0 && TN % 2 == 0, "tile");
+  static_assert(BM * kLinStep % (1024 * kWaves) == 0 && BN * kLinStep % (1024 * kWaves) == 0 && TM % 2 == 0 && TN % 2 == 0, "tile");
 };
 
-template <class T, int HB, int BM, int BN, int WM, int WN, int S, int WGS>
-__global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_tile_kernel(LinearParams p, int ntm, int ntn) {
-  using C = LinearTile<T, HB, BM, BN, WM, WN, S>;
-  constexpr int PR = HB / 16;  // 16-byte pieces of a row in a stage
+template <class T, int BM, int BN, int WM, int WN, int S, int WGS>
+__global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4)
+void linear_tile_kernel(LinearParams p, int ntm, int ntn) {
+  using C = LinearTile<T, BM, BN, WM, WN, S>;
   constexpr int TM = C::TM, TN = C::TN;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[S * C::kStage];
   const int lane = (int)threadIdx.x & 63;
@@ -120,14 +114,14 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
   const int xbytes = (mrows - 1) * (int)p.x_stride + p.kbytes;
   const int wbytes = (nrows - 1) * (int)p.w_stride + p.kbytes;
   // this lane's row and piece of each copy of 1024 bytes
-  const int lrow = lane / PR, piece = ((lane % PR) ^ lin_place<PR>(lrow)) * 16;
+  const int lrow = lane >> 3, piece = ((lane & 7) ^ lrow) * 16;
   int voff[C::kCopies];
 #pragma unroll
   for (int j = 0; j < C::kXCopies; ++j)
-    voff[j] = (64 / PR * (wave * C::kXCopies + j) + lrow) * (int)p.x_stride + piece;
+    voff[j] = (8 * (wave * C::kXCopies + j) + lrow) * (int)p.x_stride + piece;
 #pragma unroll
   for (int j = 0; j < C::kWCopies; ++j) {
-    const int r = 64 / PR * (wave * C::kWCopies + j) + lrow;  // LDS row; its weight row:
+    const int r = 8 * (wave * C::kWCopies + j) + lrow;  // LDS row; its weight row:
     const int n = (r & ~31) + ((r >> 2) & 3) * 8 + ((r >> 4) & 1) * 4 + (r & 3);
     voff[C::kXCopies + j] = n * (int)p.w_stride + piece;
   }
@@ -136,7 +130,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
   // (two at a time, an odd last one followed by one of zeros), since sums that arrive by several ways would
   // have to be moved, through scratch memory.
   constexpr bool PAIRS = TM * TN >= 64;
-  const int total = (p.kbytes + HB - 1) / HB;
+  const int total = (p.kbytes + kLinStep - 1) / kLinStep;
   // a part of the reduction (blockIdx.y) or all of it
   const int first = p.partial ? (int)blockIdx.y * p.part_steps : 0;
   const int wanted = p.partial && total - first > p.part_steps ? p.part_steps : total - first;
@@ -146,11 +140,11 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
   u32x4_t xr, wr;
   uint32_t dst;
   const auto copies_of = [&](int step, int stage) {
-    const int k = (first + step) * HB, left = step < wanted ? p.kbytes - k : 0;
+    const int k = (first + step) * kLinStep, left = step < wanted ? p.kbytes - k : 0;
     xr = row_buffer(xb + k, left > 0 ? xbytes - k : 0);
     wr = row_buffer(wb + k, left > 0 ? wbytes - k : 0);
     dst = lds0 + stage * C::kStage;
-    if (left < HB) {  // the tail: pieces past the row's end are out of range
+    if (left < kLinStep) {  // the tail: pieces past the row's end are out of range
 #pragma unroll
       for (int j = 0; j < C::kCopies; ++j) voff[j] = piece < left ? voff[j] : 0x7fffff00;
     }
@@ -159,7 +153,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
     if (j < C::kXCopies)
       lds_copy(xr, dst + (wave * C::kXCopies + j) * 1024, voff[j]);
     else
-      lds_copy(wr, dst + BM * HB + (wave * C::kWCopies + j - C::kXCopies) * 1024, voff[j]);
+      lds_copy(wr, dst + BM * kLinStep + (wave * C::kWCopies + j - C::kXCopies) * 1024, voff[j]);
   };
 
   // what the epilogue needs of the columns and rows that this lane finishes
@@ -179,21 +173,19 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
   for (int i = 0; i < TN; ++i)
 #pragma unroll
     for (int j = 0; j < TM; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
-  Fragment<HB> a[TN], b[TM];
+  Fragment a[TN], b[TM];
   // this lane's 16 bytes of fragment row lane % 16 in either half of the step: pieces lane / 16 and 4 + lane / 16
-  const int fr = (lane & 15) * HB, sw = lin_place<PR>(lane & 15);
+  const int fr = (lane & 15) * kLinStep, sw = lane & 7;
   const int at0 = fr + (((lane >> 4) ^ sw) << 4), at1 = fr + (((4 + (lane >> 4)) ^ sw) << 4);
-  const int xat = wm * TM * 16 * HB, wat = BM * HB + wn * TN * 16 * HB;
+  const int xat = wm * TM * 16 * kLinStep, wat = BM * kLinStep + wn * TN * 16 * kLinStep;
   const auto read_a = [&](int stage_at, int i, int h) {
-    a[i].set(h, *reinterpret_cast<const u32x4_t*>(smem + stage_at + wat + i * 16 * HB + (h ? at1 : at0)));
+    a[i].set(h, *reinterpret_cast<const u32x4_t*>(smem + stage_at + wat + i * 16 * kLinStep + (h ? at1 : at0)));
   };
   const auto read_b = [&](int stage_at, int j, int h) {
-    b[j].set(h, *reinterpret_cast<const u32x4_t*>(smem + stage_at + xat + j * 16 * HB + (h ? at1 : at0)));
+    b[j].set(h, *reinterpret_cast<const u32x4_t*>(smem + stage_at + xat + j * 16 * kLinStep + (h ? at1 : at0)));
   };
   // Products FROM..TO-1 of the NM of quarter (i0, j0), with hook(n) before product n.
-  constexpr int LH = HB / 64;                      // 64-byte halves of a step
-  constexpr int NH = __is_same(T, E4m3) ? 1 : LH;  // those that are products of their own
-  static_assert(!__is_same(T, E4m3) || HB == 128, "8-bit products take 128 bytes");
+  constexpr int NH = __is_same(T, E4m3) ? 1 : 2;  // 64-byte halves of a step that are products of their own
   constexpr int NM = NH * (TN / 2) * (TM / 2);
   const auto quarter = [&](int i0, int j0, int from, int to, auto hook) {
 #pragma unroll
@@ -227,7 +219,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int h = 0; h < LH; ++h) {
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int i = 0; i < TN / 2; ++i) read_a(0, i, h);
 #pragma unroll
@@ -241,10 +233,10 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
       const int nstage = stage + 1 == S ? 0 : stage + 1;
       const int nxt = nstage * C::kStage;
       quarter(0, F, 0, NM, [&](int n) {
-        spread(n, LH * TM / 2, NM, [&](int r) { read_b(cur, G + r % (TM / 2), r / (TM / 2)); });
+        spread(n, TM, NM, [&](int r) { read_b(cur, G + r % (TM / 2), r / (TM / 2)); });
       });
       quarter(0, G, 0, NM, [&](int n) {
-        spread(n, LH * TN / 2, NM, [&](int r) { read_a(cur, TN / 2 + r % (TN / 2), r / (TN / 2)); });
+        spread(n, TN, NM, [&](int r) { read_a(cur, TN / 2 + r % (TN / 2), r / (TN / 2)); });
       });
       quarter(TN / 2, G, 0, SPLIT, [&](int) {});
       // this wave has read the stage (lgkmcnt) and its copies of the next one have landed (vmcnt)
@@ -255,12 +247,12 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
       __builtin_amdgcn_sched_barrier(0);
       // the rest of the step: the next one's first operands and the copies
       const auto rest = [&](int n) {
-        spread(n, LH * (TN + TM) / 2, REST, [&](int r) {
+        spread(n, TN + TM, REST, [&](int r) {
           if constexpr (NH == 1) {  // a fragment is one operand: B's only after its last use
-            if (r < LH * TN / 2)
+            if (r < TN)
               read_a(nxt, r % (TN / 2), r / (TN / 2));
             else
-              read_b(nxt, G + (r - LH * TN / 2) % (TM / 2), (r - LH * TN / 2) / (TM / 2));
+              read_b(nxt, G + (r - TN) % (TM / 2), (r - TN) / (TM / 2));
           } else {
             const int h = r / (TN / 2 + TM / 2), q = r % (TN / 2 + TM / 2);
             if (q < TN / 2)
@@ -359,7 +351,8 @@ __global__ __launch_bounds__(64 * WM * WN, (WGS * WM * WN + 3) / 4) void linear_
 // Joins the parts of a split reduction, one wave per 16 x 32 block of a 64 x 64 tile, and finishes it.
 template <class T>
 __global__ __launch_bounds__(64) void linear_join_kernel(LinearParams p, int ntn, int tiles, int parts) {
-  const int lane = (int)threadIdx.x, tile = (int)blockIdx.x >> 3, wave = (int)blockIdx.x >> 1 & 3, j = (int)blockIdx.x & 1;
+  const int lane = (int)threadIdx.x;
+  const int tile = (int)blockIdx.x >> 3, wave = (int)blockIdx.x >> 1 & 3, j = (int)blockIdx.x & 1;
   const float4_t* at = reinterpret_cast<const float4_t*>(p.partial) + (int64_t)(tile * 4 + wave) * 256 + j * 64 + lane;
   const int64_t m = (int64_t)(tile / ntn) * 64 + (wave >> 1) * 32 + j * 16 + (lane & 15);
   const int n = tile % ntn * 64 + (wave & 1) * 32 + (lane >> 4) * 8;

@@ -26,8 +26,8 @@ from ._lib import SEngineError
 E4M3_MAX = 448.0
 
 
-def random_reader_params(seed: int = 0, embed: int = 384, depth: int = 2, mlp_ratio: int = 4, num_classes: int = 1000,
-                         queries: int = 1) -> dict:
+def random_reader_params(seed: int = 0, embed: int = 384, depth: int = 2, mlp_ratio: int = 4,
+                         num_classes: int = 1000, queries: int = 1) -> dict:
     """Random weights of the shapes a TokenReader takes."""
     g = torch.Generator().manual_seed(seed)
 
@@ -67,11 +67,14 @@ class TokenReader:
         self.p = {k: v.detach().to(dev, dtype).contiguous() for k, v in params.items()}
         self.embed = self.p["norm.weight"].numel()
         if self.embed % heads or self.embed // heads % 8:
-            raise SEngineError(f"TokenReader: {self.embed} channels do not split into {heads} heads of a multiple of 8")
+            raise SEngineError(f"TokenReader: {self.embed} channels do not split into {heads} heads of a multiple of 8 "
+                               "values")
         self.depth = 0
         while f"block.{self.depth}.q.weight" in params:
             self.depth += 1
-        self.fc1 = [e4m3_rows(params[f"block.{i}.fc1.weight"].to(dev)) for i in range(self.depth)] if eight_bit else None
+        self.fc1 = None
+        if eight_bit:
+            self.fc1 = [e4m3_rows(params[f"block.{i}.fc1.weight"].to(dev)) for i in range(self.depth)]
 
     def encode(self, tokens: torch.Tensor):
         """Every block's (keys, values) of the tokens (B, N, C): each (B, N, heads, C / heads)."""

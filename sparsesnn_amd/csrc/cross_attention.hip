@@ -78,7 +78,8 @@ __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
 //     reading K and V (they pass 64 MB): 64 x 3136, 128 sequences, 8 heads x 48: 113 (alone 166); one query of 196
 //     keys, 4 sequences: 9.4 (alone, with waves of their own: 8)
 //   parts of the keys where there are fewer workgroups than CUs, up to two a CU, of 256 keys or more (512 with 64
-//     rows or more): one query of up to 16384 keys, 8 sequences of unequal lengths, 8 key heads x 128: in 8 parts 62, in 16 71, in 12 68
+//     rows or more): one query of up to 16384 keys, 8 sequences of unequal lengths, 8 key heads x 128: in 8 parts
+//     62, in 16 71, in 12 68
 constexpr int kCUs = 256;
 struct CrossPlan {
   int rows_a_block;
@@ -175,8 +176,8 @@ static hipError_t by_width(CrossParams& p, const CrossPlan& q, hipStream_t strea
 using namespace sengine;
 
 extern "C" int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const void* q, const void* k,
-                                              const void* v, const int32_t* key_lengths, const void* key_mask, void* out,
-                                              void* workspace, size_t workspace_bytes, hipStream_t stream) {
+                                              const void* v, const int32_t* key_lengths, const void* key_mask,
+                                              void* out, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (!d) return set_error(-1, "cross_attention: null descriptor");
   if (d->B < 0 || d->Lq < 0 || d->Lk < 0 || d->Hq < 1 || d->Hkv < 1)
     return set_error(-2, "cross_attention: needs B, Lq, Lk >= 0 and heads >= 1");

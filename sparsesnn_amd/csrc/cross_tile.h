@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
 
   float4_t o[DV][QF];
   float top[QF];
-  float4_t total[QF];  // the sum of the weights (all four the same) from a product with ones: of what V is multiplied by
+  float4_t total[QF];  // the sum of the weights (all four the same), from a product with ones: of what multiplies V
 #pragma unroll
   for (int f = 0; f < QF; ++f) {
     top[f] = -INFINITY;
@@ -254,9 +254,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
       };
       float4_t s[NK][QF];
       u32x4_t pr[KT / 32][QF];
-      // O and the sum take on the weights and stage sv's values (V), then the scores of stage sk are formed (K); either may be
-      // left out.  Each fragment's operand is read while the products of the one before are made, and no earlier: read
-      // further ahead they would not fit the registers.
+      // O and the sum take on the weights and stage sv's values (V), then the scores of stage sk are formed (K);
+      // either may be left out.  Each fragment's operand is read while the products of the one before are made, and
+      // no earlier: read further ahead they would not fit the registers.
       const auto products = [&](auto V, int sv, auto K, int sk) {
         constexpr int NVG = decltype(V)::value ? DV : 0, NG = NVG + (decltype(K)::value ? NK : 0);
         const uint8_t *va = ring + sv * C::kStage, *ka = ring + sk * C::kStage;

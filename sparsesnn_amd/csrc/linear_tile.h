@@ -87,9 +87,9 @@ struct LinearTile {
   static constexpr int kWaves = WM * WN;
   static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   static constexpr int kStage = (BM + BN) * kLinStep;
-  static constexpr int kXCopies = BM * kLinStep / 1024 / kWaves, kWCopies = BN * kLinStep / 1024 / kWaves;  // of a wave a stage
+  static constexpr int kXCopies = BM / 8 / kWaves, kWCopies = BN / 8 / kWaves;  // LDS copies of a wave a stage
   static constexpr int kCopies = kXCopies + kWCopies;
-  static_assert(BM * kLinStep % (1024 * kWaves) == 0 && BN * kLinStep % (1024 * kWaves) == 0 && TM % 2 == 0 && TN % 2 == 0, "tile");
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && TM % 2 == 0 && TN % 2 == 0, "tile");
 };
 
 template <class T, int BM, int BN, int WM, int WN, int S, int WGS>
@@ -290,9 +290,11 @@ void linear_tile_kernel(LinearParams p, int ntm, int ntn) {
       const int64_t tile = (int64_t)blockIdx.y * ntm * ntn + (int64_t)mt * ntn + nt;
       float4_t* at = reinterpret_cast<float4_t*>(p.partial) + (tile * C::kWaves + wave) * 256 + lane;
 #pragma unroll
-      for (int i = 0; i < TN; ++i)
+      for (int j = 0; j < TM; ++j) {
+        if (m0 + (wm * TM + j) * 16 >= p.M) break;  // rows that the join does not read either
 #pragma unroll
-        for (int j = 0; j < TM; ++j) at[(i * TM + j) * 64] = acc[i][j];
+        for (int i = 0; i < TN; ++i) at[(i * TM + j) * 64] = acc[i][j];
+      }
       return;
     }
   }
@@ -353,21 +355,29 @@ template <class T>
 __global__ __launch_bounds__(64) void linear_join_kernel(LinearParams p, int ntn, int tiles, int parts) {
   const int lane = (int)threadIdx.x;
   const int tile = (int)blockIdx.x >> 3, wave = (int)blockIdx.x >> 1 & 3, j = (int)blockIdx.x & 1;
+  const int64_t m16 = (int64_t)(tile / ntn) * 64 + (wave >> 1) * 32 + j * 16, m = m16 + (lane & 15);
+  if (m16 >= p.M) return;
   const float4_t* at = reinterpret_cast<const float4_t*>(p.partial) + (int64_t)(tile * 4 + wave) * 256 + j * 64 + lane;
-  const int64_t m = (int64_t)(tile / ntn) * 64 + (wave >> 1) * 32 + j * 16 + (lane & 15);
   const int n = tile % ntn * 64 + (wave & 1) * 32 + (lane >> 4) * 8;
-  Columns<T, 8> cols[1];
+  Columns<T, 8> cols;
   RowScales<T, 1, 16> rscales;
-  cols[0].load(p, n);
+  cols.load(p, n);
   rscales.load(p, m);
-  float4_t acc[2][1] = {{at[0]}, {at[128]}};
+  by_output(p, [&](auto o, auto vec) {
+    using O = decltype(o);
+    constexpr bool VEC = decltype(vec)::value;
+    Raw<O, 8> res[1];  // on its way beside the parts
+    linear_residual<O, VEC, 1, 16, 8>(p, m, n, res);
+    float4_t lo = at[0], hi = at[128];
 #pragma unroll 8
-  for (int q = 1; q < parts; ++q) {
-    const float4_t* part = at + (int64_t)q * tiles * 4 * 256;
-    acc[0][0] += part[0];
-    acc[1][0] += part[128];
-  }
-  linear_epilogue<T, 1, 2>(p, m, n, acc, cols, rscales);
+    for (int q = 1; q < parts; ++q) {
+      const float4_t* part = at + (int64_t)q * tiles * 4 * 256;
+      lo += part[0];
+      hi += part[128];
+    }
+    float v[1][8] = {{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+    linear_finish<T, O, VEC, 1, 16, 8>(p, m, n, v, cols, rscales, res);
+  });
 }
 
 }  // namespace sengine

@@ -34,8 +34,9 @@ def random_reader_params(seed: int = 0, embed: int = 384, depth: int = 2, mlp_ra
     def w(n, k):
         return torch.randn((n, k), generator=g) / math.sqrt(k)
 
-    p = {"queries": torch.randn((queries, embed), generator=g), "norm.weight": 1 + 0.1 * torch.randn(embed, generator=g),
-         "head.weight": w(num_classes, embed), "head.bias": 0.1 * torch.randn(num_classes, generator=g)}
+    p = {"queries": torch.randn((queries, embed), generator=g),
+         "norm.weight": 1 + 0.1 * torch.randn(embed, generator=g), "head.weight": w(num_classes, embed),
+         "head.bias": 0.1 * torch.randn(num_classes, generator=g)}
     for i in range(depth):
         pre = f"block.{i}."
         for n, (rows, cols) in {"q": (embed, embed), "kv": (2 * embed, embed), "out": (embed, embed),

@@ -61,7 +61,41 @@ struct RowReduce {
   }
 };
 
-template <class T, class OUT, int L, int NV, int VEC>
+// N values at p as floats, of which `left` are there; zeros beyond.  WHOLE: all are, at a multiple of their size;
+// otherwise a whole piece is still one access, of whatever alignment.
+template <bool WHOLE, class T, int N>
+__device__ __forceinline__ void load_piece(const T* p, int left, float (&v)[N]) {
+  if constexpr (WHOLE) {
+    load_floats<T, N>(p, v);
+  } else if (left >= N) {
+    typedef T vec_t __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    const vec_t x = *reinterpret_cast<const vec_t*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (float)x[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+  }
+}
+
+template <bool WHOLE, class T, int N>
+__device__ __forceinline__ void store_piece(T* p, int left, const float (&v)[N]) {
+  if constexpr (WHOLE) {
+    store_floats(p, v);
+  } else {
+    alignas(16) T x[N];
+    store_floats(x, v);
+    if (left >= N) {
+      __builtin_memcpy(p, x, sizeof(x));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i < left) p[i] = x[i];
+    }
+  }
+}
+
+template <class T, class OUT, int L, int NV, int VEC, bool WHOLE>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(RmsParams p) {
   constexpr int NTH = L < 256 ? 256 : L;
   __shared__ float lds[L > 64 ? L / 64 : 1];
@@ -76,7 +110,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(RmsParams p
   for (int j = 0; j < NV; ++j) {
     const int at = (j * L + lane) * VEC;
     if (at < p.D) {
-      load_floats<T, VEC>(x + at, v[j]);
+      load_piece<WHOLE>(x + at, p.D - at, v[j]);
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[j][i] = 0.f;
@@ -88,7 +122,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(RmsParams p
       const int at = (j * L + lane) * VEC;
       if (at < p.D) {
         float r[VEC];
-        load_floats<T, VEC>(res + at, r);
+        load_piece<WHOLE>(res + at, p.D - at, r);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[j][i] += r[i];
       }
@@ -104,7 +138,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(RmsParams p
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int at = (j * L + lane) * VEC;
-      if (at < p.D) store_floats<T, VEC>(st + at, v[j]);
+      if (at < p.D) store_piece<WHOLE>(st + at, p.D - at, v[j]);
     }
   }
   const float rstd = 1.0f / sqrtf(ss / (float)p.D + p.eps);
@@ -118,9 +152,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(RmsParams p
 #pragma unroll
         for (int i = 0; i < VEC; ++i) w[i] = 1.f;
       } else if (p.w_type == SENGINE_ENC_F32) {
-        load_floats<float, VEC>(static_cast<const float*>(p.w) + at, w);
+        load_piece<WHOLE>(static_cast<const float*>(p.w) + at, p.D - at, w);
       } else {
-        load_floats<T, VEC>(static_cast<const T*>(p.w) + at, w);
+        load_piece<WHOLE>(static_cast<const T*>(p.w) + at, p.D - at, w);
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -143,44 +177,43 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(RmsParams p
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int at = (j * L + lane) * VEC;
-    if (at < p.D) store_floats(out + at, v[j]);
+    if (at < p.D) store_piece<WHOLE>(out + at, p.D - at, v[j]);
   }
 }
 
-template <class T, class OUT, int L, int NV, int VEC>
+template <class T, class OUT, int L, int NV, bool WHOLE>
 static hipError_t run(const RmsParams& p, hipStream_t stream) {
-  constexpr int NTH = L < 256 ? 256 : L;
+  constexpr int NTH = L < 256 ? 256 : L, VEC = 16 / (int)sizeof(T);
   const int64_t wgs = (p.rows + NTH / L - 1) / (NTH / L);
-  rms_norm_kernel<T, OUT, L, NV, VEC><<<dim3((unsigned)wgs), dim3(NTH), 0, stream>>>(p);
+  rms_norm_kernel<T, OUT, L, NV, VEC, WHOLE><<<dim3((unsigned)wgs), dim3(NTH), 0, stream>>>(p);
   return hipGetLastError();
 }
 
-// Lanes per row by the pieces a row has: 16 lanes for up to 64 pieces (four rows a wave: a 384-wide
+// Lanes per row by the pieces of 16 bytes a row has: 16 lanes for up to 64 pieces (four rows a wave: a 384-wide
 // 16-bit row is 48 pieces, 3 a lane with none idle), a wave up to 256, then a workgroup.
-template <class T, class OUT, int VEC>
+template <class T, class OUT, bool WHOLE>
 static hipError_t by_width(const RmsParams& p, hipStream_t stream) {
+  constexpr int VEC = 16 / (int)sizeof(T);
   const int n = (p.D + VEC - 1) / VEC;
-  if (n <= 16) return run<T, OUT, 16, 1, VEC>(p, stream);
-  if (n <= 32) return run<T, OUT, 16, 2, VEC>(p, stream);
-  if (n <= 48) return run<T, OUT, 16, 3, VEC>(p, stream);
-  if (n <= 64) return run<T, OUT, 16, 4, VEC>(p, stream);
-  if (n <= 128) return run<T, OUT, 64, 2, VEC>(p, stream);
-  if (n <= 192) return run<T, OUT, 64, 3, VEC>(p, stream);
-  if (n <= 256) return run<T, OUT, 64, 4, VEC>(p, stream);
-  if (n <= 512) return run<T, OUT, 256, 2, VEC>(p, stream);
-  if (n <= 1024) return run<T, OUT, 256, 4, VEC>(p, stream);
-  if (n <= 4096) return run<T, OUT, 1024, 4, VEC>(p, stream);
-  if constexpr (VEC <= 4) {
-    if (n <= 8192) return run<T, OUT, 1024, 8, VEC>(p, stream);
-  }
-  if constexpr (VEC == 1) return run<T, OUT, 1024, 32, VEC>(p, stream);
+  if (n <= 16) return run<T, OUT, 16, 1, WHOLE>(p, stream);
+  if (n <= 32) return run<T, OUT, 16, 2, WHOLE>(p, stream);
+  if (n <= 48) return run<T, OUT, 16, 3, WHOLE>(p, stream);
+  if (n <= 64) return run<T, OUT, 16, 4, WHOLE>(p, stream);
+  if (n <= 128) return run<T, OUT, 64, 2, WHOLE>(p, stream);
+  if (n <= 192) return run<T, OUT, 64, 3, WHOLE>(p, stream);
+  if (n <= 256) return run<T, OUT, 64, 4, WHOLE>(p, stream);
+  if (n <= 512) return run<T, OUT, 256, 2, WHOLE>(p, stream);
+  if (n <= 1024) return run<T, OUT, 256, 4, WHOLE>(p, stream);
+  if (n <= 4096) return run<T, OUT, 1024, 4, WHOLE>(p, stream);
+  if constexpr (VEC == 4) return run<T, OUT, 1024, 8, WHOLE>(p, stream);
   return hipErrorInvalidValue;  // not reached: D <= kRmsMaxD
 }
 
 constexpr int kRmsMaxD = 32768;
 
-// 16-byte pieces where every row of every array begins at a multiple of its piece and D is whole
-// pieces, else single elements.
+// Whole aligned pieces where every row of every array begins at a multiple of its piece and D is whole pieces.
+// Otherwise (bf16, 43984 x 1445 with a residual: 118 us, element by element 358) a row's pieces begin anywhere and
+// its last may be short.
 template <class T, class OUT>
 static hipError_t by_alignment(const RmsParams& p, hipStream_t stream) {
   constexpr int VEC = 16 / (int)sizeof(T);
@@ -191,8 +224,8 @@ static hipError_t by_alignment(const RmsParams& p, hipStream_t stream) {
   if (p.D % VEC == 0 && fits(p.x, p.x_stride, e) && fits(p.res, p.res_stride, e) &&
       fits(p.stream, p.stream_stride, e) && fits(p.out, p.out_stride, sizeof(OUT)) &&
       fits(p.w, 0, 16 / VEC))
-    return by_width<T, OUT, VEC>(p, stream);
-  return by_width<T, OUT, 1>(p, stream);
+    return by_width<T, OUT, true>(p, stream);
+  return by_width<T, OUT, false>(p, stream);
 }
 
 template <class T>

@@ -87,6 +87,7 @@ __device__ __forceinline__ void by_activation(int act, F f) {
 template <class O, int NV>
 struct Raw {
   typedef O vec_t __attribute__((ext_vector_type(NV), aligned(NV * sizeof(O) < 16 ? NV * sizeof(O) : 16)));
+  typedef O any_t __attribute__((ext_vector_type(NV), aligned(sizeof(O))));  // the same at any element
   vec_t v;
 };
 
@@ -102,6 +103,8 @@ __device__ __forceinline__ void linear_residual(const LinearParams& p, int64_t m
     const O* at = static_cast<const O*>(p.res) + row * p.res_stride + n;
     if constexpr (VEC) {
       r[u].v = *reinterpret_cast<const typename Raw<O, NV>::vec_t*>(at);
+    } else if (n + NV <= p.N) {
+      r[u].v = *reinterpret_cast<const typename Raw<O, NV>::any_t*>(at);
     } else {
 #pragma unroll
       for (int e = 0; e < NV; ++e)
@@ -173,15 +176,17 @@ __device__ __forceinline__ void linear_finish(const LinearParams& p, int64_t m, 
   for (int u = 0; u < NR; ++u) {
     if (m + STEP * u >= p.M) continue;
     O* at = static_cast<O*>(p.out) + (m + STEP * u) * p.out_stride + n;
-    if constexpr (VEC) {
-      typename Raw<O, NV>::vec_t x;
+    typename Raw<O, NV>::vec_t x;
 #pragma unroll
-      for (int e = 0; e < NV; ++e) x[e] = (O)v[u][e];
+    for (int e = 0; e < NV; ++e) x[e] = (O)v[u][e];
+    if constexpr (VEC) {
       *reinterpret_cast<typename Raw<O, NV>::vec_t*>(at) = x;
+    } else if (n + NV <= p.N) {
+      *reinterpret_cast<typename Raw<O, NV>::any_t*>(at) = x;
     } else {
 #pragma unroll
       for (int e = 0; e < NV; ++e)
-        if (n + e < p.N) at[e] = (O)v[u][e];
+        if (n + e < p.N) at[e] = x[e];
     }
   }
 }

@@ -93,7 +93,8 @@ struct Raw {
 
 // NV columns from n on of NR rows m, m + STEP, ... of the residual.  They are not used before linear_finish, so
 // that all rows' loads are in flight together.  VEC: N is a multiple of 8 and the rows of out and residual begin at
-// multiples of 16 bytes; otherwise values are read and stored one by one.
+// multiples of 16 bytes; otherwise the same accesses begin at any element, and only a row's last columns go one by
+// one (93982 x 377 x 144 bf16 with GELU and a residual: 71 us, all one by one 145).
 template <class O, bool VEC, int NR, int STEP, int NV>
 __device__ __forceinline__ void linear_residual(const LinearParams& p, int64_t m, int n, Raw<O, NV> (&r)[NR]) {
   if (!p.res || n >= p.N) return;

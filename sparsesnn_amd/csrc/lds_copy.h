@@ -7,14 +7,17 @@ namespace sengine {
 // One LDS copy: 64 lanes x 16 bytes from rsrc at each lane's offset to LDS bytes dst..dst + 1023; lanes out of
 // the buffer's range write zeros.  Written as asm so that later LDS reads do not wait for it: the caller waits
 // (vmcnt) and, where other waves copied too, meets them at a barrier.  It returns nothing in registers.
+// A memory instruction reads an SGPR that a VALU instruction wrote only five wait states later, and the descriptor
+// comes from one (v_readfirstlane, or v_readlane where it was spilled): the compiler, which does not see the load,
+// cannot put them, so the move and the s_nop are those five.
 __device__ __forceinline__ void lds_copy(u32x4_t rsrc, uint32_t dst, int voff) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
+      "s_nop 3\n\t"
       "buffer_load_dwordx4 %1, %2, 0 offen lds"
       :
       : "s"(dst), "v"(voff), "s"(rsrc)
-      : "memory");
+      : "memory", "m0");
 }
 
 __device__ __forceinline__ uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }

@@ -133,11 +133,13 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
   const int64_t kend = spans * (part + 1) / p.parts * 64;
   const int k1 = kend < n ? (int)kend : n;
 
-  // the rows' queries as matrix operands; a negative scale goes into their sign
+  // the rows' queries as matrix operands; a negative scale goes into their sign, and one of zero makes them zeros (or
+  // NaN, where they are infinite or NaN): with cs = 0 the places past the end, which score -infinity, would be NaN
   const int row0 = (block * C::WPH + (SHARED ? wave % C::WPH : 0)) * 16 * QF;
   u32x4_t q[QF][DK];
   const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
-  const float cs = fabsf(p.scale) * 1.4426950408889634f;
+  const bool flat = p.scale == 0.f;
+  const float cs = flat ? 1.f : fabsf(p.scale) * 1.4426950408889634f;
 #pragma unroll
   for (int f = 0; f < QF; ++f) {
     const int row = row0 + 16 * f + c;
@@ -150,6 +152,13 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
         q[f][t] = *reinterpret_cast<const u32x4_t*>(at + 32 * t + 8 * g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[f][t][i] ^= flip;
+        if (flat) {
+          typedef T vec8_t __attribute__((ext_vector_type(8)));
+          vec8_t x = __builtin_bit_cast(vec8_t, q[f][t]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = (T)((float)x[i] * 0.f);
+          q[f][t] = __builtin_bit_cast(u32x4_t, x);
+        }
       }
     }
   }

@@ -878,6 +878,14 @@ def _token_input(t, name: str, device=None):
                            "(call them under torch.no_grad())")
 
 
+def _token_number(x, name: str) -> float:
+    """eps or scale as the number it is at the call (a tensor's value may be another one at the next), to 32 bits."""
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+        raise SEngineError(f"{name} requires a gradient: the token operators are inference only "
+                           "(call them under torch.no_grad())")
+    return ctypes.c_float(x).value
+
+
 def _token_rows(t: torch.Tensor, name: str):
     """(rows, row stride in elements) of (..., width), whose rows must lie evenly spaced."""
     if t.is_contiguous():
@@ -975,6 +983,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
     (y, stream, scale): y's codes and one fp32 scale a row (shape x.shape[:-1]), y ~ codes * scale.
     stream is s rounded to x's type, None without a residual.  `out`, `stream_out` (which may be
     `residual`, updated in place) and `scale` take the results where given."""
+    if type(eps) is not float:
+        eps = _token_number(eps, "eps")
     key = None
     if out is None and stream_out is None and scale is None:
         try:
@@ -1142,6 +1152,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
     as they are.  Scores, their maximum and sums are fp32; the weights are rounded to q's type for
     the product with v.  Few queries of many keys are computed in parts of the keys through scratch
     memory of torch's allocator, the parts joined in a fixed order."""
+    if scale is not None and type(scale) is not float:
+        scale = _token_number(scale, "scale")
     key = None
     if out is None:
         try:

@@ -886,6 +886,12 @@ def _token_number(x, name: str) -> float:
     return ctypes.c_float(x).value
 
 
+def _token_sizes(what: str, *sizes):
+    """Sizes that the descriptors hold in 32 bits; ctypes would cut them without a word."""
+    if max(sizes) >= 2**31:
+        raise SEngineError(f"{what} must be under 2**31, got {', '.join(map(str, sizes))}")
+
+
 def _token_rows(t: torch.Tensor, name: str):
     """(rows, row stride in elements) of (..., width), whose rows must lie evenly spaced."""
     if t.is_contiguous():
@@ -943,6 +949,7 @@ def _rms_norm_plan(key, x, weight, residual, eps, out_dtype, out, stream_out, sc
     if x.dim() == 0:
         raise SEngineError("x: expected (..., D)")
     shape, D = x.shape, x.shape[-1]
+    _token_sizes("rms_norm: D", D)
     rows, xs = _token_rows(x, "x")
     rs = ws = 0
     if residual is not None:
@@ -1020,6 +1027,7 @@ def _linear_plan(key, x, weight, bias, activation, residual, x_scale, weight_sca
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
     N, K = weight.shape
+    _token_sizes("linear: N and K", N, K)
     M, xs = _token_rows(x, "x")
     wst = _token_rows(weight, "weight")[1]
     eight = code == ENC_E4M3
@@ -1104,6 +1112,7 @@ def _cross_plan(key, q, k, v, scale, key_lengths, key_mask, out):
                            f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, Lq, Hq, d = q.shape
     Lk, Hkv = k.shape[1], k.shape[2]
+    _token_sizes("cross_attention: B, Lq, Lk, heads and d", B, Lq, Lk, Hq, Hkv, d)
     if out is not None:
         if not isinstance(out, torch.Tensor):
             raise TypeError("out must be a torch.Tensor")

@@ -93,10 +93,12 @@ static LinearPlan plan(const LinearParams& p, bool wide) {
   constexpr int kCUs = 256;
   const int steps = (p.kbytes + kLinStep - 1) / kLinStep;
   if (p.M <= 16) return {kLinRows, 1, 0};
-  // LDS copies: whole 16-byte pieces, offsets inside a tile in 31 bits
+  // LDS copies: whole 16-byte pieces, offsets inside a tile in 31 bits and from its first row on (rows may lie
+  // backwards in memory: the other kernels take any stride)
+  const auto near = [](int64_t stride) { return stride >= 0 && stride < 1 << 22; };
   const bool copies = p.kbytes % 16 == 0 && p.x_stride % 16 == 0 && p.w_stride % 16 == 0 &&
                       (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.w % 16 == 0 && p.kbytes < (1 << 29) &&
-                      p.x_stride < (1 << 22) && p.w_stride < (1 << 22);
+                      near(p.x_stride) && near(p.w_stride);
   if (!copies) return {kLinAny, 1, 0};
   if (!wide && tiles_of(p, 256) >= kCUs && steps >= 8) return {kLin256, 1, 0};
   if (tiles_of(p, 128) >= kCUs) return {kLin128, 1, 0};

@@ -21,6 +21,12 @@ struct LinearParams {
   int vec;               // N is a multiple of 8, out and res rows begin at multiples of 16 bytes
 };
 
+// Where the 128-byte step after the one at k begins, and whether there is one (rows go up to 2^31 - 1 bytes, past which
+// a step at 2^31 lies: unsigned), and whether the row has all of its 16-byte piece at k, which lies inside it.
+__host__ __device__ inline bool has_step(uint32_t k, int kbytes) { return k < (uint32_t)kbytes; }
+__host__ __device__ inline uint32_t next_step(uint32_t k) { return k + 128; }
+__host__ __device__ inline bool whole_piece(int k, int kbytes) { return kbytes - k >= 16; }
+
 template <int V>
 struct Int {
   static constexpr int value = V;

@@ -28,7 +28,8 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
     for (int j = 0; j < 2; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
 
   const int row = tid >> 3, piece = (tid & 7) * 16;  // rows row and row + 32 of each operand
-  for (int k = 0; k < p.kbytes; k += kLinStep) {
+  for (uint32_t at = 0; has_step(at, p.kbytes); at = next_step(at)) {
+    const int k = (int)at;
     u32x4_t xv[2], wv[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -91,7 +92,7 @@ static int64_t tiles_of(const LinearParams& p, int b) { return (p.M + b - 1) / b
 
 static LinearPlan plan(const LinearParams& p, bool wide) {
   constexpr int kCUs = 256;
-  const int steps = (p.kbytes + kLinStep - 1) / kLinStep;
+  const int steps = p.kbytes / kLinStep + (p.kbytes % kLinStep != 0);
   if (p.M <= 16) return {kLinRows, 1, 0};
   // LDS copies: whole 16-byte pieces, offsets inside a tile in 31 bits and from its first row on (rows may lie
   // backwards in memory: the other kernels take any stride)

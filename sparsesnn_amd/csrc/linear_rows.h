@@ -14,7 +14,7 @@ namespace sengine {
 __device__ __forceinline__ u32x4_t fetch_piece(const uint8_t* base, int k, int kbytes) {
   u32x4_t v = u32x4_t{0, 0, 0, 0};
   if (k >= kbytes) return v;
-  if (k + 16 <= kbytes) {
+  if (whole_piece(k, kbytes)) {
     __builtin_memcpy(&v, base + k, 16);
     return v;
   }

@@ -87,6 +87,13 @@ struct CrossPlan {
   int parts;
 };
 
+// Keys and query rows (of all sequences and heads) that the kernels' counts hold.
+static bool keys_fit(const sengine_cross_desc* d) { return d->Lk <= 0x3fffffff; }
+static bool rows_fit(const sengine_cross_desc* d) {
+  const int64_t queries = (int64_t)d->B * d->Lq;
+  return queries <= 0x7fffffff && queries * d->Hq <= 0x7fffffff;
+}
+
 static CrossPlan plan(const sengine_cross_desc* d) {
   const int64_t rows = (int64_t)d->Lq * (d->Hq / d->Hkv);
   const auto wgs_of = [&](int r) { return (int64_t)d->B * d->Hkv * ((rows + r - 1) / r); };
@@ -98,7 +105,7 @@ static CrossPlan plan(const sengine_cross_desc* d) {
   else if (rows > 16)
     q.rows_a_block = 64;
   if (rows <= 64 && d->d <= 48 && d->d % 16 == 0 && d->Hkv % 4 == 0 && d->k_stride[2] == d->d &&
-      d->v_stride[2] == d->d && (int64_t)d->B * d->Lk * d->Hkv * d->d >= 1 << 24)
+      d->v_stride[2] == d->d && (double)d->B * d->Lk * d->Hkv * d->d >= 1 << 24)
     q.heads = 4;
   const int64_t wgs = (int64_t)d->B * (d->Hkv / q.heads) * ((rows + q.rows_a_block - 1) / q.rows_a_block);
   constexpr int64_t kWant = 2 * kCUs;  // workgroups
@@ -186,8 +193,8 @@ extern "C" int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const
     return set_error(-2, "cross_attention: the head size must be a multiple of 8 up to 128");
   if (d->type != SENGINE_ENC_F16 && d->type != SENGINE_ENC_BF16)
     return set_error(-2, "cross_attention: q, k and v must be fp16 or bf16");
-  if (d->Lk > 0x3fffffff) return set_error(-2, "cross_attention: more than 2^30 keys");
-  if ((int64_t)d->B * d->Lq * d->Hq > 0x7fffffffll) return set_error(-2, "cross_attention: too many query rows");
+  if (!keys_fit(d)) return set_error(-2, "cross_attention: more than 2^30 keys");
+  if (!rows_fit(d)) return set_error(-2, "cross_attention: too many query rows");
   if (d->B == 0 || d->Lq == 0) return 0;
   if (!q || !out || (d->Lk > 0 && (!k || !v))) return set_error(-1, "cross_attention: null q, k, v or out");
   CrossParams p{};
@@ -239,7 +246,9 @@ extern "C" int sengine_amd_cross_attention(const sengine_cross_desc* d, const vo
 extern "C" int sengine_amd_cross_attention_workspace(const sengine_cross_desc* d, size_t* bytes) {
   if (!d || !bytes) return set_error(-1, "cross_attention_workspace: null argument");
   *bytes = 0;
-  if (d->B < 1 || d->Lq < 1 || d->Lk < 1 || d->Hkv < 1 || d->Hq < d->Hkv || d->d < 8) return 0;
+  if (d->B < 1 || d->Lq < 1 || d->Lk < 1 || d->Hkv < 1 || d->Hq < d->Hkv || d->d < 8 || d->d > 128 ||
+      !keys_fit(d) || !rows_fit(d))
+    return 0;  // nothing to do, or refused by the entry
   const int parts = plan(d).parts;
   if (parts > 1) *bytes = cross_workspace(d, parts);
   return 0;

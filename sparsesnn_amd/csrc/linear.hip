@@ -88,7 +88,14 @@ struct LinearPlan {
   int kernel, parts, part_steps;
 };
 
-static int64_t tiles_of(const LinearParams& p, int b) { return (p.M + b - 1) / b * ((p.N + b - 1) / b); }
+static int64_t tiles_of(const LinearParams& p, int b) { return (p.M + b - 1) / b * (((int64_t)p.N + b - 1) / b); }
+
+// Sizes that the kernels' counts hold: a row in 31 bits of bytes, a column in 31 bits up to the end of its tile, the
+// 64 x 64 tiles in 31 bits.
+static bool sizes_fit(const sengine_linear_desc* d) {
+  return d->K <= 0x3fffffff && d->N <= 0x7fffff00 && d->M <= 64ll * 0x7fffffff &&
+         (d->M + 63) / 64 * (((int64_t)d->N + 63) / 64) <= 0x7fffffff;
+}
 
 static LinearPlan plan(const LinearParams& p, bool wide) {
   constexpr int kCUs = 256;
@@ -160,8 +167,7 @@ extern "C" int sengine_amd_linear_ws(const sengine_linear_desc* d, const void* x
   if (d->activation < SENGINE_ACT_NONE || d->activation > SENGINE_ACT_SILU)
     return set_error(-2, "linear: unknown activation");
   if (!e4m3 && (x_scale || weight_scale)) return set_error(-2, "linear: scales go with e4m3 operands only");
-  const int64_t mtiles = (d->M + 63) / 64, ntiles = ((int64_t)d->N + 63) / 64;
-  if (d->K > 0x3fffffff || mtiles * ntiles > 0x7fffffffll) return set_error(-2, "linear: sizes too large");
+  if (!sizes_fit(d)) return set_error(-2, "linear: sizes too large");
   if (d->M == 0) return 0;
   if (!out || (d->K > 0 && (!x || !weight))) return set_error(-1, "linear: null x, weight or out");
   if (d->M > 1 && d->out_stride < d->N) return set_error(-2, "linear: output rows overlap");
@@ -211,7 +217,7 @@ extern "C" int sengine_amd_linear(const sengine_linear_desc* d, const void* x, c
 extern "C" int sengine_amd_linear_workspace(const sengine_linear_desc* d, size_t* bytes) {
   if (!d || !bytes) return set_error(-1, "linear_workspace: null argument");
   *bytes = 0;
-  if (d->M < 1 || d->N < 1 || d->K < 1 || d->K > 0x3fffffff) return 0;
+  if (d->M < 1 || d->N < 1 || d->K < 1 || !sizes_fit(d)) return 0;  // nothing to do, or refused by the entry
   const int e = type_bytes(d->in_type);
   LinearParams p{};
   p.M = d->M;

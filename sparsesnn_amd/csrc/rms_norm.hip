@@ -181,12 +181,27 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(RmsParams p
   }
 }
 
+// A launch holds fewer than 2^32 threads: 2^28 rows of 16 lanes and more go in several.
+constexpr int64_t kRmsThreads = 1ll << 31;  // of a launch
+
 template <class T, class OUT, int L, int NV, bool WHOLE>
-static hipError_t run(const RmsParams& p, hipStream_t stream) {
+static hipError_t run(RmsParams p, hipStream_t stream) {
   constexpr int NTH = L < 256 ? 256 : L, VEC = 16 / (int)sizeof(T);
-  const int64_t wgs = (p.rows + NTH / L - 1) / (NTH / L);
-  rms_norm_kernel<T, OUT, L, NV, VEC, WHOLE><<<dim3((unsigned)wgs), dim3(NTH), 0, stream>>>(p);
-  return hipGetLastError();
+  constexpr int64_t kMost = kRmsThreads / L;  // rows of a launch
+  const int64_t rows = p.rows;
+  for (int64_t first = 0; first < rows; first += kMost) {
+    p.rows = rows - first < kMost ? rows - first : kMost;
+    const int64_t wgs = (p.rows + NTH / L - 1) / (NTH / L);
+    rms_norm_kernel<T, OUT, L, NV, VEC, WHOLE><<<dim3((unsigned)wgs), dim3(NTH), 0, stream>>>(p);
+    const hipError_t rc = hipGetLastError();
+    if (rc != hipSuccess) return rc;
+    p.x = static_cast<const T*>(p.x) + kMost * p.x_stride;
+    if (p.res) p.res = static_cast<const T*>(p.res) + kMost * p.res_stride;
+    if (p.stream) p.stream = static_cast<T*>(p.stream) + kMost * p.stream_stride;
+    p.out = static_cast<OUT*>(p.out) + kMost * p.out_stride;
+    if (p.scale) p.scale += kMost;
+  }
+  return hipSuccess;
 }
 
 // Lanes per row by the pieces of 16 bytes a row has: 16 lanes for up to 64 pieces (four rows a wave: a 384-wide

@@ -488,7 +488,7 @@ int sengine_amd_release_weights(void);
  * Root-mean-square norm with the residual's addition.  Per row: s = x + residual (or x), y =
  * s / sqrt(mean(s^2) + eps) * weight (1 where null).  stream_out (or null) receives s and out
  * receives y, both in x's type; with out_type = SENGINE_ENC_E4M3 out receives y / c as e4m3 and
- * scale[row] = c = max|y| / 448 (1 for a row of zeros).  Everything before a store is fp32; y is
+ * scale[row] = c = max|y| / 448, at least 2^-126 (1 for a row of zeros).  Everything before a store is fp32; y is
  * formed from the unrounded s.  residual and stream_out are of x's type, weight of x's type or
  * fp32.  1 <= D <= 32768, rows < 2^31; an output may be the input it has the rows of.
  */

@@ -2,7 +2,7 @@
 //   s = x + r              (stored, rounded once, as the new stream when the caller wants it)
 //   y = s / sqrt(mean(s^2) + eps) * w
 // y is stored in x's type, or as e4m3 codes q with one fp32 scale c a row, y ~ q * c:
-//   c = max |y| / 448 (1 for a row of zeros), q = e4m3(y / c).
+//   c = max |y| / 448, at least 2^-126 (1 for a row of zeros), q = e4m3(y / c).
 // s, the sum of squares and y are fp32; y is rounded once, when it is stored.
 //
 // Bandwidth bound: x and r are read once and y and s written once, because a row stays in
@@ -166,7 +166,10 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_kernel(RmsParams p
   }
   if constexpr (__is_same(OUT, E4m3)) {
     top = RowReduce<L>::largest(top, lds);
-    const float c = top == 0 ? 1.f : __builtin_bit_cast(float, top) / 448.f;
+    // a quotient below the normal numbers has lost bits, or all of them: codes of the smallest normal scale instead
+    constexpr float kLeast = 1.17549435e-38f;
+    const float quotient = __builtin_bit_cast(float, top) / 448.f;
+    const float c = top == 0 ? 1.f : quotient < kLeast ? kLeast : quotient;  // a NaN stays
     if (lane == 0) p.scale[row] = c;
 #pragma unroll
     for (int j = 0; j < NV; ++j)

@@ -987,7 +987,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
 
     x is fp16, bf16 or fp32; residual and stream have its shape and type; weight (D,) its type or
     fp32.  Returns (y, stream) with y in x's type, or with out_dtype=torch.float8_e4m3fn
-    (y, stream, scale): y's codes and one fp32 scale a row (shape x.shape[:-1]), y ~ codes * scale.
+    (y, stream, scale): y's codes and one fp32 scale a row (shape x.shape[:-1]), y ~ codes * scale, which is
+    max|y| / 448, at least 2**-126 and 1 for a row of zeros.
     stream is s rounded to x's type, None without a residual.  `out`, `stream_out` (which may be
     `residual`, updated in place) and `scale` take the results where given."""
     if type(eps) is not float:

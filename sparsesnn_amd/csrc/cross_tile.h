@@ -4,7 +4,8 @@
 // workgroup takes 16 QF rows a wave of one sequence and key head and a range of its keys, KT keys at a time:
 //   S = K Q^T    matrix instructions, keys x rows: a lane has 4 keys a fragment of one row
 //   P            exponentials against the row's reference maximum, which is raised (and the sums rescaled)
-//                only when a score passes it by 2^8: the result does not depend on the reference
+//                only when a score passes it by 2^8: the result does not depend on the reference.  fp16 weights are
+//                those times 2^7: up to 2^15, and down to 2^-31 of the reference before they are lost (kWeightShift)
 //   O^T += V^T P^T   the P a lane has is the operand as it lies: the order of the reduction's keys over the
 //                lanes is free as long as V's operand, read from LDS transposed, has the same
 // K and V are copied into LDS by buffer loads, S tiles in flight.  SHARED: all waves work on the same tile
@@ -51,6 +52,12 @@ struct CrossParams {
 };
 
 constexpr int kCrossList = 4096;  // keys of a mask at a time
+
+// The weights are rounded to T for the product with V.  fp16 ends at 2^-24, and many keys that far below the largest
+// weigh something together (2^20 keys, 2^-26 each: 1.5 %): the exponent is moved up by what the raised reference leaves
+// of the type's range.  It cancels in the division by the sum.  bf16 has fp32's range.
+template <class T>
+constexpr float kWeightShift = __is_same(T, _Float16) ? 7.f : 0.f;
 
 template <class T>
 __device__ __forceinline__ float4_t mma_16(u32x4_t a, u32x4_t b, float4_t c) {
@@ -362,7 +369,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void cross_tile_kernel(CrossParams p)
         }
 #pragma unroll
         for (int f = 0; f < QF; ++f) {
-          const float ref = top[f] == -INFINITY ? 0.f : -top[f];  // every score so far is -infinity: they weigh nothing
+          // (every score so far is -infinity: they weigh nothing)
+          const float ref = top[f] == -INFINITY ? 0.f : kWeightShift<T> - top[f];
 #pragma unroll
           for (int u = 0; u < KT / 32; ++u) {
             typedef T vec8_t __attribute__((ext_vector_type(8)));

@@ -214,11 +214,13 @@ extern "C" int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const
   p.group = d->Hq / d->Hkv;
   p.rows = d->Lq * p.group;
   if ((uintptr_t)workspace % 16) return set_error(-2, "cross_attention: the workspace must be aligned to 16 bytes");
-  // the tile kernel: rows of d values that begin at multiples of 16 bytes, offsets in a stretch of keys in 31 bits
+  // the tile kernel: rows of d values that begin at multiples of 16 bytes, offsets in 31 bits: of a stretch's 4096 keys
+  // with a mask, of a tile's 64 without one (whose base moves from tile to tile)
   const auto aligned = [](const void* a, const int64_t* s) {
     return (uintptr_t)a % 16 == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
   };
-  const auto near = [](int64_t s) { return s >= 0 && s <= 0x3ffff; };
+  const int64_t most = key_mask ? 0x3ffff : 0xffffff;
+  const auto near = [&](int64_t s) { return s >= 0 && s <= most; };
   if (aligned(q, d->q_stride) && aligned(k, d->k_stride) && aligned(v, d->v_stride) && aligned(out, d->out_stride) &&
       near(p.k_l) && near(p.v_l)) {
     const CrossPlan plan_ = plan(d);

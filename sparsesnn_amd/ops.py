@@ -14,6 +14,7 @@ from dataclasses import dataclass, replace
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import (ACTIVATIONS, ENC_BF16, ENC_BITS, ENC_E4M3, ENC_F16, ENC_F32, NEURON_IF, NEURON_LIF, NEURON_MS,
@@ -858,6 +859,22 @@ _TOKEN_TYPES = {torch.float16: ENC_F16, torch.bfloat16: ENC_BF16, torch.float32:
                 torch.float8_e4m3fn: ENC_E4M3}
 
 
+_NOT_RECORDED = ("the token operators cannot be recorded by a tracer, which would see their outputs' allocation only "
+                 "(capture a HIP graph instead)")
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+
+
+def _token_modes(*args):
+    """What a call refuses that its arguments' layouts do not show: tangents of forward-mode differentiation (there is no
+    rule for them, and no_grad does not turn them off), and a recording by torch.fx."""
+    for t in args:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise SEngineError("an input has a tangent: the token operators are inference only "
+                               "(call them outside of forward_ad.dual_level())")
+    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise SEngineError(_NOT_RECORDED)
+
+
 def _type_code(t: torch.Tensor, allowed, name: str) -> int:
     if t.dtype not in allowed:
         raise SEngineError(f"{name}: expected dtype {' or '.join(str(d) for d in allowed)}, got {t.dtype}")
@@ -869,6 +886,8 @@ def _token_input(t, name: str, device=None):
     (these operators have no backward; it is refused rather than cut off)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
+    if torch.jit.is_tracing():  # shapes are tensors then, so that no call is found among the remembered ones
+        raise SEngineError(_NOT_RECORDED)
     if not t.is_cuda:
         raise SEngineError(f"{name} must be on a HIP device (got {t.device})")
     if device is not None and t.device != device:
@@ -991,6 +1010,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
     max|y| / 448, at least 2**-126 and 1 for a row of zeros.
     stream is s rounded to x's type, None without a residual.  `out`, `stream_out` (which may be
     `residual`, updated in place) and `scale` take the results where given."""
+    if _dispatch_modes() or forward_ad._current_level >= 0:
+        _token_modes(x, weight, residual, eps)
     if type(eps) is not float:
         eps = _token_number(eps, "eps")
     key = None
@@ -1077,6 +1098,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     (..., N) has out_dtype, bias (N,) fp16, bf16 or fp32; `out` may be `residual`.  A long reduction
     with few results is computed in parts through scratch memory of torch's allocator, the parts
     added in a fixed order."""
+    if _dispatch_modes() or forward_ad._current_level >= 0:
+        _token_modes(x, weight, bias, residual, x_scale, weight_scale)
     key = None
     if out is None:
         try:
@@ -1162,6 +1185,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
     as they are.  Scores, their maximum and sums are fp32; the weights are rounded to q's type for
     the product with v.  Few queries of many keys are computed in parts of the keys through scratch
     memory of torch's allocator, the parts joined in a fixed order."""
+    if _dispatch_modes() or forward_ad._current_level >= 0:
+        _token_modes(q, k, v, scale)
     if scale is not None and type(scale) is not float:
         scale = _token_number(scale, "scale")
     key = None

@@ -75,7 +75,7 @@ class TokenReader:
             self.depth += 1
         self.fc1 = None
         if eight_bit:
-            self.fc1 = [e4m3_rows(params[f"block.{i}.fc1.weight"].to(dev)) for i in range(self.depth)]
+            self.fc1 = [e4m3_rows(params[f"block.{i}.fc1.weight"].detach().to(dev)) for i in range(self.depth)]
 
     def encode(self, tokens: torch.Tensor):
         """Every block's (keys, values) of the tokens (B, N, C): each (B, N, heads, C / heads)."""

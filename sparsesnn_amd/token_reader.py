@@ -82,11 +82,12 @@ class TokenReader:
         if tokens.dim() != 3 or tokens.shape[-1] != self.embed:
             raise SEngineError(f"encode: expected (B, N, {self.embed}), got {tuple(tokens.shape)}")
         B, N, C = tokens.shape
+        d = C // self.heads
         memory = []
         for i in range(self.depth):
             pre = f"block.{i}."
             y, _ = ops.rms_norm(tokens, self.p[pre + "norm_kv.weight"], eps=self.eps)
-            kv = ops.linear(y, self.p[pre + "kv.weight"], self.p[pre + "kv.bias"]).view(B, N, 2, self.heads, -1)
+            kv = ops.linear(y, self.p[pre + "kv.weight"], self.p[pre + "kv.bias"]).view(B, N, 2, self.heads, d)
             memory.append((kv[:, :, 0], kv[:, :, 1]))
         return memory
 
@@ -102,7 +103,7 @@ class TokenReader:
             pre = f"block.{i}."
             w = lambda name: (self.p[pre + name + ".weight"], self.p[pre + name + ".bias"])
             y, _ = ops.rms_norm(x, self.p[pre + "norm1.weight"], eps=self.eps)
-            q = ops.linear(y, *w("q")).view(B, Lq, self.heads, -1)
+            q = ops.linear(y, *w("q")).view(B, Lq, self.heads, C // self.heads)
             o = ops.cross_attention(q, k, v, key_lengths=key_lengths, key_mask=key_mask)
             a = ops.linear(o.view(B, Lq, C), *w("out"))
             norm2 = self.p[pre + "norm2.weight"]

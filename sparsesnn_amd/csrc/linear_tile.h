@@ -49,7 +49,7 @@ __device__ __forceinline__ void linear_tile_of(int id, int ntm, int ntn, int& mt
 // with 64 fragments there are no others to move them through.  The compiler knows neither that this is a
 // matrix instruction nor its waits: a and b come from LDS reads (it waits for those by itself), sums of the
 // same fragment follow each other at distances the hardware interlocks, and before anything else reads the
-// sums the caller lets mma_drain pass.
+// sums the caller lets mma_drain pass, which no instruction is scheduled across.
 template <class T, bool ACCUM>  // ACCUM: the sums are in accumulation registers, else in ordinary ones
 __device__ __forceinline__ void mma_inplace(u32x4_t a, u32x4_t b, float4_t& c) {
   if constexpr (__is_same(T, _Float16) && ACCUM)
@@ -68,7 +68,11 @@ __device__ __forceinline__ void mma_inplace(u32x8_t a, u32x8_t b, float4_t& c) {
   else
     asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
 }
-__device__ __forceinline__ void mma_drain() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+__device__ __forceinline__ void mma_drain() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 // A lane's share of a fragment in one step: 16 bytes of each 64-byte half of its row.
 struct Fragment {
@@ -283,8 +287,8 @@ void linear_tile_kernel(LinearParams p, int ntm, int ntn) {
       if (s < steps) step(s, Int<0>{});
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup's use of LDS
+    mma_drain();  // here, where no other path has joined yet: joining may move the sums
   }
-  mma_drain();
   if constexpr (TM * TN == 4) {
     if (p.partial) {  // this part's sums, as the lanes have them
       const int64_t tile = (int64_t)blockIdx.y * ntm * ntn + (int64_t)mt * ntn + nt;

@@ -9,7 +9,10 @@ namespace sengine {
 // (vmcnt) and, where other waves copied too, meets them at a barrier.  It returns nothing in registers.
 // A memory instruction reads an SGPR that a VALU instruction wrote only five wait states later, and the descriptor
 // comes from one (v_readfirstlane, or v_readlane where it was spilled): the compiler, which does not see the load,
-// cannot put them, so the move and the s_nop are those five.
+// cannot put them, so the move and the s_nop are those five.  m0 is named as written, so that no use of the compiler's
+// own is moved across; that it is not saved, which the compiler then warns of, is as it should be.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void lds_copy(u32x4_t rsrc, uint32_t dst, int voff) {
   asm volatile(
       "s_mov_b32 m0, %0\n\t"
@@ -19,6 +22,7 @@ __device__ __forceinline__ void lds_copy(u32x4_t rsrc, uint32_t dst, int voff) {
       : "s"(dst), "v"(voff), "s"(rsrc)
       : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 __device__ __forceinline__ uint32_t scalar(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 

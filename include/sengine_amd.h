@@ -517,9 +517,10 @@ enum {
  * residual[m, n].  x (M, K) and weight (N, K; nn.Linear's layout) are both fp16, both bf16 or both
  * e4m3; the scales (fp32, null = 1) go with e4m3.  out and residual have out_type (fp16, bf16 or
  * fp32), bias has bias_type (one of the same); bias and residual may be null.  The sum and the
- * epilogue are fp32, out is rounded once.  (The 8-bit matrix instructions keep about 16 bits of a
- * sum; e4m3 operands with an fp32 output are multiplied as fp16 instead, at half the rate.)  out may
- * be residual itself.
+ * epilogue are fp32, out is rounded once.  (The 8-bit matrix instructions are off by up to 2^-12 of the
+ * sum of the products' magnitudes; e4m3 operands with an fp32 output are multiplied as fp16 instead, at
+ * half the rate.)  out may be residual itself, and shares no memory with x or weight.  K < 2^30, N <=
+ * 2^31 - 256; input strides may be negative.
  */
 typedef struct sengine_linear_desc {
   int64_t M;
@@ -547,7 +548,8 @@ int sengine_amd_linear_ws(const sengine_linear_desc* d, const void* x, const voi
  * != 0 (bytes; null = all).  A query with no key gets zeros; a key or value that does not count is
  * never used, whatever it holds.  q, k, v and out are fp16 or bf16 with strides per (batch, row,
  * head) in elements and the d values of a head side by side; d is a multiple of 8 up to 128.  A
- * batch stride of 0 shares the encoder's states between the sequences.
+ * batch stride of 0 shares the encoder's states between the sequences.  out may be q itself, and shares
+ * no memory with k or v.  Lk < 2^30, B Lq Hq < 2^31.
  */
 typedef struct sengine_cross_desc {
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];

@@ -8,7 +8,9 @@
 
 namespace sengine {
 
-// Any alignment and any strides: one wave a query row and head, an online softmax over 64 keys at a time, lane j
+// Any alignment and any strides (rows at odd elements, through the C entry only; keys too far apart for a tile's
+// offsets): one query of 1024 masked keys 2^18 elements apart, 128 sequences, 32 heads on 8 x 128: 908 us (the tile
+// kernel without the mask 110), bound by its single-element loads.  One wave a query row and head, an online softmax over 64 keys at a time, lane j
 // forming the dot product of key j, then the lanes sharing the values' columns.
 template <class T>
 __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
@@ -72,14 +74,15 @@ __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
 // Which form, and in how many parts (us, measured as they stand here).
 //   rows of a workgroup (rows: the queries of a key head's group): 16, on waves with tiles of their own, where there
 //     are no more; else the most of 256, 128, 64 that leave a workgroup for every CU, 256 for heads over 64 values
-//     only: 4 x 4096 x 4001, 16 heads x 128: 256 rows 535, 128 rows 668; 4 x 4096 x 4096 x 64: 398 and 384;
-//     1000 x 1000, 8 heads x 64: 26, 21 and with 64 rows 18
+//     only: 4 x 4096 x 4001, 16 heads x 128: 256 rows 481, 128 rows 530; 4 x 4096 x 4096 x 64: 322, 313 and with 64
+//     rows 362; 1000 x 1000, 8 heads x 64: 128 rows 20, 64 rows 15
 //   four key heads together where a head's row is not whole cache lines, up to 48 values, and the time is that of
-//     reading K and V (they pass 64 MB): 64 x 3136, 128 sequences, 8 heads x 48: 113 (alone 166); one query of 196
-//     keys, 4 sequences: 9.4 (alone, with waves of their own: 8)
+//     reading K and V (they pass 64 MB): 64 x 3136, 128 sequences, 8 heads x 48: 113 (alone 164); one query of 196
+//     keys, 4 sequences: 11.6 (alone, with waves of their own: 11.3).  Heads of 16, 32 and 48 values have this form;
+//     others whose rows are not whole lines either (24, 40, 56, 80 ..) are read alone, and were not measured merged
 //   parts of the keys where there are fewer workgroups than CUs, up to two a CU, of 256 keys or more (512 with 64
 //     rows or more): one query of up to 16384 keys, 8 sequences of unequal lengths, 8 key heads x 128: in 8 parts
-//     62, in 16 71, in 12 68
+//     63, in 16 72, in 12 69
 constexpr int kCUs = 256;
 struct CrossPlan {
   int rows_a_block;

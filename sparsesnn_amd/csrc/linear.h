@@ -261,9 +261,10 @@ __device__ __forceinline__ half8_t widen_e4m3(uint32_t lo, uint32_t hi) {
 //
 // The 8-bit instruction does not keep all of a 32-bit sum: its result was measured up to 2^-12 of the
 // sum of the magnitudes off, 1.4e-5 of the result on normally distributed operands (the 16x16x32 8-bit
-// form is the same; the 16-bit ones are within 2^-21).  That is a tenth of an fp16 output's rounding, so
-// 16-bit outputs take it; an fp32 output is computed from the codes widened to fp16 (E4m3Wide), at half
-// the rate, with sums of 32 bits.
+// form is the same; the 16-bit ones are within 2^-21).  For products of random signs that is a tenth of an
+// fp16 output's rounding, so 16-bit outputs take it.  A sum that cancels loses more of its own bits, up to
+// 2^-12 of the magnitudes that went into it.  An fp32 output is computed from the codes widened to fp16
+// (E4m3Wide), at half the rate, with sums of 32 bits.
 typedef int int8v_t __attribute__((ext_vector_type(8)));
 
 // One 64-byte half of that step, for the types whose instruction takes it.

@@ -8,7 +8,8 @@
 
 namespace sengine {
 
-// Any strides, any alignment, any K.  Workgroup = 64 rows x 64 columns, four waves of 32 x 32; per
+// Any strides, any alignment, any K: 8192 x 4096 x 8191 bf16 1410 us (8192 wide 424), since nothing is in flight during
+// the products and the tile is 64 x 64; one operand whose rows are no whole pieces brings a call here.  Workgroup = 64 rows x 64 columns, four waves of 32 x 32; per
 // 128 bytes of the reduction both operands' rows go through registers into LDS: whole 16-byte pieces
 // by one load of whatever alignment, the row's last piece byte by byte, zeros beyond.
 constexpr int kLinPitch = 128 + 16;  // LDS row: 16 bytes more, so that 16 rows' pieces spread over the banks
@@ -75,14 +76,16 @@ static hipError_t run_tile(const LinearParams& p, int parts, hipStream_t stream)
   return hipGetLastError();
 }
 
-// Which kernel, and in how many parts.  Measured (bf16, us, the kernels as they stand here):
-//   up to 16 token rows     1 x 512 x 8192: rows 13, 64 x 64 tiles 30
-//   256 x 256 tiles, if there is one for every CU and 8 steps: 4096 x 4096 x 512: 28 (128: 35), x 4096: 104 (129);
-//                           with 6 steps, x 384 and GELU on 100352 x 1536: 270 (242)
-//   128 x 128 tiles, if there is one for every CU: 2048 x 2048 x 1024: 18 (64: 21); 3001 x 1000 x 1552: 27 (26);
-//                           1024 x 1024 x 1024: 13 (11)
+// Which kernel, and in how many parts.  Measured (bf16, us a call among others, the kernels as they stand here):
+//   up to 16 token rows     4 x 1536 x 384: rows 8.6 (64 x 64 tiles: 8.6; the kernels alone 3.2 and 4.8), 1 x 512 x
+//                           8192: 11.3 (tiles in parts: 12.5; alone 11.5 and 8.4).  Few columns of a long reduction
+//                           are where the rule is not the faster side any more: 16 x 512 x 8192: 16.7 (12.8)
+//   256 x 256 tiles, if there is one for every CU and 8 steps: 4096 x 4096 x 512: 26 (128: 28), x 4096: 104 (120);
+//                           with 6 steps, x 384 and GELU on 100352 x 1536: 253 (216)
+//   128 x 128 tiles, if there is one for every CU: 2048 x 2048 x 1024: 15 (64: 19); 3001 x 1000 x 1552: 23 (24);
+//                           1024 x 1024 x 1024: 10.6 (7.9)
 //   64 x 64 tiles otherwise, in parts of 12 steps or more up to two workgroups a CU, where the reduction has 48
-//                           steps: 32 x 4096 x 8192: 18 (in one: 31), x 512: 15 (30); 64 x 512 x 2048: 15 (12)
+//                           steps: 32 x 4096 x 8192: 17.6 (in one: 33), x 512: 12.5 (30); 64 x 512 x 2048: 14.6 (10)
 enum { kLinAny, kLinRows, kLin64, kLin128, kLin256 };
 struct LinearPlan {
   int kernel, parts, part_steps;

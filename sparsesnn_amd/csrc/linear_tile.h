@@ -14,10 +14,10 @@
 // beside the rest of the step's products the freed stage is refilled and the next stage's first operands
 // are read.  The second half of B becomes the first of the next step.
 //
-// Bound by, as measured: 256 x 256 tiles: 8192 x 4096 x 8192 bf16 416 us (1.32 PFLOP/s), 8192^3 e4m3 453
-// (2.43): matrix cores and the clock that they leave; without the copies 8192^3 bf16 takes 757 of 857 us.
+// Bound by, as measured: 256 x 256 tiles: 8192 x 4096 x 8192 bf16 418 to 424 us (1.31 PFLOP/s), 8192^3 e4m3
+// 447 (2.46): matrix cores and the clock that they leave; without the copies 8192^3 bf16 takes 757 of 857 us.
 // A wave of 128 x 128 needs two thirds of the LDS reads of eight waves of 128 x 64.  128 x 128 tiles:
-// 100352 x 1536 x 384 fp16 with GELU 249 us, 22 a step and 130 for the starts, epilogues and stores of 9408
+// 100352 x 1536 x 384 fp16 with GELU 248 us, 22 a step and 130 for the starts, epilogues and stores of 9408
 // tiles.  64 x 64 tiles: 0.2 us a step, three workgroups a CU.  Stages of 64 bytes, twice as many, are
 // slower everywhere (8192^3 bf16 974 us): twice the meetings, half lines.
 //

@@ -8,7 +8,9 @@
 // Bandwidth bound: x and r are read once and y and s written once, because a row stays in
 // registers: L lanes hold a row, NV pieces of VEC elements each, and the sum of squares and the
 // largest |y| are reduced over those L lanes (in the order of a butterfly, the same every time).
-// 401408 x 384 fp16 with a residual to e4m3: 195 us, 5.5 TB/s (a copy of 2 GB reaches 4.9); 4 x 384: 3.2 us.
+// 401408 x 384 fp16 with a residual to e4m3: 197 us, 5.5 TB/s (a copy of 2 GB reaches 4.9); 4 x 384: 3.0 us.  With a
+// residual, fp32 100000 x 384: 108 us (5.7 TB/s), to e4m3 91; fp16 16384 x 16384: 360 (6.0), fp32 8192 x 32768: 798
+// (5.4).  Narrow rows leave lanes idle: fp16 400000 x 64: 45 (4.5 TB/s), x 8: 28 (0.9).
 #include "token_types.h"
 
 namespace sengine {

@@ -1092,10 +1092,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 
     x and weight are both fp16, both bf16, or both float8_e4m3fn with fp32 scales of x's rows
     (x_scale, as rms_norm returns it) and of weight's rows (weight_scale, (N,)).  The sums and what
-    follows them are fp32 (the 8-bit matrix instructions keep about 16 bits of a sum, which a 16-bit
-    result hides; an fp32 result of e4m3 operands takes the 16-bit ones at half the rate); the result
-    is rounded once to out_dtype (fp16, bf16 or fp32; x's type, for e4m3 bf16, by default).  residual
-    (..., N) has out_dtype, bias (N,) fp16, bf16 or fp32; `out` may be `residual`.  A long reduction
+    follows them are fp32; the 8-bit matrix instructions that make 16-bit results of e4m3 operands are
+    off by up to 2**-12 of the sum of the products' magnitudes (a tenth of an fp16 rounding, but more
+    of a sum that cancels), and an fp32 result takes the 16-bit instructions instead, at half the
+    rate, with sums of 32 bits.  The result is rounded once to out_dtype (fp16, bf16 or fp32; x's type, for e4m3 bf16, by default).  residual
+    (..., N) has out_dtype, bias (N,) fp16, bf16 or fp32; `out` may be `residual` but must share no
+    memory with x or weight.  A long reduction
     with few results is computed in parts through scratch memory of torch's allocator, the parts
     added in a fixed order."""
     if _dispatch_modes() or forward_ad._current_level >= 0:
@@ -1183,7 +1185,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
     in the others is never used.  Any strides whose rows of d values are contiguous and begin at
     multiples of 16 bytes; k and v expanded over the batch (one encoder pass, many queries) are read
     as they are.  Scores, their maximum and sums are fp32; the weights are rounded to q's type for
-    the product with v.  Few queries of many keys are computed in parts of the keys through scratch
+    the product with v, fp16 ones down to 2**-31 of the largest.  `out` may be q but must share no
+    memory with k or v.  Few queries of many keys are computed in parts of the keys through scratch
     memory of torch's allocator, the parts joined in a fixed order."""
     if _dispatch_modes() or forward_ad._current_level >= 0:
         _token_modes(q, k, v, scale)

@@ -549,7 +549,7 @@ int sengine_amd_linear_ws(const sengine_linear_desc* d, const void* x, const voi
  * never used, whatever it holds.  q, k, v and out are fp16 or bf16 with strides per (batch, row,
  * head) in elements and the d values of a head side by side; d is a multiple of 8 up to 128.  A
  * batch stride of 0 shares the encoder's states between the sequences.  out may be q itself, and shares
- * no memory with k or v.  Lk < 2^30, B Lq Hq < 2^31.
+ * no memory with k or v.  Lk < 2^30, B Lq Hq <= 2^31 - 256.
  */
 typedef struct sengine_cross_desc {
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];

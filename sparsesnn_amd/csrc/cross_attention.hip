@@ -94,7 +94,7 @@ struct CrossPlan {
 static bool keys_fit(const sengine_cross_desc* d) { return d->Lk <= 0x3fffffff; }
 static bool rows_fit(const sengine_cross_desc* d) {
   const int64_t queries = (int64_t)d->B * d->Lq;
-  return queries <= 0x7fffffff && queries * d->Hq <= 0x7fffffff;
+  return queries <= 0x7fffff00 && queries * d->Hq <= 0x7fffff00;  // up to the end of the last block of 256
 }
 
 static CrossPlan plan(const sengine_cross_desc* d) {
@@ -138,7 +138,7 @@ static hipError_t run_tile(CrossParams& p, hipStream_t stream) {
   p.spread = units % 8 == 0 || units >= 64;
   p.units = (int)units;
   const int64_t wgs = (p.spread ? (units + 7) / 8 * 8 : units) * p.inner;
-  if (wgs > 0x7fffffffll) return hipErrorInvalidValue;
+  if (!launchable(wgs, 64 * NW)) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)wgs), block(64 * NW);
   if (p.mask)
     cross_tile_kernel<T, DV, NW, QF, KT, S, HPW, SHARED, true, WPE><<<grid, block, 0, stream>>>(p);
@@ -238,6 +238,7 @@ extern "C" int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const
     return (int)(d->type == SENGINE_ENC_F16 ? by_width<_Float16>(p, plan_, stream)
                                             : by_width<__bf16>(p, plan_, stream));
   }
+  if (!launchable((int64_t)d->B * d->Lq * d->Hq, 64)) return (int)hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)((int64_t)d->B * d->Lq * d->Hq));
   if (d->type == SENGINE_ENC_F16)
     cross_row_kernel<_Float16><<<grid, dim3(64), 0, stream>>>(p);

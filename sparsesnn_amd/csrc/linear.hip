@@ -71,6 +71,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearParams p) {
 template <class T, int BM, int BN, int WM, int WN, int S, int WGS>
 static hipError_t run_tile(const LinearParams& p, int parts, hipStream_t stream) {
   const int64_t ntm = (p.M + BM - 1) / BM, ntn = (p.N + BN - 1) / BN;
+  if (!launchable(ntm * ntn, 64 * WM * WN)) return hipErrorInvalidConfiguration;
   linear_tile_kernel<T, BM, BN, WM, WN, S, WGS>
       <<<dim3((unsigned)(ntm * ntn), (unsigned)parts), dim3(64 * WM * WN), 0, stream>>>(p, (int)ntm, (int)ntn);
   return hipGetLastError();
@@ -125,6 +126,7 @@ static hipError_t run(LinearParams p, float* workspace, size_t bytes, hipStream_
   const LinearPlan q = plan(p, __is_same(T, E4m3Wide));
   switch (q.kernel) {
     case kLinRows:
+      if (!launchable((p.N + 15) / 16, 512)) return hipErrorInvalidConfiguration;
       linear_rows_kernel<T, 8, 4><<<dim3((unsigned)((p.N + 15) / 16)), dim3(512), 0, stream>>>(p);
       return hipGetLastError();
     case kLin64: {
@@ -146,6 +148,7 @@ static hipError_t run(LinearParams p, float* workspace, size_t bytes, hipStream_
       if constexpr (!__is_same(T, E4m3Wide)) return run_tile<T, 256, 256, 2, 2, 2, 1>(p, 1, stream);
       [[fallthrough]];
     default:
+      if (!launchable(tiles_of(p, 64), 256)) return hipErrorInvalidConfiguration;
       linear_any_kernel<T><<<dim3((unsigned)tiles_of(p, 64)), dim3(256), 0, stream>>>(p);
       return hipGetLastError();
   }

@@ -24,6 +24,9 @@ inline int type_bytes(int code) {
   return code == SENGINE_ENC_F32 ? 4 : code == SENGINE_ENC_E4M3 ? 1 : 2;
 }
 
+// Whether one launch can have so many workgroups: its threads count to 2^32 - 1.
+inline bool launchable(int64_t wgs, int threads) { return wgs <= 0xffffffffll / threads; }
+
 // One element of a run-time type (a vector of coefficients read once per column).
 __device__ __forceinline__ float load_as_float(const void* p, int code, int64_t i) {
   if (code == SENGINE_ENC_F32) return static_cast<const float*>(p)[i];

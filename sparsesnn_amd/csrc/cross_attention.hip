@@ -10,8 +10,8 @@ namespace sengine {
 
 // Any alignment and any strides (rows at odd elements, through the C entry only; keys too far apart for a tile's
 // offsets): one query of 1024 masked keys 2^18 elements apart, 128 sequences, 32 heads on 8 x 128: 908 us (the tile
-// kernel without the mask 110), bound by its single-element loads.  One wave a query row and head, an online softmax over 64 keys at a time, lane j
-// forming the dot product of key j, then the lanes sharing the values' columns.
+// kernel without the mask 110), bound by its single-element loads.  One wave a query row and head, an online softmax
+// over 64 keys at a time, lane j forming the dot product of key j, then the lanes sharing the values' columns.
 template <class T>
 __global__ __launch_bounds__(64) void cross_row_kernel(CrossParams p) {
   __shared__ float sq[128], sp[64];

@@ -23,8 +23,8 @@
 // reads as long as the products.  One query of up to 16384 keys (8 sequences, 8 key heads x 128) 57 us and 64 queries
 // of 3136 keys (128 sequences, 8 heads x 48) 113 us: bandwidth, 4.9 and 5.5 TB/s.
 //
-// The masked kernel of 128 rows keeps 14 of its vector registers in scratch memory at 97 to 128 values (60 bytes a lane),
-// that of four merged heads of 32 values 20 bytes; masked kernels keep up to 80 scalar ones in vector registers.
+// The masked kernel of 128 rows keeps 14 of its vector registers in scratch memory at 97 to 128 values (60 bytes a
+// lane), that of four merged heads of 32 values 20 bytes; masked kernels keep up to 80 scalar ones in vector registers.
 //
 // LDS: a key's row has PR 16-byte pieces, piece j at place j ^ f(row): 8 lanes that read a piece of 8 rows, and
 // 16 lanes that read 32 bytes of 4 rows, touch every bank once.

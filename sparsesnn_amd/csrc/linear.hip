@@ -9,9 +9,9 @@
 namespace sengine {
 
 // Any strides, any alignment, any K: 8192 x 4096 x 8191 bf16 1410 us (8192 wide 424), since nothing is in flight during
-// the products and the tile is 64 x 64; one operand whose rows are no whole pieces brings a call here.  Workgroup = 64 rows x 64 columns, four waves of 32 x 32; per
-// 128 bytes of the reduction both operands' rows go through registers into LDS: whole 16-byte pieces
-// by one load of whatever alignment, the row's last piece byte by byte, zeros beyond.
+// the products and the tile is 64 x 64; one operand whose rows are no whole pieces brings a call here.  Workgroup =
+// 64 rows x 64 columns, four waves of 32 x 32; per 128 bytes of the reduction both operands' rows go through registers
+// into LDS: whole 16-byte pieces by one load of whatever alignment, the row's last piece byte by byte, zeros beyond.
 constexpr int kLinPitch = 128 + 16;  // LDS row: 16 bytes more, so that 16 rows' pieces spread over the banks
 
 template <class T>

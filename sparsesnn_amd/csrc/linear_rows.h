@@ -3,8 +3,9 @@
 // Workgroup = 16 weight rows and up to 16 token rows; its W waves share the reduction, wave w taking the
 // 128-byte steps w, w + W, ...  Operands go from memory straight into the matrix instructions' registers
 // (a step of 16 weight rows is two loads a lane, whatever their alignment), U steps ahead of their use, and
-// the waves' sums are joined in LDS.  4 x 1536 x 384 fp16: 3.9 us; 1 x 512 x 8192: 11.5 and 16 rows of it 16.5, on 32 workgroups; with 17 rows or more
-// the token rows' reads take longer than the tiles' copies (32 x 4096 x 8192: 27 us, in tiles 18).
+// the waves' sums are joined in LDS.  4 x 1536 x 384 fp16: 3.9 us; 1 x 512 x 8192: 11.5 and 16 rows of it 16.5, on
+// 32 workgroups; with 17 rows or more the token rows' reads take longer than the tiles' copies (32 x 4096 x 8192: 27 us,
+// in tiles 18).
 #pragma once
 #include "linear.h"
 

@@ -1095,11 +1095,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     follows them are fp32; the 8-bit matrix instructions that make 16-bit results of e4m3 operands are
     off by up to 2**-12 of the sum of the products' magnitudes (a tenth of an fp16 rounding, but more
     of a sum that cancels), and an fp32 result takes the 16-bit instructions instead, at half the
-    rate, with sums of 32 bits.  The result is rounded once to out_dtype (fp16, bf16 or fp32; x's type, for e4m3 bf16, by default).  residual
-    (..., N) has out_dtype, bias (N,) fp16, bf16 or fp32; `out` may be `residual` but must share no
-    memory with x or weight.  A long reduction
-    with few results is computed in parts through scratch memory of torch's allocator, the parts
-    added in a fixed order."""
+    rate, with sums of 32 bits.  The result is rounded once to out_dtype (fp16, bf16 or fp32; x's
+    type, for e4m3 bf16, by default).  residual (..., N) has out_dtype, bias (N,) fp16, bf16 or fp32;
+    `out` may be `residual` but must share no memory with x or weight.  A long reduction with few
+    results is computed in parts through scratch memory of torch's allocator, the parts added in a
+    fixed order."""
     if _dispatch_modes() or forward_ad._current_level >= 0:
         _token_modes(x, weight, bias, residual, x_scale, weight_scale)
     key = None

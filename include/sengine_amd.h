@@ -571,6 +571,51 @@ int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const void* q, c
                                    size_t workspace_bytes, hipStream_t stream);
 
 /*
+ * Rotary positions with several axes.  q (B, L, Hq, d) and k (B, L, Hk, d; Hk = 0: none) of one type (fp16, bf16 or
+ * fp32), strides per (batch, token, head) in elements.  The first 2 P values of every head, P the sum of the axes'
+ * sections, are P pairs: (x[j], x[P + j]), or with `interleaved` (x[2 j], x[2 j + 1]); the first sections[0] of them
+ * belong to axis 0, and so on.  A pair turns by positions[b, l, axis] * frequencies[j] radians, (x0, x1) ->
+ * (x0 cos - x1 sin, x0 sin + x1 cos); the values behind the pairs are copied.  positions are int32, or fp32 with
+ * `pos_float`, pos_stride per (batch, token) and a token's axes side by side; a batch stride of 0 shares them.  The
+ * angle is reduced in 64 bits, the rest is fp32, an output is rounded once.  out_q may be q itself and out_k k;
+ * otherwise they share no memory with an input.  d <= 1024, (Hq + Hk) d <= 65536.
+ */
+typedef struct sengine_rotary_desc {
+  int64_t q_stride[3], k_stride[3], out_q_stride[3], out_k_stride[3], pos_stride[2];
+  int32_t B, L, Hq, Hk, d;
+  int32_t axes, sections[4];
+  int32_t type, pos_float, interleaved;
+} sengine_rotary_desc;
+int sengine_amd_rotary(const sengine_rotary_desc* d, const void* q, const void* k, const void* positions,
+                       const float* frequencies, void* out_q, void* out_k, hipStream_t stream);
+
+/*
+ * The linear operator with a weight in 4 bits: out[m, n] = act(row_scale[n] * sum_k x[m, k] group_scale[n, k / group]
+ * code[n, k] + bias[n]) + residual[m, n].  Codes are e2m1, two a byte and the lower half first, rows weight_stride
+ * bytes apart; group_scale is e4m3, ceil(K / group) a row, rows scale_stride bytes apart; row_scale fp32 (null = 1).
+ * group is 32, 64 or 128, K even.  x is fp16 or bf16; out, residual and bias as sengine_amd_linear's.  Products of
+ * codes and scales are exact, sums and epilogue fp32, out is rounded once.  out may be residual itself, and shares no
+ * memory with the inputs otherwise.  K < 2^30 - 16, N <= 2^31 - 256.
+ * With scratch memory (16-byte aligned, of at least sengine_amd_linear_e2m1_workspace's bytes; what it holds before
+ * does not matter) many token rows are multiplied with the weight widened to 16 bits there; without it, or with less,
+ * every 64 token rows read the codes again.
+ */
+typedef struct sengine_linear_e2m1_desc {
+  int64_t M;
+  int64_t x_stride, weight_stride, scale_stride, residual_stride, out_stride;
+  int32_t N, K, group;
+  int32_t in_type, out_type, bias_type, activation;
+} sengine_linear_e2m1_desc;
+int sengine_amd_linear_e2m1(const sengine_linear_e2m1_desc* d, const void* x, const void* weight,
+                            const void* group_scale, const float* row_scale, const void* bias, const void* residual,
+                            void* out, hipStream_t stream);
+int sengine_amd_linear_e2m1_workspace(const sengine_linear_e2m1_desc* d, size_t* bytes);
+int sengine_amd_linear_e2m1_ws(const sengine_linear_e2m1_desc* d, const void* x, const void* weight,
+                               const void* group_scale, const float* row_scale, const void* bias,
+                               const void* residual, void* out, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream);
+
+/*
  * Peak calibration on the box (the role of the reference's sengine/tuning/hw_calibrate.py:
  * 17-134, which times a memcpy and a dense fp16 GEMM).  Measurement entry points, not on
  * the operator path.

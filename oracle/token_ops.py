@@ -105,3 +105,40 @@ def cross_attention(q, k, v, scale=None, key_lengths=None, key_mask=None):
             out[b, :, h] = o
             bound[b, :, h] = rel * (p @ vv.abs()) + tiny
     return out, bound + half_step(out, q.dtype)
+
+
+def rotary(x, positions, frequencies, sections, interleaved):
+    """(value, bound) of the first 2 P values of each head of x (B, L, heads, d) turned, the rest as it is."""
+    axis = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(sections)).to(x.device)
+    angle = positions.double()[..., axis] * frequencies.double()  # (B, L, P) or (L, P)
+    cos, sin = torch.cos(angle)[..., None, :], torch.sin(angle)[..., None, :]
+    n = len(axis)
+    a, b = (slice(0, 2 * n, 2), slice(1, 2 * n, 2)) if interleaved else (slice(0, n), slice(n, 2 * n))
+    y, err = x.double().clone(), torch.zeros(x.shape, dtype=torch.float64, device=x.device)
+    x0, x1 = x[..., a].double(), x[..., b].double()
+    y[..., a], y[..., b] = x0 * cos - x1 * sin, x0 * sin + x1 * cos
+    # the reduced angle is an fp32 number of half turns up to 1 (off by 2^-25, pi times that in radians), formed in 64
+    # bits from a few roundings relative to the whole angle; sine and cosine are off by two units more, the products
+    # and their sum round three times
+    rel = math.pi * 2.0**-25 + 4 * U + angle.abs()[..., None, :] * 2.0**-50 + 3 * U
+    err[..., a] = err[..., b] = (x0.abs() + x1.abs()) * rel
+    # what is not turned is stored as it was
+    bound = err + torch.where(err > 0, half_step(y, x.dtype), 0.0)
+    return y, bound
+
+
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
+
+
+def e2m1_weight(weight, group_scale, K):
+    """The (N, K) values, in 64 bits, of e2m1 codes two a byte and the e4m3 scales of their groups."""
+    codes = torch.stack([weight & 15, weight >> 4], -1).flatten(1).long()
+    group = next(g for g in (32, 64, 128) if -(-K // g) == group_scale.shape[1])
+    values = torch.tensor(E2M1, dtype=torch.float64, device=weight.device)[codes]
+    return values * torch.repeat_interleave(group_scale.double(), group, 1)[:, :K]
+
+
+def linear_e2m1(x, weight, group_scale, row_scale, bias, act, residual, out_dtype):
+    """(value, bound): the products of codes and scales are exact, so the linear operator's bound holds."""
+    w = e2m1_weight(weight, group_scale, x.shape[-1])
+    return linear(x, w, bias, act, residual, None, row_scale, out_dtype)

@@ -65,11 +65,35 @@ class CrossDesc(ctypes.Structure):
     ]
 
 
+class RotaryDesc(ctypes.Structure):
+    """Mirror of ``sengine_rotary_desc``."""
+
+    _fields_ = [
+        ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("out_q_stride", ctypes.c_int64 * 3),
+        ("out_k_stride", ctypes.c_int64 * 3), ("pos_stride", ctypes.c_int64 * 2), ("B", ctypes.c_int32),
+        ("L", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hk", ctypes.c_int32), ("d", ctypes.c_int32),
+        ("axes", ctypes.c_int32), ("sections", ctypes.c_int32 * 4), ("type", ctypes.c_int32),
+        ("pos_float", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+    ]
+
+
+class LinearE2m1Desc(ctypes.Structure):
+    """Mirror of ``sengine_linear_e2m1_desc``."""
+
+    _fields_ = [
+        ("M", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("weight_stride", ctypes.c_int64),
+        ("scale_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64),
+        ("N", ctypes.c_int32), ("K", ctypes.c_int32), ("group", ctypes.c_int32), ("in_type", ctypes.c_int32),
+        ("out_type", ctypes.c_int32), ("bias_type", ctypes.c_int32), ("activation", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _DP = ctypes.POINTER(ConvLifDesc)
 _I32, _I64, _F = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 _SZP = ctypes.POINTER(ctypes.c_size_t)
 _NDP, _LDP, _CDP = ctypes.POINTER(RmsNormDesc), ctypes.POINTER(LinearDesc), ctypes.POINTER(CrossDesc)
+_RDP, _L4DP = ctypes.POINTER(RotaryDesc), ctypes.POINTER(LinearE2m1Desc)
 
 # name -> (restype, argtypes); every symbol declared in include/sengine_amd.h
 SIGNATURES = {
@@ -125,6 +149,10 @@ SIGNATURES = {
     "sengine_amd_cross_attention": (ctypes.c_int, [_CDP, _P, _P, _P, _P, _P, _P, _P]),
     "sengine_amd_cross_attention_workspace": (ctypes.c_int, [_CDP, _SZP]),
     "sengine_amd_cross_attention_ws": (ctypes.c_int, [_CDP, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "sengine_amd_rotary": (ctypes.c_int, [_RDP, _P, _P, _P, _P, _P, _P, _P]),
+    "sengine_amd_linear_e2m1": (ctypes.c_int, [_L4DP, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "sengine_amd_linear_e2m1_workspace": (ctypes.c_int, [_L4DP, _SZP]),
+    "sengine_amd_linear_e2m1_ws": (ctypes.c_int, [_L4DP, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "sengine_amd_pack_spikes": (ctypes.c_int, [_P, _I32, _I64, _I32, _P, _P]),
     "sengine_amd_unpack_spikes": (ctypes.c_int, [_P, _I64, _I32, _P, _I32, _P]),
 }

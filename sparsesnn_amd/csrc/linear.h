@@ -120,11 +120,11 @@ __device__ __forceinline__ void linear_residual(const LinearParams& p, int64_t m
   }
 }
 
-// The coefficients of NV columns and NR rows STEP apart; only 8-bit operands have scales.  Tile kernels load them
-// before their products, so that the epilogue does not wait for them.
+// The coefficients of NV columns and NR rows STEP apart; only 8-bit operands and widened 4-bit weights have scales.
+// Tile kernels load them before their products, so that the epilogue does not wait for them.
 template <class T, int NV>
 struct Columns {
-  static constexpr bool kScaled = sizeof(T) == 1;
+  static constexpr bool kScaled = Operand<T>::kScaled;
   float w[kScaled ? NV : 1], bias[NV];
   __device__ __forceinline__ void load(const LinearParams& p, int n) {
 #pragma unroll
@@ -137,7 +137,7 @@ struct Columns {
 };
 template <class T, int NR, int STEP>
 struct RowScales {
-  static constexpr bool kScaled = sizeof(T) == 1;
+  static constexpr bool kScaled = Operand<T>::kScaled;
   float x[kScaled ? NR : 1];
   __device__ __forceinline__ void load(const LinearParams& p, int64_t m) {
     if constexpr (kScaled) {
@@ -270,10 +270,10 @@ typedef int int8v_t __attribute__((ext_vector_type(8)));
 // One 64-byte half of that step, for the types whose instruction takes it.
 template <class T>
 __device__ __forceinline__ float4_t mma_64b(u32x4_t a, u32x4_t b, float4_t c) {
-  if constexpr (__is_same(T, _Float16)) {
+  if constexpr (__is_same(typename Operand<T>::type, _Float16)) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
                                                   0, 0);
-  } else if constexpr (__is_same(T, __bf16)) {
+  } else if constexpr (__is_same(typename Operand<T>::type, __bf16)) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
                                                    0, 0, 0);
   } else {
@@ -295,5 +295,10 @@ __device__ __forceinline__ float4_t mma_128b(u32x4_t a0, u32x4_t a1, u32x4_t b0,
     return mma_64b<T>(a1, b1, mma_64b<T>(a0, b0, c));
   }
 }
+
+// The linear operator on 16-bit operands of which the weight's rows have fp32 scales (w_scale), and the scratch memory
+// that it takes parts in (linear.hip).  p is filled as by the entry.
+hipError_t launch_linear_scaled(const LinearParams& p, bool fp16, float* workspace, size_t bytes, hipStream_t stream);
+size_t linear_scaled_workspace(const LinearParams& p);
 
 }  // namespace sengine

@@ -154,6 +154,15 @@ static hipError_t run(LinearParams p, float* workspace, size_t bytes, hipStream_
   }
 }
 
+hipError_t launch_linear_scaled(const LinearParams& p, bool fp16, float* workspace, size_t bytes, hipStream_t stream) {
+  return fp16 ? run<F16Rows>(p, workspace, bytes, stream) : run<Bf16Rows>(p, workspace, bytes, stream);
+}
+
+size_t linear_scaled_workspace(const LinearParams& p) {
+  const LinearPlan q = plan(p, false);
+  return q.parts > 1 ? (size_t)(q.parts * tiles_of(p, 64)) * 64 * 64 * 4 : 0;
+}
+
 }  // namespace sengine
 
 using namespace sengine;

@@ -52,9 +52,10 @@ __device__ __forceinline__ void linear_tile_of(int id, int ntm, int ntn, int& mt
 // sums the caller lets mma_drain pass, which no instruction is scheduled across.
 template <class T, bool ACCUM>  // ACCUM: the sums are in accumulation registers, else in ordinary ones
 __device__ __forceinline__ void mma_inplace(u32x4_t a, u32x4_t b, float4_t& c) {
-  if constexpr (__is_same(T, _Float16) && ACCUM)
+  using V = typename Operand<T>::type;
+  if constexpr (__is_same(V, _Float16) && ACCUM)
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-  else if constexpr (__is_same(T, _Float16))
+  else if constexpr (__is_same(V, _Float16))
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
   else if constexpr (ACCUM)
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));

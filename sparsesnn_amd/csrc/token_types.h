@@ -20,6 +20,31 @@ struct E4m3Wide {  // the same bytes, multiplied as the fp16 values they stand f
   uint8_t bits;
 };
 
+struct F16Rows {  // fp16, whose rows (of a weight) have fp32 scales as 8-bit ones do
+  _Float16 v;
+};
+
+struct Bf16Rows {
+  __bf16 v;
+};
+
+// The type that a matrix instruction takes, and whether operands have scales of their rows.
+template <class T>
+struct Operand {
+  using type = T;
+  static constexpr bool kScaled = sizeof(T) == 1;
+};
+template <>
+struct Operand<F16Rows> {
+  using type = _Float16;
+  static constexpr bool kScaled = true;
+};
+template <>
+struct Operand<Bf16Rows> {
+  using type = __bf16;
+  static constexpr bool kScaled = true;
+};
+
 inline int type_bytes(int code) {
   return code == SENGINE_ENC_F32 ? 4 : code == SENGINE_ENC_E4M3 ? 1 : 2;
 }

@@ -18,7 +18,8 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import (ACTIVATIONS, ENC_BF16, ENC_BITS, ENC_E4M3, ENC_F16, ENC_F32, NEURON_IF, NEURON_LIF, NEURON_MS,
-                   WLAYOUT_HWIO, WLAYOUT_OIHW, ConvLifDesc, CrossDesc, LinearDesc, RmsNormDesc, SEngineError, check)
+                   WLAYOUT_HWIO, WLAYOUT_OIHW, ConvLifDesc, CrossDesc, LinearDesc, LinearE2m1Desc, RmsNormDesc, RotaryDesc,
+                   SEngineError, check)
 
 __all__ = [
     "ConvSpec", "make_desc", "geometry", "set_fused_kernel", "compress_2_4", "pack_dense_weights", "pack_spikes",
@@ -27,7 +28,8 @@ __all__ = [
     "ENC_BITS", "ENC_F16", "ENC_F32", "NEURON_LIF", "NEURON_IF", "NEURON_MS", "WLAYOUT_OIHW", "WLAYOUT_HWIO",
     "neuron_code", "fused_sparse_conv_bn_add_neuron", "spiking_self_attention", "stem_conv_bn_neuron",
     "fused_sparse_conv_bn_lif_pair", "fused_sparse_conv_bn_lif_split", "fused_sparse_conv_bn_lif_tail", "tail_eligible",
-    "fused_plan", "rms_norm", "linear", "cross_attention", "ENC_BF16", "ENC_E4M3",
+    "fused_plan", "rms_norm", "linear", "cross_attention", "rotary", "linear_e2m1", "ENC_BF16",
+    "ENC_E4M3",
 ]
 
 
@@ -1213,4 +1215,196 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     check(_lib.load().sengine_amd_cross_attention_ws(
         desc, qp, kp, vp, _ptr(key_lengths), _ptr(key_mask), op, _ptr(ws), size, _stream(dev)), "cross_attention")
+    return out
+
+
+def _heads_out(t, shape, dtype, name: str, device):
+    """An output (B, L, heads, d) given by the caller: any strides, the values of a head side by side."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device != device or t.dtype != dtype or t.shape != shape:
+        raise SEngineError(f"{name}: expected {dtype} {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} on "
+                           f"{t.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise SEngineError(f"{name} requires a gradient: the token operators are inference only")
+
+
+def _head_strides(t, name: str):
+    """Strides per (batch, token, head) of (B, L, heads, d), whose heads' values must lie side by side."""
+    s = t.stride()
+    if t.numel() and t.shape[3] > 1 and s[3] != 1:
+        raise SEngineError(f"{name}: the values of a head must lie side by side (strides {s})")
+    # a stride over a single element is never taken: 0 keeps it from looking unaligned
+    return (ctypes.c_int64 * 3)(*(x if n > 1 else 0 for n, x in zip(t.shape[:3], s)))
+
+
+def _rotary_plan(key, q, k, positions, frequencies, sections, interleaved, out_q, out_k):
+    """(descriptor, device) of a checked call."""
+    _token_input(q, "q")
+    dev, code = q.device, _type_code(q, (torch.float16, torch.bfloat16, torch.float32), "q")
+    if q.dim() != 4:
+        raise SEngineError(f"q: expected (B, L, heads, d), got {tuple(q.shape)}")
+    B, L, Hq, d = q.shape
+    Hk = 0
+    if k is not None:
+        _token_input(k, "k", dev)
+        if k.dtype != q.dtype or k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != d:
+            raise SEngineError(f"k: expected {q.dtype} ({B}, {L}, heads, {d}), got {k.dtype} {tuple(k.shape)}")
+        Hk = k.shape[2]
+    elif out_k is not None:
+        raise SEngineError("out_k: there is no k")
+    if not 1 <= len(sections) <= 4 or any(type(n) is not int or n < 0 for n in sections):
+        raise SEngineError(f"sections: expected 1 to 4 numbers of pairs, got {sections!r}")
+    _token_sizes("rotary: B, L, heads, d and sections", B, L, Hq, Hk, d, *sections)
+    pairs, axes = sum(sections), len(sections)
+    _token_vector(frequencies, pairs, "frequencies", dev)
+    _type_code(frequencies, (torch.float32,), "frequencies")
+    _token_input(positions, "positions", dev)
+    if positions.dtype not in (torch.int32, torch.float32):
+        raise SEngineError(f"positions: expected dtype torch.int32 or torch.float32, got {positions.dtype}")
+    if tuple(positions.shape) not in ((B, L, axes), (L, axes)) or (axes > 1 and positions.stride(-1) != 1):
+        raise SEngineError(f"positions: expected ({B}, {L}, {axes}) or ({L}, {axes}) with a token's axes side by side, got "
+                           f"{tuple(positions.shape)}")
+    ps = positions.stride() if positions.dim() == 3 else (0, *positions.stride())
+    for t, x, name in ((out_q, q, "out_q"), (out_k, k, "out_k")):
+        if t is not None:
+            _heads_out(t, x.shape, q.dtype, name, dev)
+    dense = lambda n: (ctypes.c_int64 * 3)(L * n * d, n * d, d)
+    zero = (ctypes.c_int64 * 3)()
+    desc = ctypes.byref(RotaryDesc(
+        _head_strides(q, "q"), zero if k is None else _head_strides(k, "k"),
+        dense(Hq) if out_q is None else _head_strides(out_q, "out_q"),
+        dense(Hk) if out_k is None else _head_strides(out_k, "out_k"), (ctypes.c_int64 * 2)(*ps[:2]), B, L, Hq, Hk, d,
+        axes, (ctypes.c_int32 * 4)(*sections), code, positions.dtype is torch.float32, bool(interleaved)))
+    return _remember(key, (desc, dev))
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, frequencies: torch.Tensor, sections,
+           interleaved: bool = False, out_q: Optional[torch.Tensor] = None, out_k: Optional[torch.Tensor] = None):
+    """Rotary positions with several axes (time, height, width) on queries q (B, L, Hq, d) and keys k (B, L, Hk, d) or
+    None; fp16, bf16 or fp32.  Returns (q', k') in their type, k' None without k.
+
+    The first 2 P values of a head are P = sum(sections) pairs, (x[j], x[P + j]), or (x[2 j], x[2 j + 1]) with
+    interleaved; the first sections[0] pairs belong to the first axis, and so on (1 to 4 axes).  Pair j turns by
+    positions[b, t, axis] * frequencies[j] radians: (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos).  The values behind
+    the pairs are copied.  positions (B, L, axes), or (L, axes) for all sequences, int32 or fp32; frequencies (P,)
+    fp32.  The angle is formed and reduced in 64 bits, so that far positions turn as near ones do; sines, cosines and
+    products are fp32, with one rounding at the end.  Any strides whose heads' d values lie side by side (d <= 1024, a
+    token's heads together up to 65536 values).  out_q may be q and out_k k; otherwise they share no memory with an
+    input."""
+    if _dispatch_modes() or forward_ad._current_level >= 0:
+        _token_modes(q, k, positions, frequencies)
+    if type(sections) is not tuple:
+        sections = tuple(sections)
+    key = None
+    if out_q is None and out_k is None:
+        try:
+            key = ("rotary", q.dtype, q.shape, q.stride(), q.device, _layout(k), positions.dtype, positions.shape,
+                   positions.stride(), positions.device, frequencies.dtype, frequencies.shape, frequencies.stride(),
+                   frequencies.device, sections, bool(interleaved))
+        except AttributeError:
+            pass  # not a tensor: the checks say so
+    plan = _TOKEN_PLANS.get(key)
+    if plan is None or (torch.is_grad_enabled() and (
+            q.requires_grad or positions.requires_grad or frequencies.requires_grad
+            or (k is not None and k.requires_grad))):
+        plan = _rotary_plan(key, q, k, positions, frequencies, sections, interleaved, out_q, out_k)
+    desc, dev = plan
+    if out_q is None:
+        out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if out_k is None and k is not None:
+        out_k = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    check(_lib.load().sengine_amd_rotary(desc, q.data_ptr(), _ptr(k), positions.data_ptr(), frequencies.data_ptr(),
+                                         out_q.data_ptr(), _ptr(out_k), _stream(dev)), "rotary")
+    return out_q, out_k
+
+
+# Types of two e2m1 codes a byte: plain bytes, and torch's own where it has one.
+_E2M1_BYTES = tuple(t for t in (torch.uint8, getattr(torch, "float4_e2m1fn_x2", None)) if t is not None)
+
+
+def _linear_e2m1_plan(key, x, weight, group_scale, row_scale, bias, activation, residual, out_dtype, out):
+    """(descriptor, bytes of scratch memory, output's shape and type, device) of a checked call."""
+    _token_input(x, "x")
+    dev, code = x.device, _type_code(x, (torch.float16, torch.bfloat16), "x")
+    _token_input(weight, "weight", dev)
+    if x.dim() == 0 or weight.dim() != 2 or weight.dtype not in _E2M1_BYTES or 2 * weight.shape[1] != x.shape[-1]:
+        raise SEngineError(f"weight: expected e2m1 codes (N, K / 2), two a byte, for x {tuple(x.shape)}, got {weight.dtype} "
+                           f"{tuple(weight.shape)}")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+    N, K = weight.shape[0], x.shape[-1]
+    _token_sizes("linear_e2m1: N and K", N, K)
+    _token_input(group_scale, "group_scale", dev)
+    _type_code(group_scale, (torch.float8_e4m3fn,), "group_scale")
+    group = next((g for g in (32, 64, 128) if tuple(group_scale.shape) == (N, -(-K // g))), 0)
+    if not group:
+        raise SEngineError(f"group_scale: expected ({N}, K / group) with groups of 32, 64 or 128 of {K} values, got "
+                           f"{tuple(group_scale.shape)}")
+    M, xs = _token_rows(x, "x")
+    wst, sst = _token_rows(weight, "weight")[1], _token_rows(group_scale, "group_scale")[1]
+    if out_dtype is None:
+        out_dtype = x.dtype
+    ocode = _TOKEN_TYPES.get(out_dtype, ENC_E4M3)
+    if ocode == ENC_E4M3:
+        raise SEngineError(f"out_dtype: expected float16, bfloat16 or float32, got {out_dtype}")
+    if row_scale is not None:
+        _token_vector(row_scale, N, "row_scale", dev)
+        _type_code(row_scale, (torch.float32,), "row_scale")
+    bcode = 0
+    if bias is not None:
+        _token_vector(bias, N, "bias", dev)
+        bcode = _type_code(bias, (torch.float16, torch.bfloat16, torch.float32), "bias")
+    shape = (*x.shape[:-1], N)
+    rs = 0
+    if residual is not None:
+        _token_input(residual, "residual", dev)
+        if residual.shape != shape or residual.dtype != out_dtype:
+            raise SEngineError(f"residual: expected {out_dtype} {shape}, got {residual.dtype} "
+                               f"{tuple(residual.shape)}")
+        rs = _token_rows(residual, "residual")[1]
+    os_ = N if out is None else _token_out(out, shape, out_dtype, "out", dev)
+    desc = ctypes.byref(LinearE2m1Desc(M, xs, wst, sst, rs, os_, N, K, group, code, ocode, bcode,
+                                       ACTIVATIONS[activation]))
+    size = ctypes.c_size_t()
+    check(_lib.load().sengine_amd_linear_e2m1_workspace(desc, ctypes.byref(size)), "linear_e2m1")
+    return _remember(key, (desc, size.value, shape, out_dtype, dev))
+
+
+def linear_e2m1(x: torch.Tensor, weight: torch.Tensor, group_scale: torch.Tensor,
+                row_scale: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, activation: str = "none",
+                residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x w^T + bias) + residual of token rows x (..., K), fp16 or bf16, with a weight (N, K) in 4 bits:
+    w[n, k] = row_scale[n] group_scale[n, k // group] code[n, k].
+
+    weight holds the codes, e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and, with the highest bit, their negatives), two a byte and
+    the lower half first: (N, K / 2) uint8 or float4_e2m1fn_x2, K even.  group_scale is (N, ceil(K / group))
+    float8_e4m3fn with groups of 32, 64 or 128 values, row_scale (N,) fp32, 1 where None; token_reader.e2m1_groups makes
+    the three of a weight.  Nothing of the weight is rounded: a code times a group's scale is a 16-bit value; sums and
+    what follows them are fp32, and the result is rounded once to out_dtype (x's type by default; fp16, bf16 or fp32).
+    activation, bias, residual and out as linear's.  Up to 64 token rows read the codes as they are, in the time that
+    their bytes take; more rows are multiplied with the weight widened to 16 bits in scratch memory of torch's
+    allocator."""
+    if _dispatch_modes() or forward_ad._current_level >= 0:
+        _token_modes(x, weight, group_scale, row_scale, bias, residual)
+    key = None
+    if out is None:
+        try:
+            key = ("linear_e2m1", x.dtype, x.shape, x.stride(), x.device, weight.dtype, weight.shape, weight.stride(),
+                   weight.device, _layout(group_scale), _layout(row_scale), activation, out_dtype, _layout(bias),
+                   _layout(residual))
+        except AttributeError:
+            pass  # not a tensor: the checks say so
+    plan = _TOKEN_PLANS.get(key)
+    if plan is None or (torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, weight, group_scale, row_scale, bias, residual))):
+        plan = _linear_e2m1_plan(key, x, weight, group_scale, row_scale, bias, activation, residual, out_dtype, out)
+    desc, size, shape, out_dtype, dev = plan
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=dev)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    check(_lib.load().sengine_amd_linear_e2m1_ws(
+        desc, x.data_ptr(), weight.data_ptr(), group_scale.data_ptr(), _ptr(row_scale), _ptr(bias), _ptr(residual),
+        out.data_ptr(), _ptr(ws), size, _stream(dev)), "linear_e2m1")
     return out

@@ -55,6 +55,30 @@ def e4m3_rows(w: torch.Tensor):
     return (w.float() / c[:, None]).to(torch.float8_e4m3fn), c
 
 
+E2M1_MIDDLES = (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)  # between neighbouring sizes of e2m1 codes
+E2M1_MAX = 6.0
+
+
+def e2m1_groups(w: torch.Tensor, group: int = 32):
+    """(codes, group scales, row scales) of a weight (N, K) in 4 bits, as ops.linear_e2m1 takes them: a row scaled to
+    the range of its groups' scales (e4m3), a group to that of its codes, which are the nearest ones."""
+    if w.dim() != 2 or w.shape[1] % 2 or group not in (32, 64, 128):
+        raise SEngineError(f"e2m1_groups: expected (N, K) with an even K and groups of 32, 64 or 128, got {tuple(w.shape)} "
+                           f"in groups of {group}")
+    N, K = w.shape
+    groups = -(-K // group)
+    w = w.detach().float()
+    row = w.abs().amax(-1) / (E2M1_MAX * E4M3_MAX) if K else torch.zeros(N, device=w.device)
+    row = torch.where(row > 0, row, torch.ones_like(row))
+    v = torch.nn.functional.pad(w / row[:, None], (0, groups * group - K)).view(N, groups, group)
+    scale = (v.abs().amax(-1) / E2M1_MAX).clamp(max=E4M3_MAX).to(torch.float8_e4m3fn)
+    s = scale.float()[:, :, None]
+    v = (v / torch.where(s > 0, s, torch.ones_like(s))).view(N, groups * group)[:, :K]
+    codes = torch.bucketize(v.abs(), torch.tensor(E2M1_MIDDLES, device=w.device))
+    codes = (codes + 8 * (v < 0)).to(torch.uint8)
+    return codes[:, ::2] | codes[:, 1::2] << 4, scale, row
+
+
 class TokenReader:
     """params as random_reader_params names them; dtype float16 or bfloat16; eight_bit: the first MLP
     product runs on e4m3 operands."""

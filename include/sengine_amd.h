@@ -616,6 +616,35 @@ int sengine_amd_linear_e2m1_ws(const sengine_linear_e2m1_desc* d, const void* x,
                                hipStream_t stream);
 
 /*
+ * Causal linear attention with a decay a head: S_t = decay[h] S_{t-1} + k_t^T v_t, out_t = scale q_t S_t, for the tokens
+ * t < lengths[b] (int32, clamped to 0..L; null = L) of each sequence and head.  q, k (B, L, H, dk) and v, out
+ * (B, L, H, dv) are fp16 or bf16 with strides per (batch, token, head) in elements, a head's values side by side, rows
+ * at multiples of 16 bytes; dk is a multiple of 8 up to 128, dv of 8 up to 256.  decay (H) is fp32 in 0..1.  state
+ * (null = zeros) and state_out (null = not wanted) are fp32 matrices (dk, dv), contiguous, with strides per
+ * (batch, head) in elements, at multiples of 16 bytes; state_out receives the state behind a sequence's last token, the
+ * state itself where it has none.  out is zero behind the last token.  The state, sums and powers of the decay are fp32.
+ * A value that is not finite reaches the outputs from its own token on and the state.  state_out may be state itself;
+ * otherwise outputs share no memory with inputs.
+ * With scratch memory (16-byte aligned, of at least sengine_amd_decay_attention_workspace's bytes; what it holds before
+ * does not matter) few heads of many tokens are computed in segments beside each other, joined in a fixed order; without
+ * it, or with less, one workgroup goes through a head's tokens.
+ */
+typedef struct sengine_decay_desc {
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  int64_t state_stride[2], state_out_stride[2];
+  int32_t B, L, H, dk, dv;
+  int32_t type;
+  float scale;
+} sengine_decay_desc;
+int sengine_amd_decay_attention(const sengine_decay_desc* d, const void* q, const void* k, const void* v,
+                                const float* decay, const float* state, const int32_t* lengths, void* out,
+                                float* state_out, hipStream_t stream);
+int sengine_amd_decay_attention_workspace(const sengine_decay_desc* d, size_t* bytes);
+int sengine_amd_decay_attention_ws(const sengine_decay_desc* d, const void* q, const void* k, const void* v,
+                                   const float* decay, const float* state, const int32_t* lengths, void* out,
+                                   float* state_out, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
  * Peak calibration on the box (the role of the reference's sengine/tuning/hw_calibrate.py:
  * 17-134, which times a memcpy and a dense fp16 GEMM).  Measurement entry points, not on
  * the operator path.

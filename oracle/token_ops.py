@@ -142,3 +142,41 @@ def linear_e2m1(x, weight, group_scale, row_scale, bias, act, residual, out_dtyp
     """(value, bound): the products of codes and scales are exact, so the linear operator's bound holds."""
     w = e2m1_weight(weight, group_scale, x.shape[-1])
     return linear(x, w, bias, act, residual, None, row_scale, out_dtype)
+
+
+def decay_attention(q, k, v, decay, state=None, lengths=None, scale=None):
+    """((value, bound) of the outputs, (value, bound) of the states), token after token."""
+    B, L, H, dk = q.shape
+    dv = v.shape[3]
+    scale = 1 / math.sqrt(dk) if scale is None else scale
+    S = torch.zeros((B, H, dk, dv), dtype=torch.float64, device=q.device) if state is None else state.double().clone()
+    A, G, F = S.abs(), torch.zeros_like(S), torch.zeros_like(S[..., :1])  # sums of magnitudes, and what they are off by
+    out = torch.zeros((B, L, H, dv), dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(out)
+    g = decay.double()[None, :, None, None]
+    f = torch.finfo(q.dtype)
+    # Relative to the sums of magnitudes.  A term of a state is a sum of 16-bit values, 24 bits of them, or with fp16 22;
+    # it and its two or three parts round by up to 2 U each when they are added.  Fp16's second part is 2^11 times as large
+    # as what it stands for and lies on steps of 2^-24 at the least, after the decay within its chunk: each token adds
+    # up to |k| 2^-36, whatever its age (F; chunks' own decay is left out of it).  A term's decay after
+    # m tokens is a product of powers, each off by its exponent's rounding (a logarithm off by a unit, a product: |ln g|
+    # 2^-22 a token) and by a unit itself, one a chunk of 64 tokens and a few more.  Outputs take the state and the
+    # weights Q K^T . D as sums of two values, 2^-18 of them in bf16 and 2^-23 in fp16, and have sums of dk and 64 terms.
+    each = torch.where(g > 0, -torch.log(g.clamp(min=1e-30)), 0.0) * 2.0**-22 + 2.0**-27 + 6 * U
+    low = 2.0**-36 if q.dtype == torch.float16 else 0
+    two = 2.0**-17 if q.dtype == torch.bfloat16 else 2.0**-21
+    n = torch.full((B,), L, device=q.device) if lengths is None else lengths.long().clamp(0, L)
+    for t in range(int(n.max()) if B and L else 0):
+        on = (t < n)[:, None, None, None]
+        qt, kt, vt = (x[:, t].double() for x in (q, k, v))
+        qt, kt, vt = (torch.where(on[..., 0], x, 0.0) for x in (qt, kt, vt))
+        kv = kt[..., :, None] * vt[..., None, :]
+        S = torch.where(on, g * S + kv, S)
+        G, F = torch.where(on, g * (G + A * each), G), F + kt.abs()[..., None] * low
+        A = torch.where(on, g * A + kv.abs(), A)
+        o, a, e = ((x[..., None, :] @ m)[..., 0, :] * abs(scale) for x, m in ((qt, S), (qt.abs(), A), (qt.abs(), G + F)))
+        out[:, t] = torch.where(on[..., 0], o * math.copysign(1, scale), 0.0)
+        bound[:, t] = torch.where(on[..., 0], a * (two + (2 * dk + 160) * U) + e, 0.0)
+    tiny = f.smallest_normal * f.eps if q.dtype == torch.float16 else 0
+    return ((out, torch.where(out != 0, bound + half_step(out, q.dtype) + tiny, bound)),
+            (S, A * (2.0**-21 if q.dtype == torch.float16 else 2.0**-22) + A * 140 * U + G + F))

@@ -88,12 +88,23 @@ class LinearE2m1Desc(ctypes.Structure):
     ]
 
 
+class DecayDesc(ctypes.Structure):
+    """Mirror of ``sengine_decay_desc``."""
+
+    _fields_ = [
+        ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+        ("out_stride", ctypes.c_int64 * 3), ("state_stride", ctypes.c_int64 * 2),
+        ("state_out_stride", ctypes.c_int64 * 2), ("B", ctypes.c_int32), ("L", ctypes.c_int32), ("H", ctypes.c_int32),
+        ("dk", ctypes.c_int32), ("dv", ctypes.c_int32), ("type", ctypes.c_int32), ("scale", ctypes.c_float),
+    ]
+
+
 _P = ctypes.c_void_p
 _DP = ctypes.POINTER(ConvLifDesc)
 _I32, _I64, _F = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 _SZP = ctypes.POINTER(ctypes.c_size_t)
 _NDP, _LDP, _CDP = ctypes.POINTER(RmsNormDesc), ctypes.POINTER(LinearDesc), ctypes.POINTER(CrossDesc)
-_RDP, _L4DP = ctypes.POINTER(RotaryDesc), ctypes.POINTER(LinearE2m1Desc)
+_RDP, _L4DP, _DDP = ctypes.POINTER(RotaryDesc), ctypes.POINTER(LinearE2m1Desc), ctypes.POINTER(DecayDesc)
 
 # name -> (restype, argtypes); every symbol declared in include/sengine_amd.h
 SIGNATURES = {
@@ -153,6 +164,9 @@ SIGNATURES = {
     "sengine_amd_linear_e2m1": (ctypes.c_int, [_L4DP, _P, _P, _P, _P, _P, _P, _P, _P]),
     "sengine_amd_linear_e2m1_workspace": (ctypes.c_int, [_L4DP, _SZP]),
     "sengine_amd_linear_e2m1_ws": (ctypes.c_int, [_L4DP, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "sengine_amd_decay_attention": (ctypes.c_int, [_DDP, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "sengine_amd_decay_attention_workspace": (ctypes.c_int, [_DDP, _SZP]),
+    "sengine_amd_decay_attention_ws": (ctypes.c_int, [_DDP, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "sengine_amd_pack_spikes": (ctypes.c_int, [_P, _I32, _I64, _I32, _P, _P]),
     "sengine_amd_unpack_spikes": (ctypes.c_int, [_P, _I64, _I32, _P, _I32, _P]),
 }

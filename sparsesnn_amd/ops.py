@@ -18,8 +18,8 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import (ACTIVATIONS, ENC_BF16, ENC_BITS, ENC_E4M3, ENC_F16, ENC_F32, NEURON_IF, NEURON_LIF, NEURON_MS,
-                   WLAYOUT_HWIO, WLAYOUT_OIHW, ConvLifDesc, CrossDesc, LinearDesc, LinearE2m1Desc, RmsNormDesc, RotaryDesc,
-                   SEngineError, check)
+                   WLAYOUT_HWIO, WLAYOUT_OIHW, ConvLifDesc, CrossDesc, DecayDesc, LinearDesc, LinearE2m1Desc, RmsNormDesc,
+                   RotaryDesc, SEngineError, check)
 
 __all__ = [
     "ConvSpec", "make_desc", "geometry", "set_fused_kernel", "compress_2_4", "pack_dense_weights", "pack_spikes",
@@ -28,8 +28,8 @@ __all__ = [
     "ENC_BITS", "ENC_F16", "ENC_F32", "NEURON_LIF", "NEURON_IF", "NEURON_MS", "WLAYOUT_OIHW", "WLAYOUT_HWIO",
     "neuron_code", "fused_sparse_conv_bn_add_neuron", "spiking_self_attention", "stem_conv_bn_neuron",
     "fused_sparse_conv_bn_lif_pair", "fused_sparse_conv_bn_lif_split", "fused_sparse_conv_bn_lif_tail", "tail_eligible",
-    "fused_plan", "rms_norm", "linear", "cross_attention", "rotary", "linear_e2m1", "ENC_BF16",
-    "ENC_E4M3",
+    "fused_plan", "rms_norm", "linear", "cross_attention", "rotary", "linear_e2m1", "decay_attention",
+    "ENC_BF16", "ENC_E4M3",
 ]
 
 
@@ -1408,3 +1408,103 @@ def linear_e2m1(x: torch.Tensor, weight: torch.Tensor, group_scale: torch.Tensor
         desc, x.data_ptr(), weight.data_ptr(), group_scale.data_ptr(), _ptr(row_scale), _ptr(bias), _ptr(residual),
         out.data_ptr(), _ptr(ws), size, _stream(dev)), "linear_e2m1")
     return out
+
+
+def _decay_plan(key, q, k, v, decay, state, lengths, scale, out, state_out):
+    """(descriptor, bytes of scratch memory, output's and state's shapes, device) of a checked call."""
+    _token_input(q, "q")
+    dev, code = q.device, _type_code(q, (torch.float16, torch.bfloat16), "q")
+    for t, name in ((k, "k"), (v, "v")):
+        _token_input(t, name, dev)
+        if t.dtype != q.dtype:
+            raise SEngineError(f"{name}: expected {q.dtype}, got {t.dtype}")
+    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:3] != q.shape[:3]:
+        raise SEngineError(f"decay_attention: expected q, k (B, L, H, dk) and v (B, L, H, dv), got {tuple(q.shape)}, "
+                           f"{tuple(k.shape)}, {tuple(v.shape)}")
+    (B, L, H, dk), dv = q.shape, v.shape[3]
+    _token_sizes("decay_attention: B, L, heads, dk and dv", B, L, H, dk, dv)
+    _token_vector(decay, H, "decay", dev)
+    _type_code(decay, (torch.float32,), "decay")
+    if lengths is not None:
+        _token_vector(lengths, B, "lengths", dev)
+        if lengths.dtype != torch.int32:
+            raise SEngineError(f"lengths: expected dtype torch.int32, got {lengths.dtype}")
+    shape, matrices = (B, L, H, dv), (B, H, dk, dv)
+    strides = []
+    for t, x, name in ((q, q, "q"), (k, k, "k"), (v, v, "v"), (out, v, "out")):
+        if name == "out":
+            if t is None:
+                strides.append((ctypes.c_int64 * 3)(L * H * dv, H * dv, dv))
+                continue
+            _heads_out(t, x.shape, q.dtype, name, dev)
+        strides.append(_head_strides(t, name))
+        if t.numel() and any(n > 1 and s % 8 for n, s in zip(t.shape, strides[-1])):
+            raise SEngineError(f"{name}: rows must begin at multiples of 16 bytes (strides {t.stride()})")
+    for t, name in ((state, "state"), (state_out, "state_out")):
+        if t is None:
+            strides.append((ctypes.c_int64 * 2)(*((H * dk * dv, dk * dv) if name == "state_out" else (0, 0))))
+            continue
+        if name == "state":
+            _token_input(t, name, dev)
+        else:
+            _heads_out(t, matrices, torch.float32, name, dev)
+        if t.dtype != torch.float32 or tuple(t.shape) != matrices:
+            raise SEngineError(f"{name}: expected torch.float32 {matrices}, got {t.dtype} {tuple(t.shape)}")
+        s = t.stride()
+        if t.numel() and ((dv > 1 and s[3] != 1) or (dk > 1 and s[2] != dv) or (B > 1 and s[0] % 4) or (H > 1 and s[1] % 4)):
+            raise SEngineError(f"{name}: its matrices must be contiguous and begin at multiples of 16 bytes (strides {s})")
+        strides.append((ctypes.c_int64 * 2)(*(x if n > 1 else 0 for n, x in zip(matrices, s[:2]))))
+    desc = ctypes.byref(DecayDesc(*strides, B, L, H, dk, dv, code, 1.0 / math.sqrt(dk) if scale is None else scale))
+    size = ctypes.c_size_t()
+    check(_lib.load().sengine_amd_decay_attention_workspace(desc, ctypes.byref(size)), "decay_attention")
+    return _remember(key, (desc, size.value, shape, matrices, dev))
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
+                    state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    state_out: Optional[torch.Tensor] = None):
+    """Causal linear attention with a decay a head: S_t = decay[h] S_{t-1} + k_t^T v_t, o_t = scale q_t S_t.  Returns
+    (o, S), o (B, L, H, dv) in q's type and the state behind each sequence's last token (B, H, dk, dv), fp32.
+
+    q and k are (B, L, H, dk), v is (B, L, H, dv), fp16 or bf16; dk is a multiple of 8 up to 128, dv of 8 up to 256; scale
+    1 / sqrt(dk) by default.  decay (H,) fp32 in 0..1: the leak of a head's state a token.  state (B, H, dk, dv) fp32 is
+    what the sequences begin with, zeros where None: a prompt is one call, and its state the next call's, of a token or of
+    many.  lengths (B,) int32: the tokens of each sequence (clamped to 0..L); what lies behind them is not used, its
+    outputs are zeros and leave the state alone.  Any strides whose rows are contiguous and begin at multiples of 16
+    bytes.  The state and all sums are fp32; long prompts are matrix products of 16-bit operands that hold what is not
+    16-bit by itself, state and weights, as sums of two or three.  A value of v that is not finite reaches the outputs
+    from its own token on.  `state_out` may be `state`, updated in place; otherwise outputs share no memory with inputs.
+    Few heads of many tokens are computed in segments through scratch memory of torch's allocator, joined in a fixed
+    order."""
+    if _dispatch_modes() or forward_ad._current_level >= 0:
+        _token_modes(q, k, v, decay, state, scale)
+    if scale is not None and type(scale) is not float:
+        scale = _token_number(scale, "scale")
+    key = None
+    if out is None and state_out is None:
+        try:
+            key = ("decay", q.dtype, q.shape, q.stride(), q.device, k.dtype, k.shape, k.stride(), k.device, v.dtype,
+                   v.shape, v.stride(), v.device, _layout(decay), _layout(state), _layout(lengths), scale)
+        except AttributeError:
+            pass  # not a tensor: the checks say so
+    plan = _TOKEN_PLANS.get(key)
+    if plan is None or (torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (q, k, v, decay, state))):
+        plan = _decay_plan(key, q, k, v, decay, state, lengths, scale, out, state_out)
+    desc, size, shape, matrices, dev = plan
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    if state_out is None:
+        state_out = torch.empty(matrices, dtype=torch.float32, device=dev)
+    pointers = qp, kp, vp, op, sp, tp = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(state) or 0,
+                                         state_out.data_ptr())
+    if (qp | kp | vp | op | sp | tp) & 15:
+        for x, t, name in zip(pointers, (q, k, v, out, state, state_out), ("q", "k", "v", "out", "state", "state_out")):
+            if x & 15 and t.numel():
+                raise SEngineError(f"{name}: must begin at a multiple of 16 bytes")
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    check(_lib.load().sengine_amd_decay_attention_ws(
+        desc, qp, kp, vp, decay.data_ptr(), sp or None, _ptr(lengths), op, tp, _ptr(ws), size, _stream(dev)),
+        "decay_attention")
+    return out, state_out

@@ -156,10 +156,13 @@ struct DecayPlan {
 constexpr int kDecaySteps = 16;  // most tokens that go one by one
 
 static DecayPlan plan(const sengine_decay_desc* d) {
-  if (d->L <= kDecaySteps) return {true, 1, d->L};
+  // the chunks' copies have offsets of 31 bits from a chunk's first token on
+  const auto near = [](int64_t stride) { return stride >= 0 && stride < 1 << 23; };
+  if (d->L <= kDecaySteps || !near(d->q_stride[1]) || !near(d->k_stride[1]) || !near(d->v_stride[1]))
+    return {true, 1, d->L};
   const int chunks = (int)(((int64_t)d->L + kDecayChunk - 1) / kDecayChunk);
-  const int waves = decay_waves(d->dv);
-  const int64_t wanted = 2048 / waves / ((int64_t)d->B * d->H);  // workgroups that fill the chip
+  const int64_t slices = (d->dv + kDecayColumns - 1) / kDecayColumns;
+  const int64_t wanted = 2048 / decay_waves(d->dv) / ((int64_t)d->B * d->H * slices);  // two waves a SIMD
   int64_t segs = wanted < chunks / 4 ? wanted : chunks / 4;
   if (segs < 2) return {false, 1, chunks * kDecayChunk};
   const int64_t per = (chunks + segs - 1) / segs;
@@ -173,10 +176,10 @@ static size_t workspace_of(const sengine_decay_desc* d, const DecayPlan& q) {
 
 template <class T, int DKP, int NW>
 static hipError_t run_chunks(const DecayParams& p, hipStream_t stream) {
-  const int64_t heads = (int64_t)p.B * p.H;
-  if (!launchable(heads * p.segs, 64 * NW)) return hipErrorInvalidConfiguration;
+  const int64_t heads = (int64_t)p.B * p.H, parts = heads * ((p.dv + kDecayColumns - 1) / kDecayColumns);
+  if (!launchable(parts * p.segs, 64 * NW)) return hipErrorInvalidConfiguration;
   if (p.segs > 1) {
-    decay_chunk_kernel<T, DKP, NW, true><<<dim3((unsigned)(heads * (p.segs - 1))), dim3(64 * NW), 0, stream>>>(p);
+    decay_chunk_kernel<T, DKP, NW, true><<<dim3((unsigned)(parts * (p.segs - 1))), dim3(64 * NW), 0, stream>>>(p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int per_state = p.dk * p.dv / 4;
@@ -184,17 +187,17 @@ static hipError_t run_chunks(const DecayParams& p, hipStream_t stream) {
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  decay_chunk_kernel<T, DKP, NW, false><<<dim3((unsigned)(heads * p.segs)), dim3(64 * NW), 0, stream>>>(p);
+  decay_chunk_kernel<T, DKP, NW, false><<<dim3((unsigned)(parts * p.segs)), dim3(64 * NW), 0, stream>>>(p);
   return hipGetLastError();
 }
 
 template <class T, int DKP>
 static hipError_t by_values(const DecayParams& p, hipStream_t stream) {
   switch (decay_waves(p.dv)) {
-    case 1:
-      return run_chunks<T, DKP, 1>(p, stream);
     case 2:
       return run_chunks<T, DKP, 2>(p, stream);
+    case 3:
+      return run_chunks<T, DKP, 3>(p, stream);
     case 4:
       return run_chunks<T, DKP, 4>(p, stream);
     default:

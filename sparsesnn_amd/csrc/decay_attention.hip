@@ -161,25 +161,33 @@ static DecayPlan plan(const sengine_decay_desc* d) {
   if (d->L <= kDecaySteps || !near(d->q_stride[1]) || !near(d->k_stride[1]) || !near(d->v_stride[1]))
     return {true, 1, d->L};
   const int chunks = (int)(((int64_t)d->L + kDecayChunk - 1) / kDecayChunk);
-  const int64_t slices = (d->dv + kDecayColumns - 1) / kDecayColumns;
-  const int64_t wanted = 2048 / decay_waves(d->dv) / ((int64_t)d->B * d->H * slices);  // two waves a SIMD
-  int64_t segs = wanted < chunks / 4 ? wanted : chunks / 4;
-  if (segs < 2) return {false, 1, chunks * kDecayChunk};
-  const int64_t per = (chunks + segs - 1) / segs;
-  segs = (chunks + per - 1) / per;
-  return {false, (int)segs, (int)per * kDecayChunk};
+  // Rounds of workgroups over the chip, times the chunks of one and a start, half as much again for the pass that makes the
+  // segments' states; and two launches more and the states' joining, in the time of chunks.
+  const int64_t heads = (int64_t)d->B * d->H * ((d->dv + kDecayColumns - 1) / kDecayColumns);
+  const int64_t slots = 256 * decay_resident(d->dk, d->dv);
+  int best = chunks;  // chunks of a segment
+  float least = (float)((heads + slots - 1) / slots) * (float)(chunks + 1);
+  for (int segs = 2; segs <= chunks && segs <= 256 && (segs - 1) * heads <= 2 * slots; ++segs) {
+    const int per = (chunks + segs - 1) / segs;
+    const int64_t rounds = (heads * ((chunks + per - 1) / per) + slots - 1) / slots;
+    const float cost = 1.5f * (float)rounds * (float)(per + 1) + 3.f + (float)segs / 16.f;
+    if (cost < least) least = cost, best = per;
+  }
+  return {false, (chunks + best - 1) / best, best * kDecayChunk};
 }
 
 static size_t workspace_of(const sengine_decay_desc* d, const DecayPlan& q) {
   return (size_t)d->B * d->H * (q.segs - 1) * d->dk * d->dv * 4;
 }
 
-template <class T, int DKP, int NW>
+template <class T, int DKP, int BLOCKS>
 static hipError_t run_chunks(const DecayParams& p, hipStream_t stream) {
+  constexpr int NV = decay_own(BLOCKS), NW = BLOCKS / NV;
   const int64_t heads = (int64_t)p.B * p.H, parts = heads * ((p.dv + kDecayColumns - 1) / kDecayColumns);
-  if (!launchable(parts * p.segs, 64 * NW)) return hipErrorInvalidConfiguration;
+  if (!launchable(parts * p.segs, 64 * BLOCKS)) return hipErrorInvalidConfiguration;
   if (p.segs > 1) {
-    decay_chunk_kernel<T, DKP, NW, true><<<dim3((unsigned)(parts * (p.segs - 1))), dim3(64 * NW), 0, stream>>>(p);
+    decay_chunk_kernel<T, DKP, 1, BLOCKS, true>
+        <<<dim3((unsigned)(parts * (p.segs - 1))), dim3(64 * BLOCKS), 0, stream>>>(p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int per_state = p.dk * p.dv / 4;
@@ -187,13 +195,13 @@ static hipError_t run_chunks(const DecayParams& p, hipStream_t stream) {
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  decay_chunk_kernel<T, DKP, NW, false><<<dim3((unsigned)(parts * p.segs)), dim3(64 * NW), 0, stream>>>(p);
+  decay_chunk_kernel<T, DKP, NV, NW, false><<<dim3((unsigned)(parts * p.segs)), dim3(64 * NW), 0, stream>>>(p);
   return hipGetLastError();
 }
 
 template <class T, int DKP>
 static hipError_t by_values(const DecayParams& p, hipStream_t stream) {
-  switch (decay_waves(p.dv)) {
+  switch (decay_blocks(p.dv)) {
     case 2:
       return run_chunks<T, DKP, 2>(p, stream);
     case 3:

@@ -2,10 +2,13 @@
 // it begins with,
 //   O  = scale ((Q K^T . D) V + L Q S),   D[i][j] = g^(i - j) for j <= i, else 0,   L[i] = g^(i + 1)
 //   S' = g^n S + K^T W V,                 W[j] = g^(n - 1 - j)
-// Workgroup = one head of one sequence, or of a segment of it, and up to 128 columns of V; a wave has 16 columns of V, S
-// and O, and S stays in its registers.  The memory pipeline copies the next chunk's rows into one half of LDS beside the
-// products with the other.  The ten 16 x 16 blocks of Q K^T . D that count are shared out over the waves and go through
-// LDS; while they are made, the other products need only what the wave has.
+// Workgroup = one head of one sequence, or of a segment of it, and up to 128 columns of V; a wave has 16 or 32 columns of V,
+// S and O, and S stays in its registers.  The memory pipeline copies a chunk's rows into LDS once those before have been
+// read, and several workgroups a CU fill each other's waits.  The ten 16 x 16 blocks of Q K^T . D that count are shared out
+// over the waves and go through LDS; while they are made, the other products need only what the wave has.
+//
+// Few heads: a first pass makes each segment's state from a state of zeros (K and V only, copies one chunk ahead), and
+// decay_scan_kernel joins them, so that K and V are read twice.
 //
 // All products are 16x16x32 matrix instructions, laid out so that what one leaves is what the next one takes:
 //   * K Q^T puts four tokens j of one token i in a lane: two such blocks, side by side in LDS, are the second operand of
@@ -15,7 +18,8 @@
 //
 // Rounding.  S is fp32.  What a 16-bit instruction takes of it and of the fp32 weights Q K^T . D is a sum of two 16-bit
 // values (of bf16, 16 bits; S of fp16, 22), so that O is as exact as its own rounding; W V, which makes S, is a sum of
-// three (bf16) or two (fp16, the second 2^11 times larger so that it does not fall below the type's range).  Weights
+// two: in bf16 of three where the last state keeps more than 2^-10 of it, in fp16 with the second 2^11 times larger so that
+// it does not fall below the type's range.  Weights
 // easily pass fp16's range: they are bf16 values always, and fp16 values of V are sums of two of them, exactly.  A
 // column of S is scaled by a power of two to fp16's range.
 //
@@ -49,8 +53,20 @@ struct DecayParams {
 constexpr int kDecayChunk = 64;
 constexpr int kDecayColumns = 128;  // most columns of V of a workgroup
 
-// Waves of a workgroup: 16 columns each.
-__host__ __device__ inline int decay_waves(int dv) { return dv <= 32 ? 2 : dv <= 48 ? 3 : dv <= 64 ? 4 : 8; }
+// Columns of V of a workgroup, in 16s; how many of them a wave has, and the waves a SIMD that its registers are limited to.
+// Measured, us: 64 columns, 64 heads of 64 over 12544 tokens, bf16: a wave 16 columns and two waves a SIMD 151, three 166, 32
+// columns 187; 48 columns of fp16: three 154, two 165; 128 columns, 16 heads of 128 over 65536 tokens: a wave 32 columns 394,
+// 16 columns 487.
+__host__ __device__ constexpr int decay_blocks(int dv) { return dv <= 32 ? 2 : dv <= 48 ? 3 : dv <= 64 ? 4 : 8; }
+__host__ __device__ constexpr int decay_own(int blocks) { return blocks == 8 ? 2 : 1; }
+__host__ __device__ constexpr int decay_waves(int blocks) { return blocks < 4 ? 3 : 2; }
+
+// Workgroups that a CU holds.
+inline int decay_resident(int dk, int dv) {
+  const int blocks = decay_blocks(dv), pk = dk <= 32 ? 4 : dk <= 64 ? 8 : 16, pv = blocks == 3 ? 8 : blocks * 2;
+  const int by_lds = 160 / (2 * pk + pv + 12 + 1), by_waves = 4 * decay_waves(blocks) / (blocks / decay_own(blocks));
+  return by_lds < by_waves ? by_lds : by_waves;
+}
 
 // g^n from log2 g: 1 for n = 0, also of g = 0.
 __device__ __forceinline__ float decay_log2(float g) { return log2f(g); }
@@ -89,7 +105,20 @@ __device__ __forceinline__ auto decay_term(float (&x)[N]) {
   const auto r = decay_pack<T>(x);
   const vec_t v = __builtin_bit_cast(vec_t, r);
 #pragma unroll
-  for (int e = 0; e < N; ++e) x[e] -= (float)v[e];
+  for (int e = 0; e < N; ++e) {
+    if constexpr (__is_same(T, __bf16)) {
+      // x - v by the instruction that adds a pair's products to x: a widened v would take one more.  (A neighbour that is
+      // not finite makes x a NaN: the sum that both belong to is one anyway.)  The factors (-1, 0) and (0, -1) are kept
+      // from the compiler, which takes the first for its inline constant -1, of which the instruction has the other half.
+      typedef __bf16 pair_t __attribute__((ext_vector_type(2)));
+      uint32_t minus = e % 2 ? 0xbf800000u : 0x0000bf80u;
+      asm("" : "+s"(minus));
+      const uint32_t word = r[e / 2];
+      x[e] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair_t, word), __builtin_bit_cast(pair_t, minus), x[e], false);
+    } else {
+      x[e] = __builtin_fmaf((float)v[e], -1.f, x[e]);
+    }
+  }
   return r;
 }
 
@@ -124,21 +153,25 @@ __device__ __forceinline__ u32x4_t decay_replace(u32x4_t v, uint16_t instead) {
   return __builtin_bit_cast(u32x4_t, t);
 }
 
-// DKP: dk rounded up to 32, 64 or 128.  STATE: a segment's state from a state of zeros, without outputs.
-template <class T, int DKP, int NW, bool STATE>
-__global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(DecayParams p) {
+// Place of the operand of tokens j 32 y .. of the tokens i of block x.
+__device__ __forceinline__ int decay_operand(int x, int y) { return x < 2 ? x : 2 * x - 2 + y; }
+
+// DKP: dk rounded up to 32, 64 or 128; NW waves of 16 NV columns.  STATE: a segment's state from a state of zeros,
+// without outputs.
+template <class T, int DKP, int NV, int NW, bool STATE>
+__global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void decay_chunk_kernel(DecayParams p) {
   constexpr bool HALF = __is_same(T, _Float16);
-  constexpr int C = kDecayChunk;
-  constexpr int PK = DKP / 8, PV = NW == 3 ? 8 : NW * 2;  // pieces of a row of Q or K, of V
+  constexpr int C = kDecayChunk, STAGES = STATE ? 2 : 1;
+  constexpr int PK = DKP / 8, PV = NV * NW == 3 ? 8 : NV * NW * 2;  // pieces of a row of Q or K, of V
   constexpr int NM = DKP / 32, NK = DKP / 16;
   constexpr int NC = PK * (STATE ? 1 : 2) + PV, NCW = (NC + NW - 1) / NW;  // copies of 1 KB a chunk, of a wave
   constexpr int kStage = NC * 1024;
   constexpr int kQ = (PK + PV) * 1024;  // a stage: K, V, Q
-  constexpr int kP = 8 * 1024;          // blocks of Q K^T . D: 4 x 2 operands, the first terms and then the second
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage + (STATE ? 0 : 2 * kP)];
-  __shared__ float powers[C];  // scale g^n
+  constexpr int kP = 6 * 1024;          // blocks of Q K^T . D: six operands' first terms, then their second ones
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[STAGES * kStage + (STATE ? 0 : 2 * kP)];
+  __shared__ float powers[16 + C + 1], behind[2 * C];  // scale g^(n - 16), zeros up to there; g^(C - 1 - j), zeros behind
   const int tid = (int)threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, a = lane & 15;
   // neighbouring heads of a segment on one XCD: where their rows share cache lines they are fetched once
   const int segs = STATE ? p.segs - 1 : p.segs;
@@ -161,29 +194,24 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(DecayParams p) 
 
   // powers of the decay as the lanes need them
   const float lg = decay_log2(p.decay[h]);
-  float begun[4], weight[4][4];  // scale L, W
-#pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    begun[x] = p.scale * decay_power(lg, 16 * x + a + 1);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) weight[x][e] = decay_power(lg, C - 1 - (16 * x + 4 * g + e));
+  for (int i = tid; i < 2 * C; i += 64 * NW) {
+    if (i <= 16 + C) powers[i] = i < 16 ? 0.f : p.scale * decay_power(lg, i - 16);
+    behind[i] = i < C ? decay_power(lg, C - 1 - i) : 0.f;
   }
-  float passed = decay_power(lg, C);
-  if constexpr (!STATE) {
-    if (tid < C) powers[tid] = p.scale * decay_power(lg, tid);
-    // blocks above the diagonal that share an operand with one that counts stay zeros
-    for (int i = tid; i < 2 * kP / 16; i += 64 * NW)
-      *reinterpret_cast<u32x4_t*>(smem + 2 * kStage + i * 16) = u32x4_t{0, 0, 0, 0};
-  }
+  // blocks above the diagonal that share an operand with one that counts stay zeros
+  for (int i = tid; i < (STATE ? 0 : 2 * kP / 16); i += 64 * NW)
+    *reinterpret_cast<u32x4_t*>(smem + STAGES * kStage + i * 16) = u32x4_t{0, 0, 0, 0};
 
-  // S: value i of fragment f is row 32 (f / 2) + 8 g + 4 (f % 2) + i, column a of the wave's
-  const int column = wave * 16 + a;
-  const bool used = wave * 16 < width;  // whether the wave has columns
-  float4_t S[NK];
-  const auto state_at = [&](int f, int i) {
-    return (int64_t)(32 * (f / 2) + 8 * g + 4 * (f % 2) + i) * p.dv + slice * kDecayColumns + column;
+  // S: value i of fragment [f][c] is row 32 (f / 2) + 8 g + 4 (f % 2) + i, column 16 c + a of the wave's
+  const int column = wave * 16 * NV + a;
+  const bool used = wave * 16 * NV < width;  // whether the wave has columns
+  float4_t S[NK][NV];
+  const auto state_at = [&](int f, int c, int i) {
+    return (int64_t)(32 * (f / 2) + 8 * g + 4 * (f % 2) + i) * p.dv + slice * kDecayColumns + column + 16 * c;
   };
-  const auto has_state = [&](int f, int i) { return 32 * (f / 2) + 8 * g + 4 * (f % 2) + i < p.dk && column < width; };
+  const auto has_state = [&](int f, int c, int i, int dk) {
+    return 32 * (f / 2) + 8 * g + 4 * (f % 2) + i < dk && column + 16 * c < width;
+  };
   const int64_t bh = b * p.H + h;
   const int64_t matrix = (int64_t)p.dk * p.dv;
   const float* from = STATE ? nullptr
@@ -193,7 +221,9 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(DecayParams p) 
 #pragma unroll
   for (int f = 0; f < NK; ++f)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) S[f][i] = from && has_state(f, i) ? from[state_at(f, i)] : 0.f;
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[f][c][i] = from && has_state(f, c, i, p.dk) ? from[state_at(f, c, i)] : 0.f;
 
   // This wave's copies: c = wave, wave + NW, .. of a stage's PK of K, PV of V, PK of Q.  A lane's 16 bytes are place
   // lane % P of a row; the piece that belongs there is fetched, or nothing where the row has none.
@@ -220,47 +250,55 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(DecayParams p) 
       lds_copy(c < PK ? kr : c < PK + PV ? vr : qr, lds0 + stage * kStage + c * 1024, voff[i]);
     }
   };
-  const auto rows = [&](const uint8_t* s, int block, int m) {  // 16 rows, values 32 m ..
-    return *reinterpret_cast<const u32x4_t*>(s + decay_at<PK>(16 * block + a, 4 * m + g));
-  };
-  // 32 tokens transposed: 16 columns whose pieces of four values are halves `half` of 16-byte pieces j
-  const auto columns = [&](const uint8_t* s, auto pieces, int step, int j, int half) {
-    constexpr int P = decltype(pieces)::value;
-    const int r = 32 * step + 4 * g + (a >> 2);
-    return read_transposed(s + decay_at<P>(r, j) + 8 * half, s + decay_at<P>(r + 16, j) + 8 * half);
+  // Where in LDS a lane's share begins: of 16 rows, their values 32 m + 8 g ..; of 32 tokens transposed, the columns 32 m + 8 p
+  // .. (p = a % 4) of K and 16 c .. of the wave's of V.  What else an address has is the same for all lanes.
+  int at_rows[NM], at_k[NM], at_v[NV];
+#pragma unroll
+  for (int m = 0; m < NM; ++m) {
+    at_rows[m] = decay_at<PK>(a, 4 * m + g);
+    at_k[m] = decay_at<PK>(4 * g + (a >> 2), 4 * m + (a & 3));
+  }
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+    at_v[c] = PK * 1024 + decay_at<PV>(4 * g + (a >> 2), 2 * (wave * NV + c) + ((a & 3) >> 1)) + 8 * (a & 1);
+  const auto transposed = [&](int at, int pitch) { return read_transposed(smem + at, smem + at + 16 * pitch); };
+  const auto meet = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if constexpr (NW > 1) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
 
+  // Tokens from here on count in the last state so much that what two terms of W V leave out would show; for outputs two
+  // are enough.
+  int late = 0;
+  if constexpr (!HALF) {
+    const float from_end = 10.f / -lg;  // tokens until less than 2^-10 is left
+    const float to = (float)(n - begin) - from_end;
+    late = !p.state_out ? left : to > 0.f ? (int)to / C * C : 0;
+    late = late < left ? late : left;
+  }
+  uint8_t* const sP = smem + STAGES * kStage;
   if (left > 0) copy(0, 0);
-  for (int t0 = 0, stage = 0; t0 < left; t0 += C, stage ^= 1) {
-    // this wave's copies have landed and its reads of the other stage and the blocks are done; so are all waves'
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (t0 + C < left) copy(t0 + C, stage ^ 1);
-    const uint8_t* const sK = smem + stage * kStage;
-    const uint8_t* const sV = sK + PK * 1024;
-    const uint8_t* const sQ = sK + kQ;
-    uint8_t* const sP = smem + 2 * kStage;
+  int t0 = 0, stage = 0;
+  const auto chunk = [&](auto terms) {
+    constexpr int TERMS = decltype(terms)::value;
+    // this wave's copies have landed and its reads of the blocks are done; so are all waves'
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    meet();
+    if (STAGES == 2 && t0 + C < left) copy(t0 + C, stage ^ 1);
+    const int at0 = STAGES == 2 ? stage * kStage : 0;
     const int live = left - t0 < C ? left - t0 : C;
-    if (live < C) {  // the last chunk: its weights count from its last token
-      passed = decay_power(lg, live);
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int apart = live - 1 - (16 * x + 4 * g + e);
-          weight[x][e] = apart >= 0 ? decay_power(lg, apart) : 0.f;
-        }
-    }
 
     if constexpr (!STATE) {
       // Blocks of K Q^T . D: tokens j of block y, i of block x >= y; the wave's are number wave, wave + NW, ..
       constexpr int NB = (10 + NW - 1) / NW;
       float4_t P[NB];
       int bx[NB], by[NB];
+      int first = wave;
+      asm("" : "+s"(first));  // what follows from it is made here, not kept in registers from chunk to chunk
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
-        const int at = wave + u * NW < 10 ? wave + u * NW : 9;
+        const int at = first + u * NW < 10 ? first + u * NW : 9;
         bx[u] = at < 1 ? 0 : at < 3 ? 1 : at < 6 ? 2 : 3;
         by[u] = at - bx[u] * (bx[u] + 1) / 2;
         P[u] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -268,104 +306,138 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(DecayParams p) 
 #pragma unroll
       for (int m = 0; m < NM; ++m)
 #pragma unroll
-        for (int u = 0; u < NB; ++u) P[u] = mma_64b<T>(rows(sK, by[u], m), rows(sQ, bx[u], m), P[u]);
+        for (int u = 0; u < NB; ++u)
+          P[u] = mma_64b<T>(*reinterpret_cast<const u32x4_t*>(smem + at_rows[m] + by[u] * 16 * PK * 16),
+                            *reinterpret_cast<const u32x4_t*>(smem + kQ + at_rows[m] + bx[u] * 16 * PK * 16), P[u]);
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
+        const int ahead = 16 * (bx[u] - by[u]) + a - 4 * g;
         float w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int apart = 16 * (bx[u] - by[u]) + a - 4 * g - i;
-          w[i] = apart >= 0 ? P[u][i] * powers[apart & (C - 1)] : 0.f;  // whatever a later token holds
-        }
+        for (int i = 0; i < 4; ++i) w[i] = ahead >= i ? P[u][i] * powers[16 + ahead - i] : 0.f;  // whatever a later token holds
         const u32x2_t hi = decay_term<__bf16>(w), lo = decay_pack<__bf16>(w);
-        if (wave + u * NW < 10) {
-          uint8_t* const at = sP + ((bx[u] * 2 + by[u] / 2) * 64 + lane) * 16 + by[u] % 2 * 8;
+        if (first + u * NW < 10) {
+          uint8_t* const at = sP + (decay_operand(bx[u], by[u] / 2) * 64 + lane) * 16 + by[u] % 2 * 8;
           *reinterpret_cast<u32x2_t*>(at) = hi;
           *reinterpret_cast<u32x2_t*>(at + kP) = lo;
         }
       }
     }
 
-    u32x4_t V[2];  // tokens 32 x ..
+    u32x4_t V[2][NV];  // tokens 32 x .., columns 16 c ..
 #pragma unroll
-    for (int x = 0; x < 2; ++x) V[x] = columns(sV, Int<PV>{}, x, 2 * wave + ((a & 3) >> 1), a & 1);
-    float4_t O[4];
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+        V[x][c] = transposed(at0 + at_v[c] + x * 32 * PV * 16, PV * 16);
+    float4_t O[4][NV];
     if constexpr (!STATE) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) O[x] = float4_t{0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int c = 0; c < NV; ++c) O[x][c] = float4_t{0.f, 0.f, 0.f, 0.f};
       if (used) {  // S^T Q^T
-        float up = 1.f, down = 1.f;
-        if constexpr (HALF) {
-          uint32_t most = 0;
+        float up[NV], down[NV];
 #pragma unroll
-          for (int f = 0; f < NK; ++f)
+        for (int c = 0; c < NV; ++c) {
+          up[c] = down[c] = 1.f;
+          if constexpr (HALF) {
+            uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) most = decay_most(most, S[f][i]);
-          decay_range(decay_across(most), up, down);
+            for (int f = 0; f < NK; ++f)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) most = decay_most(most, S[f][c][i]);
+            decay_range(decay_across(most), up[c], down[c]);
+          }
         }
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-          float s[8];
+          u32x4_t hi[NV], lo[NV], r[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[e] = HALF ? S[2 * m + e / 4][e % 4] * up : S[2 * m + e / 4][e % 4];
-          const u32x4_t hi = decay_term<T>(s), lo = decay_pack<T>(s);
-          u32x4_t r[4];
+          for (int c = 0; c < NV; ++c) {
+            float s[8];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) r[x] = rows(sQ, x, m);
+            for (int e = 0; e < 8; ++e) s[e] = HALF ? S[2 * m + e / 4][c][e % 4] * up[c] : S[2 * m + e / 4][c][e % 4];
+            hi[c] = decay_term<T>(s);
+            lo[c] = decay_pack<T>(s);
+          }
 #pragma unroll
-          for (int x = 0; x < 4; ++x) O[x] = mma_64b<T>(hi, r[x], O[x]);
+          for (int x = 0; x < 4; ++x)
+            r[x] = *reinterpret_cast<const u32x4_t*>(smem + kQ + at_rows[m] + x * 16 * PK * 16);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) O[x] = mma_64b<T>(lo, r[x], O[x]);
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<T>(hi[c], r[x], O[x][c]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<T>(lo[c], r[x], O[x][c]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float back = HALF ? __shfl(down, 4 * g + i, 64) : 1.f;  // the column's factor where O has it
+        for (int x = 0; x < 4; ++x) {
+          const float begun = powers[16 + 16 * x + a + 1];  // scale L
 #pragma unroll
-          for (int x = 0; x < 4; ++x) O[x][i] *= HALF ? begun[x] * back : begun[x];
+          for (int c = 0; c < NV; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)  // a column's factor where O has it
+              O[x][c][i] *= HALF ? begun * __shfl(down[c], 4 * g + i, 64) : begun;
         }
       }
     }
     if (used) {  // S' = g^n S + K^T W V
+      const float passed = decay_power(lg, live);
 #pragma unroll
-      for (int f = 0; f < NK; ++f) S[f] *= passed;
+      for (int f = 0; f < NK; ++f)
+#pragma unroll
+        for (int c = 0; c < NV; ++c) S[f][c] *= passed;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        typedef T vec_t __attribute__((ext_vector_type(8)));
-        const vec_t t = __builtin_bit_cast(vec_t, V[x]);
-        float y[8];
+        u32x4_t w[NV][3];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = (float)t[e] * weight[2 * x + e / 4][e % 4];
-        u32x4_t w[3];
-        w[0] = decay_term<T>(y);
-        if constexpr (HALF) {
+        for (int c = 0; c < NV; ++c) {
+          typedef T vec_t __attribute__((ext_vector_type(8)));
+          const vec_t t = __builtin_bit_cast(vec_t, V[x][c]);
+          float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] *= 2048.f;
-          w[1] = decay_pack<T>(y);
-        } else {
-          w[1] = decay_term<T>(y);
-          w[2] = decay_pack<T>(y);
+          for (int e = 0; e < 8; ++e)  // weights count from the chunk's last token
+            y[e] = (float)t[e] * behind[C - live + 32 * x + 16 * (e / 4) + 4 * g + e % 4];
+          w[c][0] = decay_term<T>(y);
+          if constexpr (HALF) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] *= 2048.f;
+            w[c][1] = decay_pack<T>(y);
+          } else {
+            w[c][1] = TERMS == 3 ? decay_term<T>(y) : decay_pack<T>(y);
+            if constexpr (TERMS == 3) w[c][2] = decay_pack<T>(y);
+          }
         }
         constexpr int G = NK < 4 ? NK : 4;  // fragments at a time, so that none waits for its own sums
 #pragma unroll
         for (int f0 = 0; f0 < NK; f0 += G) {
           u32x4_t r[G];
 #pragma unroll
-          for (int f = 0; f < G; ++f) r[f] = columns(sK, Int<PK>{}, x, 4 * ((f0 + f) / 2) + (a & 3), (f0 + f) % 2);
+          for (int f = 0; f < G; ++f)
+            r[f] = transposed(at0 + at_k[(f0 + f) / 2] + 8 * ((f0 + f) % 2) + x * 32 * PK * 16, PK * 16);
 #pragma unroll
-          for (int f = 0; f < G; ++f) S[f0 + f] = mma_64b<T>(r[f], w[0], S[f0 + f]);
-          if constexpr (HALF) {
-            float4_t rest[G];
+          for (int c = 0; c < NV; ++c) {
 #pragma unroll
-            for (int f = 0; f < G; ++f) rest[f] = mma_64b<T>(r[f], w[1], float4_t{0.f, 0.f, 0.f, 0.f});
+            for (int f = 0; f < G; ++f) S[f0 + f][c] = mma_64b<T>(r[f], w[c][0], S[f0 + f][c]);
+            if constexpr (HALF) {
+              float4_t rest[G];
 #pragma unroll
-            for (int f = 0; f < G; ++f)
+              for (int f = 0; f < G; ++f) rest[f] = mma_64b<T>(r[f], w[c][1], float4_t{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-              for (int i = 0; i < 4; ++i) S[f0 + f][i] = __builtin_fmaf(rest[f][i], 1.f / 2048.f, S[f0 + f][i]);
-          } else {
+              for (int f = 0; f < G; ++f)
 #pragma unroll
-            for (int f = 0; f < G; ++f) S[f0 + f] = mma_64b<T>(r[f], w[1], S[f0 + f]);
+                for (int i = 0; i < 4; ++i) S[f0 + f][c][i] = __builtin_fmaf(rest[f][i], 1.f / 2048.f, S[f0 + f][c][i]);
+            } else {
 #pragma unroll
-            for (int f = 0; f < G; ++f) S[f0 + f] = mma_64b<T>(r[f], w[2], S[f0 + f]);
+              for (int f = 0; f < G; ++f) S[f0 + f][c] = mma_64b<T>(r[f], w[c][1], S[f0 + f][c]);
+              if constexpr (TERMS == 3) {
+#pragma unroll
+                for (int f = 0; f < G; ++f) S[f0 + f][c] = mma_64b<T>(r[f], w[c][2], S[f0 + f][c]);
+              }
+            }
           }
         }
       }
@@ -373,75 +445,101 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(DecayParams p) 
     if constexpr (!STATE) {
       if (used) {
         // a value that is not finite, times zero, is not a number in its row
-        float4_t odd = mma_64b<T>(V[0], u32x4_t{0, 0, 0, 0}, float4_t{0.f, 0.f, 0.f, 0.f});
-        odd = mma_64b<T>(V[1], u32x4_t{0, 0, 0, 0}, odd);
+        float4_t odd = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int c = 0; c < NV; ++c) odd = mma_64b<T>(V[x][c], u32x4_t{0, 0, 0, 0}, odd);
         const float any = (odd[0] + odd[1]) + (odd[2] + odd[3]);
         if (__builtin_expect(__any(any != any), 0)) {
           // its token's outputs and later ones: how many such values there are up to each token, by ones
           constexpr uint16_t one = HALF ? 0x3c00u : 0x3f80u;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float4_t count = float4_t{0.f, 0.f, 0.f, 0.f};
+          for (int c = 0; c < NV; ++c) {
 #pragma unroll
-            for (int y = 0; y <= x / 2; ++y) {
-              float w[8];
+            for (int x = 0; x < 4; ++x) {
+              float4_t count = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-              for (int e = 0; e < 8; ++e) w[e] = 32 * y + 16 * (e / 4) + 4 * g + e % 4 <= 16 * x + a ? 1.f : 0.f;
-              count = mma_64b<T>(decay_replace<T, false>(V[y], one), decay_pack<T>(w), count);
+              for (int y = 0; y <= x / 2; ++y) {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = 32 * y + 16 * (e / 4) + 4 * g + e % 4 <= 16 * x + a ? 1.f : 0.f;
+                count = mma_64b<T>(decay_replace<T, false>(V[y][c], one), decay_pack<T>(w), count);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (count[i] > 0.f) O[x][c][i] = __builtin_nanf("");
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (count[i] > 0.f) O[x][i] = __builtin_nanf("");
-          }
-#pragma unroll
-          for (int y = 0; y < 2; ++y) V[y] = decay_replace<T, true>(V[y], 0);
-        }
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the blocks are written
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (used) {  // (Q K^T . D) V
-        u32x4_t first[2], second[2];
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          first[y] = V[y];
-          if constexpr (HALF) {
-            typedef T vec_t __attribute__((ext_vector_type(8)));
-            const vec_t t = __builtin_bit_cast(vec_t, V[y]);
-            float s[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = (float)t[e];
-            first[y] = decay_term<__bf16>(s);
-            second[y] = decay_pack<__bf16>(s);
-          }
-        }
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          u32x4_t hi[4], lo[4];
-#pragma unroll
-          for (int x = 2 * y; x < 4; ++x) {
-            hi[x] = *reinterpret_cast<const u32x4_t*>(sP + ((x * 2 + y) * 64 + lane) * 16);
-            lo[x] = *reinterpret_cast<const u32x4_t*>(sP + kP + ((x * 2 + y) * 64 + lane) * 16);
-          }
-#pragma unroll
-          for (int x = 2 * y; x < 4; ++x) O[x] = mma_64b<__bf16>(first[y], hi[x], O[x]);
-#pragma unroll
-          for (int x = 2 * y; x < 4; ++x) O[x] = mma_64b<__bf16>(first[y], lo[x], O[x]);
-          if constexpr (HALF) {
-#pragma unroll
-            for (int x = 2 * y; x < 4; ++x) O[x] = mma_64b<__bf16>(second[y], hi[x], O[x]);
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int t = 16 * x + a, at = wave * 16 + 4 * g;
-          if (t < live && at < width) {
-            const float o[4] = {O[x][0], O[x][1], O[x][2], O[x][3]};
-            *reinterpret_cast<u32x2_t*>(out + (int64_t)(t0 + t) * p.o_l + at) = decay_pack<T>(o);
+            for (int y = 0; y < 2; ++y) V[y][c] = decay_replace<T, true>(V[y][c], 0);
           }
         }
       }
     }
+    if (STAGES == 1 || !STATE) meet();  // the blocks are written, and K, V and Q have been read
+    if (STAGES == 1 && t0 + C < left) copy(t0 + C, 0);
+    if constexpr (!STATE) {
+      if (used) {  // (Q K^T . D) V
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          u32x4_t first[NV], second[NV], hi[4], lo[4];
+#pragma unroll
+          for (int c = 0; c < NV; ++c) {
+            first[c] = V[y][c];
+            if constexpr (HALF) {
+              typedef T vec_t __attribute__((ext_vector_type(8)));
+              const vec_t t = __builtin_bit_cast(vec_t, V[y][c]);
+              float s[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) s[e] = (float)t[e];
+              first[c] = decay_term<__bf16>(s);
+              second[c] = decay_pack<__bf16>(s);
+            }
+          }
+#pragma unroll
+          for (int x = 2 * y; x < 4; ++x) {
+            hi[x] = *reinterpret_cast<const u32x4_t*>(sP + (decay_operand(x, y) * 64 + lane) * 16);
+            lo[x] = *reinterpret_cast<const u32x4_t*>(sP + kP + (decay_operand(x, y) * 64 + lane) * 16);
+          }
+#pragma unroll
+          for (int x = 2 * y; x < 4; ++x)
+#pragma unroll
+            for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<__bf16>(first[c], hi[x], O[x][c]);
+#pragma unroll
+          for (int x = 2 * y; x < 4; ++x)
+#pragma unroll
+            for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<__bf16>(first[c], lo[x], O[x][c]);
+          if constexpr (HALF) {
+#pragma unroll
+            for (int x = 2 * y; x < 4; ++x)
+#pragma unroll
+              for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<__bf16>(second[c], hi[x], O[x][c]);
+          }
+        }
+      }
+      if (used) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int t = 16 * x + a;
+          if (t >= live) continue;
+          T* const row = out + (int64_t)(t0 + t) * p.o_l + wave * 16 * NV + 4 * g;
+#pragma unroll
+          for (int c = 0; c < NV; ++c) {
+            if (wave * 16 * NV + 16 * c + 4 * g >= width) continue;
+            const float o[4] = {O[x][c][0], O[x][c][1], O[x][c][2], O[x][c][3]};
+            *reinterpret_cast<u32x2_t*>(row + 16 * c) = decay_pack<T>(o);
+          }
+        }
+      }
+    }
+    t0 += C;
+    stage ^= STAGES - 1;
+  };
+  if constexpr (HALF) {
+    while (t0 < left) chunk(Int<2>{});
+  } else {
+    while (t0 < late) chunk(Int<2>{});
+    while (t0 < left) chunk(Int<3>{});
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup's use of LDS
   if constexpr (!STATE) {
@@ -454,11 +552,15 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(DecayParams p) 
               : p.state_out && seg == (n > 0 ? (n - 1) / p.seg_len : 0) ? p.state_out + b * p.so_b + h * p.so_h
                                                                        : nullptr;
   if (!to) return;
+  int dk = p.dk;
+  asm("" : "+s"(dk));  // the comparisons are made again, not kept from the state's loading on
 #pragma unroll
   for (int f = 0; f < NK; ++f)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (has_state(f, i)) to[state_at(f, i)] = S[f][i];
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (has_state(f, c, i, dk)) to[state_at(f, c, i)] = S[f][c][i];
 }
 
 }  // namespace sengine

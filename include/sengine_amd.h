@@ -598,7 +598,7 @@ int sengine_amd_rotary(const sengine_rotary_desc* d, const void* q, const void* 
  * memory with the inputs otherwise.  K < 2^30 - 16, N <= 2^31 - 256.
  * With scratch memory (16-byte aligned, of at least sengine_amd_linear_e2m1_workspace's bytes; what it holds before
  * does not matter) many token rows are multiplied with the weight widened to 16 bits there; without it, or with less,
- * every 64 token rows read the codes again.
+ * every 64 token rows read the codes again, as they do of few weight rows in any case.
  */
 typedef struct sengine_linear_e2m1_desc {
   int64_t M;

@@ -44,76 +44,93 @@ __device__ __forceinline__ void across_groups(u32x4_t& v) {
   v = u32x4_t{c[0], c[1], d[0], d[1]};
 }
 
-// Few token rows: the time is that of reading the codes once.  Workgroup = 16 weight rows and up to 16 MT token rows;
-// its W waves share the reduction, wave w taking the segments of 128 values w, w + W, ..  A segment of a row is 64
-// bytes, 16 a lane and as they lie in memory; four lane swaps later lane group g has the eight values 32 m + 8 g ..
-// that it holds in matrix instruction m, whose 32 values belong to one group: its sums are multiplied by the group's
-// scale in fp32 (G instructions share a scale).
-template <class T, int MT, int G, int W, int U>
-__global__ __launch_bounds__(64 * W) void linear_e2m1_kernel(E2m1Params p) {
+// Few token rows: the time is that of reading the codes once.  Workgroup = 16 NT weight rows and up to 16 MT token rows; its
+// W waves share the reduction, each a range of its segments of 128 values.  A segment of a row is 64 bytes, 16 a lane and as
+// they lie in memory; four lane swaps later lane group g has the eight values 32 m + 8 g .. that it holds in matrix
+// instruction m, whose 32 values belong to one group: its sums are multiplied by the group's scale in fp32 (G instructions
+// share a scale).  x comes from the caches for every workgroup anew: with NT = 2 half as often.
+//
+// Measured, bf16 and groups of 32, us a call among others: 8 x 8192 x 8192 14.7 (36 MB of codes and scales: 2.4 TB/s; NT = 1
+// 18.5), 1 x 13.8, 32 x 23.6 (37), 64 x 39 (67); 1 x 4096 x 4096 10.0 (NT = 2 9.9: the host's time), 64 x 1024 x 4096 18.6
+// (21).  8 x 8192 x 8192 with waves that take segments in turn, not ranges: 20.
+template <class T, int MT, int NT, int G, int W, int U, int XB>
+__global__ __launch_bounds__(64 * W, NT == 2 ? 2 : 3) void linear_e2m1_kernel(E2m1Params p) {
   constexpr int NG = 4 / G;  // scales of a segment
-  __shared__ float4_t part[W][MT][64];
+  __shared__ float4_t part[W][MT * NT][64];
   const LinearParams& q = p.lin;
   const int lane = (int)threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15;
-  const int ntn = (q.N + 15) / 16;
-  const int n0 = (int)(blockIdx.x % ntn) * 16;
+  const int ntn = (q.N + 16 * NT - 1) / (16 * NT);
+  const int n0 = (int)(blockIdx.x % ntn) * (16 * NT);
   const int64_t m0 = (int64_t)(blockIdx.x / ntn) * (16 * MT);
   // rows past the end repeat the last one; what they give is not stored
-  const int wr = n0 + r < q.N ? n0 + r : q.N - 1;
-  const uint8_t* wp = q.w + (int64_t)wr * q.w_stride + g * 16;
-  const uint8_t* sp = p.scale + (int64_t)wr * p.scale_stride;
-  const uint8_t* xp[MT];
-  float4_t acc[MT];
+  const uint8_t *wp[NT], *sp[NT], *xp[MT];
+  float4_t acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int wr = n0 + 16 * i + r < q.N ? n0 + 16 * i + r : q.N - 1;
+    wp[i] = q.w + (int64_t)wr * q.w_stride + g * 16;
+    sp[i] = p.scale + (int64_t)wr * p.scale_stride;
+  }
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int64_t m = m0 + 16 * t + r < q.M ? m0 + 16 * t + r : q.M - 1;
     xp[t] = q.x + m * q.x_stride + g * 16;
-    acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[t][i] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
-  struct Batch {
-    u32x4_t w[U], x[U][MT][4];
-    uint32_t s[U];
-  };
-  const int full = q.K / 128;
+  // This wave's whole segments: neighbouring ones, so that a row's lines are its own.
+  const int full = q.K / 128, per = (full + W - 1) / W;
+  const int first = wave * per < full ? wave * per : full;
+  const int mine = full - first < per ? full - first : per;
   const auto load16 = [](const uint8_t* a) {
     u32x4_t v;
     __builtin_memcpy(&v, a, 16);
     return v;
   };
-  const auto load = [&](Batch& b, int s) {  // the whole segments among s, s + W, ..
+  struct Batch {  // U segments: their codes and scales
+    u32x4_t w[NT][U];
+    uint32_t s[NT][U * NG / 4 > 0 ? U * NG / 4 : 1];
+  };
+  static_assert(U * NG % 4 == 0, "whole words of scales");
+  const auto load = [&](Batch& b, int j) {  // segments j .. of the wave's
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t k = s + u * W;
-      if (k >= full) break;
-      b.w[u] = load16(wp + k * 64);
-      if constexpr (NG == 4) {
-        __builtin_memcpy(&b.s[u], sp + k * 4, 4);
-      } else if constexpr (NG == 2) {
-        uint16_t two;
-        __builtin_memcpy(&two, sp + k * 2, 2);
-        b.s[u] = two;
+    for (int i = 0; i < NT; ++i) {
+      const int64_t k = first + j;
+      if (j + U <= mine) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) b.w[i][u] = load16(wp[i] + (k + u) * 64);
+        __builtin_memcpy(b.s[i], sp[i] + k * NG, U * NG);
       } else {
-        b.s[u] = sp[k];
+        uint8_t* const s = reinterpret_cast<uint8_t*>(b.s[i]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (j + u >= mine) break;
+          b.w[i][u] = load16(wp[i] + (k + u) * 64);
+          __builtin_memcpy(s + u * NG, sp[i] + (k + u) * NG, NG);
+        }
       }
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int m = 0; m < 4; ++m) b.x[u][t][m] = load16(xp[t] + k * 256 + m * 64);
     }
   };
-  const auto multiply = [&](u32x4_t w, uint32_t scales, const u32x4_t (&x)[MT][4]) {
+  const auto load_x = [&](u32x4_t (&v)[MT][4], int64_t k) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int m = 0; m < 4; ++m) v[t][m] = load16(xp[t] + k * 256 + m * 64);
+  };
+  const auto multiply = [&](int i, u32x4_t w, uint32_t scales, int at, const u32x4_t (&x)[MT][4]) {
     across_groups(w);
+    scales >>= 8 * at;
     const float s[4] = {__builtin_amdgcn_cvt_f32_fp8(scales, 0), __builtin_amdgcn_cvt_f32_fp8(scales, 1),
                         __builtin_amdgcn_cvt_f32_fp8(scales, 2), __builtin_amdgcn_cvt_f32_fp8(scales, 3)};
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
+    for (int n = 0; n < NG; ++n) {
       float4_t sum[MT];
 #pragma unroll
       for (int t = 0; t < MT; ++t) sum[t] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int m = i * G; m < (i + 1) * G; ++m) {
+      for (int m = n * G; m < (n + 1) * G; ++m) {
         const u32x4_t b = widen_e2m1<T>(w[m]);
 #pragma unroll
         for (int t = 0; t < MT; ++t) sum[t] = mma_64b<T>(x[t][m], b, sum[t]);
@@ -121,43 +138,57 @@ __global__ __launch_bounds__(64 * W) void linear_e2m1_kernel(E2m1Params p) {
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = __builtin_fmaf(sum[t][e], s[i], acc[t][e]);
+        for (int e = 0; e < 4; ++e) acc[t][i][e] = __builtin_fmaf(sum[t][e], s[n], acc[t][i][e]);
     }
   };
-  const auto use = [&](const Batch& b, int s) {
+  // Codes and scales are on their way U to 2 U segments ahead of their use, x, which the caches hold, up to one.
+  u32x4_t x[XB][MT][4];
+  const auto use = [&](const Batch& b, int j) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s + u * W < full) multiply(b.w[u], b.s[u], b.x[u]);
+    for (int u = 0; u < U; ++u) {
+      if (j + u >= mine) break;
+      const int64_t k = first + j + u;
+      if (XB == 1)
+        load_x(x[0], k);
+      else if (j + u + 1 < mine)
+        load_x(x[(u + 1) % XB], k + 1);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) multiply(i, b.w[i][u], b.s[i][u * NG / 4], u * NG % 4, x[u % XB]);
+    }
   };
-  if (wave < full) {
+  if (mine > 0) {
     Batch b0, b1;
-    load(b0, wave);
-    for (int s = wave; s < full; s += 2 * U * W) {
-      load(b1, s + U * W);
-      use(b0, s);
-      load(b0, s + 2 * U * W);
-      use(b1, s + U * W);
+    load(b0, 0);
+    if (XB == 2) load_x(x[0], first);
+    for (int j = 0; j < mine; j += 2 * U) {
+      load(b1, j + U);
+      use(b0, j);
+      load(b0, j + 2 * U);
+      use(b1, j + U);
     }
   }
-  if (q.K % 128 != 0 && wave == full % W) {  // the reduction's tail: zeros past its end
-    const u32x4_t w = fetch_piece(wp, full * 64, q.K / 2 - g * 16);
-    uint32_t scales = 0;
-    for (int i = 0; i < NG && full * NG + i < p.groups; ++i) scales |= (uint32_t)sp[full * NG + i] << (8 * i);
-    u32x4_t x[MT][4];
+  if (q.K % 128 != 0 && wave == W - 1) {  // the reduction's tail: zeros past its end
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int m = 0; m < 4; ++m) x[t][m] = fetch_piece(xp[t], full * 256 + m * 64, q.kbytes - g * 16);
-    multiply(w, scales, x);
+      for (int m = 0; m < 4; ++m) x[0][t][m] = fetch_piece(xp[t], full * 256 + m * 64, q.kbytes - g * 16);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      uint32_t scales = 0;
+      for (int n = 0; n < NG && full * NG + n < p.groups; ++n) scales |= (uint32_t)sp[i][full * NG + n] << (8 * n);
+      multiply(i, fetch_piece(wp[i], full * 64, q.K / 2 - g * 16), scales, 0, x[0]);
+    }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) part[wave][t * NT + i][lane] = acc[t][i];
   __syncthreads();
-  // Wave t finishes token rows 16 t ..: a lane one of them, columns 4 (lane % 4) ..  The sums lie as the matrix
+  // A wave finishes 16 token rows of 16 columns: a lane one of them, columns 4 (lane % 4) ..  The sums lie as the matrix
   // instruction leaves them: value e of lane l is token 4 (l / 16) + e, column l % 16.
-  if (wave >= MT) return;
-  const int row = lane >> 2, col = n0 + 4 * (lane & 3);
-  const int64_t m = m0 + 16 * wave + row;
+  if (wave >= MT * NT) return;
+  const int row = lane >> 2, col = n0 + 16 * (wave % NT) + 4 * (lane & 3);
+  const int64_t m = m0 + 16 * (wave / NT) + row;
   by_output(q, [&](auto o, auto vec) {
     using O = decltype(o);
     constexpr bool VEC = decltype(vec)::value;
@@ -176,7 +207,7 @@ __global__ __launch_bounds__(64 * W) void linear_e2m1_kernel(E2m1Params p) {
   });
 }
 
-// s * c as 16-bit values, eight a thread, rows of `width` of them (K rounded up to 8, zeros behind K).
+// s * c as 16-bit values (4096 x 8192 in 19 us, 4.2 TB/s), eight a thread, rows of `width` of them (K rounded up to 8, zeros behind K).
 template <class T>
 __global__ __launch_bounds__(256) void widen_e2m1_kernel(E2m1Params p, T* out, int width, int shift) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -199,7 +230,11 @@ __global__ __launch_bounds__(256) void widen_e2m1_kernel(E2m1Params p, T* out, i
   *reinterpret_cast<vec_t*>(out + n * width + k) = v;
 }
 
-constexpr int64_t kE2m1Rows = 64;  // most token rows of the kernel above where there is scratch memory
+// Whether a call with scratch memory widens the weight there and multiplies it as a 16-bit one: where the kernel above would
+// take more than a round of 32 columns and 64 token rows a CU.  Measured (bf16, us; widened and not): 128 x 8192 x 8192 64 and
+// 76, 256 x 4096 x 4096 32 and 41, 4000 x 384 x 384 14 and 18; 128 x 4096 x 4096 30 and 22, 1000 x 384 x 384 14 and 10; 70 x
+// 8192 x 8192 62 and 59.
+static bool widens(int64_t M, int64_t N) { return M > 64 && (N + 31) / 32 * ((M + 63) / 64) > 256; }
 
 static LinearParams widened(const E2m1Params& p, const void* weight) {
   LinearParams q = p.lin;
@@ -209,24 +244,32 @@ static LinearParams widened(const E2m1Params& p, const void* weight) {
 }
 static size_t widened_bytes(const LinearParams& p) { return (((size_t)p.K + 7) / 8 * 16 * p.N + 255) / 256 * 256; }
 
-template <class T, int MT, int G, int W, int U>
+template <class T, int MT, int NT, int G, int W, int U, int XB>
 static hipError_t run_rows(const E2m1Params& p, hipStream_t stream) {
-  const int64_t wgs = ((int64_t)p.lin.N + 15) / 16 * ((p.lin.M + 16 * MT - 1) / (16 * MT));
+  const int64_t wgs = ((int64_t)p.lin.N + 16 * NT - 1) / (16 * NT) * ((p.lin.M + 16 * MT - 1) / (16 * MT));
   if (!launchable(wgs, 64 * W)) return hipErrorInvalidConfiguration;
-  linear_e2m1_kernel<T, MT, G, W, U><<<dim3((unsigned)wgs), dim3(64 * W), 0, stream>>>(p);
+  linear_e2m1_kernel<T, MT, NT, G, W, U, XB><<<dim3((unsigned)wgs), dim3(64 * W), 0, stream>>>(p);
   return hipGetLastError();
+}
+
+template <class T, int MT, int G>
+static hipError_t by_columns(const E2m1Params& p, hipStream_t stream) {
+  // 32 weight rows a workgroup where that leaves one for every CU
+  const int64_t wide = ((int64_t)p.lin.N + 31) / 32 * ((p.lin.M + 16 * MT - 1) / (16 * MT));
+  if (wide >= 256) return run_rows<T, MT, 2, G, 8, 4, MT == 1 ? 2 : 1>(p, stream);
+  return run_rows<T, MT, 1, G, 8, 4, MT == 1 ? 2 : 1>(p, stream);
 }
 
 template <class T, int G>
 static hipError_t by_rows(const E2m1Params& p, hipStream_t stream) {
-  if (p.lin.M <= 16) return run_rows<T, 1, G, 8, 4>(p, stream);
-  if (p.lin.M <= 32) return run_rows<T, 2, G, 8, 2>(p, stream);
-  return run_rows<T, 4, G, 8, 1>(p, stream);
+  if (p.lin.M <= 16) return by_columns<T, 1, G>(p, stream);
+  if (p.lin.M <= 32) return by_columns<T, 2, G>(p, stream);
+  return by_columns<T, 4, G>(p, stream);
 }
 
 template <class T>
 static hipError_t run(const E2m1Params& p, int group, uint8_t* workspace, size_t bytes, hipStream_t stream) {
-  if (p.lin.M > kE2m1Rows && p.lin.K > 0 && workspace && bytes >= widened_bytes(p.lin)) {
+  if (widens(p.lin.M, p.lin.N) && p.lin.K > 0 && workspace && bytes >= widened_bytes(p.lin)) {
     const int width = (p.lin.K + 7) / 8 * 8;
     const int64_t wgs = ((int64_t)p.lin.N * (width / 8) + 255) / 256;
     if (!launchable(wgs, 256)) return hipErrorInvalidConfiguration;
@@ -316,7 +359,7 @@ extern "C" int sengine_amd_linear_e2m1(const sengine_linear_e2m1_desc* d, const 
 extern "C" int sengine_amd_linear_e2m1_workspace(const sengine_linear_e2m1_desc* d, size_t* bytes) {
   if (!d || !bytes) return set_error(-1, "linear_e2m1_workspace: null argument");
   *bytes = 0;
-  if (d->M <= kE2m1Rows || d->N < 1 || d->K < 1 || !sizes_fit(d)) return 0;  // no need, or refused by the entry
+  if (d->N < 1 || d->K < 1 || !sizes_fit(d) || !widens(d->M, d->N)) return 0;  // no need, or refused by the entry
   E2m1Params p{};
   p.lin.M = d->M;
   p.lin.N = d->N;

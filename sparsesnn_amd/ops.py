@@ -1383,9 +1383,8 @@ def linear_e2m1(x: torch.Tensor, weight: torch.Tensor, group_scale: torch.Tensor
     float8_e4m3fn with groups of 32, 64 or 128 values, row_scale (N,) fp32, 1 where None; token_reader.e2m1_groups makes
     the three of a weight.  Nothing of the weight is rounded: a code times a group's scale is a 16-bit value; sums and
     what follows them are fp32, and the result is rounded once to out_dtype (x's type by default; fp16, bf16 or fp32).
-    activation, bias, residual and out as linear's.  Up to 64 token rows read the codes as they are, in the time that
-    their bytes take; more rows are multiplied with the weight widened to 16 bits in scratch memory of torch's
-    allocator."""
+    activation, bias, residual and out as linear's.  Up to 64 token rows, and more of narrow weights, read the codes as
+    they are; beyond, they are multiplied with the weight widened to 16 bits in scratch memory of torch's allocator."""
     if _dispatch_modes() or forward_ad._current_level >= 0:
         _token_modes(x, weight, group_scale, row_scale, bias, residual)
     key = None

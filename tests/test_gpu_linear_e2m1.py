@@ -28,7 +28,7 @@ def _case(g, M, N, K, group, dtype):
 SIZES = [(1, 1, 2, 32), (1, 16, 32, 32), (2, 3, 30, 32), (4, 1536, 384, 32), (3, 40, 96, 64), (5, 17, 130, 32),
          (7, 33, 128, 128), (16, 100, 1554, 64), (17, 64, 256, 128), (29, 1000, 1554, 64), (33, 130, 4096, 32),
          (48, 24, 200, 64), (64, 257, 640, 128), (65, 40, 100, 32), (100, 200, 512, 64), (300, 130, 1030, 128),
-         (700, 520, 2048, 32), (2100, 1100, 384, 64), (1, 1000, 8192, 32), (16, 50, 0, 32), (80, 50, 0, 64)]
+         (700, 520, 2048, 32), (2100, 1100, 384, 64), (1030, 600, 1030, 32), (65, 8200, 96, 128), (9000, 40, 100, 32), (1, 1000, 8192, 32), (16, 50, 0, 32), (80, 50, 0, 64)]
 
 
 @pytest.mark.parametrize("M,N,K,group", SIZES)
@@ -114,7 +114,7 @@ def test_not_numbers(dev, M):
     assert y[1:, keep].isfinite().all()
 
 
-@pytest.mark.parametrize("M,K", [(65, 130), (200, 256)])
+@pytest.mark.parametrize("M,K", [(8200, 130), (16000, 256)])
 def test_many_rows_without_scratch_memory(dev, M, K):
     """The C entry without a workspace, or with one that is too small, reads the codes for every 64 rows."""
     g = _gen(dev, M)

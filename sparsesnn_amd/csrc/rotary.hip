@@ -5,7 +5,10 @@
 // reduced to half a turn either way in 64 bits (a position of 10^6 at a radian a step has lost 16 bits of its turn in
 // 32), its sine and cosine and the products are fp32, and a result is rounded once.
 //
-// Bandwidth bound: queries and keys are read and written once, in one launch.  A workgroup takes a few tokens: their
+// Bandwidth bound: queries and keys are read and written once, in one launch.  32768 tokens x 40 heads x 128 bf16, neighbouring
+// pairs: 118 us (5.7 TB/s; two items a thread in flight 123), pairs P apart 126 (one item 129).  8 x 12544 tokens x 16 heads x
+// 48 fp16, pairs P apart: 64 us (4.8 TB/s; two half lines an access), neighbouring 53; workgroups of twice the tokens 69, of
+// four times 76.  A single token: 3.2 us.  A workgroup takes a few tokens: their
 // sines and cosines, which all heads share, go to LDS; then its threads go through the tokens' pieces of VEC values in
 // the order in which they lie in memory.
 #include "token_types.h"
@@ -70,7 +73,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p) {
   }
   __syncthreads();
 
-  constexpr int U = 2;  // items of a thread in flight
+  constexpr int U = NEAR ? 1 : 2;  // items of a thread in flight
   const int items = ntok * p.per_token;
   for (int i0 = tid; i0 < items; i0 += 256 * U) {
     float a[U][VEC], b[U][VEC];
@@ -126,8 +129,8 @@ static hipError_t run(RotaryParams p, int d, bool copies, hipStream_t stream) {
   if (per_token > kRotItems) return hipErrorInvalidValue;     // not reached: the entry's limits
   if (per_token == 0) return hipSuccess;
   p.per_token = (int)per_token;
-  // Four items a thread, as long as that leaves 512 workgroups.
-  int64_t n = (1024 + per_token - 1) / per_token;
+  // Up to four items a thread, as long as that leaves 512 workgroups.
+  int64_t n = 1024 / per_token;
   if (n > p.tokens / 512) n = p.tokens / 512;
   if (n > kRotAngles / p.pairs) n = kRotAngles / p.pairs;
   if (n > kRotTokens) n = kRotTokens;

@@ -1311,9 +1311,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         plan = _rotary_plan(key, q, k, positions, frequencies, sections, interleaved, out_q, out_k)
     desc, dev = plan
     if out_q is None:
-        out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out_q = torch.empty_like(q, memory_format=torch.contiguous_format)
     if out_k is None and k is not None:
-        out_k = torch.empty(k.shape, dtype=k.dtype, device=dev)
+        out_k = torch.empty_like(k, memory_format=torch.contiguous_format)
     check(_lib.load().sengine_amd_rotary(desc, q.data_ptr(), _ptr(k), positions.data_ptr(), frequencies.data_ptr(),
                                          out_q.data_ptr(), _ptr(out_k), _stream(dev)), "rotary")
     return out_q, out_k
@@ -1396,12 +1396,14 @@ def linear_e2m1(x: torch.Tensor, weight: torch.Tensor, group_scale: torch.Tensor
         except AttributeError:
             pass  # not a tensor: the checks say so
     plan = _TOKEN_PLANS.get(key)
-    if plan is None or (torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, group_scale, row_scale, bias, residual))):
+    if plan is None or (torch.is_grad_enabled() and (
+            x.requires_grad or group_scale.requires_grad
+            or (row_scale is not None and row_scale.requires_grad) or (bias is not None and bias.requires_grad)
+            or (residual is not None and residual.requires_grad))):
         plan = _linear_e2m1_plan(key, x, weight, group_scale, row_scale, bias, activation, residual, out_dtype, out)
     desc, size, shape, out_dtype, dev = plan
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=dev)
+        out = x.new_empty(shape) if out_dtype is x.dtype else torch.empty(shape, dtype=out_dtype, device=dev)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     check(_lib.load().sengine_amd_linear_e2m1_ws(
         desc, x.data_ptr(), weight.data_ptr(), group_scale.data_ptr(), _ptr(row_scale), _ptr(bias), _ptr(residual),
@@ -1410,7 +1412,7 @@ def linear_e2m1(x: torch.Tensor, weight: torch.Tensor, group_scale: torch.Tensor
 
 
 def _decay_plan(key, q, k, v, decay, state, lengths, scale, out, state_out):
-    """(descriptor, bytes of scratch memory, output's and state's shapes, device) of a checked call."""
+    """(descriptor, bytes of scratch memory, states' shape, device) of a checked call."""
     _token_input(q, "q")
     dev, code = q.device, _type_code(q, (torch.float16, torch.bfloat16), "q")
     for t, name in ((k, "k"), (v, "v")):
@@ -1428,7 +1430,7 @@ def _decay_plan(key, q, k, v, decay, state, lengths, scale, out, state_out):
         _token_vector(lengths, B, "lengths", dev)
         if lengths.dtype != torch.int32:
             raise SEngineError(f"lengths: expected dtype torch.int32, got {lengths.dtype}")
-    shape, matrices = (B, L, H, dv), (B, H, dk, dv)
+    matrices = (B, H, dk, dv)
     strides = []
     for t, x, name in ((q, q, "q"), (k, k, "k"), (v, v, "v"), (out, v, "out")):
         if name == "out":
@@ -1456,7 +1458,7 @@ def _decay_plan(key, q, k, v, decay, state, lengths, scale, out, state_out):
     desc = ctypes.byref(DecayDesc(*strides, B, L, H, dk, dv, code, 1.0 / math.sqrt(dk) if scale is None else scale))
     size = ctypes.c_size_t()
     check(_lib.load().sengine_amd_decay_attention_workspace(desc, ctypes.byref(size)), "decay_attention")
-    return _remember(key, (desc, size.value, shape, matrices, dev))
+    return _remember(key, (desc, size.value, matrices, dev))
 
 
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: torch.Tensor,
@@ -1488,14 +1490,16 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
         except AttributeError:
             pass  # not a tensor: the checks say so
     plan = _TOKEN_PLANS.get(key)
-    if plan is None or (torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (q, k, v, decay, state))):
+    if plan is None or (torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or v.requires_grad or decay.requires_grad
+            or (state is not None and state.requires_grad))):
         plan = _decay_plan(key, q, k, v, decay, state, lengths, scale, out, state_out)
-    desc, size, shape, matrices, dev = plan
+    desc, size, matrices, dev = plan
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
     if state_out is None:
-        state_out = torch.empty(matrices, dtype=torch.float32, device=dev)
+        state_out = (torch.empty(matrices, dtype=torch.float32, device=dev) if state is None
+                     else torch.empty_like(state, memory_format=torch.contiguous_format))
     pointers = qp, kp, vp, op, sp, tp = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(state) or 0,
                                          state_out.data_ptr())
     if (qp | kp | vp | op | sp | tp) & 15:

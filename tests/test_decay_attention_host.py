@@ -80,7 +80,7 @@ def test_checks_its_tensors():
     def plan(q=q, k=q, v=v, g=g, state=None, lengths=None, out=None, state_out=None):
         return ops._decay_plan(None, q, k, v, g, state, lengths, None, out, state_out)
 
-    assert plan(state=s, lengths=n, out=v, state_out=s)[1:4] == (0, (2, 5, 4, 48), (2, 4, 64, 48))
+    assert plan(state=s, lengths=n, out=v, state_out=s)[1:3] == (0, (2, 4, 64, 48))
     for kw, word in (
             (dict(q=_t(2, 5, 4, 64, dtype=F32)), "dtype"), (dict(k=_t(2, 5, 4, 64, dtype=torch.bfloat16)), "k:"),
             (dict(k=_t(2, 6, 4, 64)), "decay_attention"), (dict(v=_t(2, 5, 3, 48)), "decay_attention"),

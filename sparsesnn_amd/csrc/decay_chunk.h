@@ -192,6 +192,33 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
   const uint8_t* v = static_cast<const uint8_t*>(p.v) + (b * p.v_b + h * p.v_h + begin * p.v_l + slice * kDecayColumns) * 2;
   T* out = static_cast<T*>(p.out) + b * p.o_b + h * p.o_h + begin * p.o_l + slice * kDecayColumns;
 
+  // This wave's copies: c = wave, wave + NW, .. of a stage's PK of K, PV of V, PK of Q.  A lane's 16 bytes are place
+  // lane % P of a row; the piece that belongs there is fetched, or nothing where the row has none.
+  int voff[NCW];
+#pragma unroll
+  for (int i = 0; i < NCW; ++i) {
+    const int c = wave + i * NW, kind = c < PK ? 0 : c < PK + PV ? 1 : 2;
+    const int at = (c - (kind == 0 ? 0 : kind == 1 ? PK : PK + PV)) * 64 + lane;
+    const int r = kind == 1 ? at / PV : at / PK;
+    const int j = kind == 1 ? decay_place<PV>(r, at % PV) : decay_place<PK>(r, at % PK);
+    const int64_t stride = kind == 0 ? p.k_l : kind == 1 ? p.v_l : p.q_l;
+    voff[i] = j * 8 < (kind == 1 ? width : p.dk) ? r * (int)stride * 2 + j * 16 : 0x7fffff00;
+  }
+  const uint32_t lds0 = lds_offset(smem);
+  const auto copy = [&](int t0, int stage) {
+    const int live = left - t0 < C ? left - t0 : C;  // rows past them are out of the buffers' range
+    const u32x4_t kr = row_buffer(k + (int64_t)t0 * p.k_l * 2, ((live - 1) * (int)p.k_l + p.dk) * 2);
+    const u32x4_t vr = row_buffer(v + (int64_t)t0 * p.v_l * 2, ((live - 1) * (int)p.v_l + width) * 2);
+    const u32x4_t qr = STATE ? kr : row_buffer(q + (int64_t)t0 * p.q_l * 2, ((live - 1) * (int)p.q_l + p.dk) * 2);
+#pragma unroll
+    for (int i = 0; i < NCW; ++i) {
+      const int c = wave + i * NW;
+      if (NC % NW != 0 && c >= NC) break;
+      lds_copy(c < PK ? kr : c < PK + PV ? vr : qr, lds0 + stage * kStage + c * 1024, voff[i]);
+    }
+  };
+  if (left > 0) copy(0, 0);  // on their way beside the powers and the state
+
   // powers of the decay as the lanes need them
   const float lg = decay_log2(p.decay[h]);
   for (int i = tid; i < 2 * C; i += 64 * NW) {
@@ -225,31 +252,15 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
 #pragma unroll
       for (int i = 0; i < 4; ++i) S[f][c][i] = from && has_state(f, c, i, p.dk) ? from[state_at(f, c, i)] : 0.f;
 
-  // This wave's copies: c = wave, wave + NW, .. of a stage's PK of K, PV of V, PK of Q.  A lane's 16 bytes are place
-  // lane % P of a row; the piece that belongs there is fetched, or nothing where the row has none.
-  int voff[NCW];
-#pragma unroll
-  for (int i = 0; i < NCW; ++i) {
-    const int c = wave + i * NW, kind = c < PK ? 0 : c < PK + PV ? 1 : 2;
-    const int at = (c - (kind == 0 ? 0 : kind == 1 ? PK : PK + PV)) * 64 + lane;
-    const int r = kind == 1 ? at / PV : at / PK;
-    const int j = kind == 1 ? decay_place<PV>(r, at % PV) : decay_place<PK>(r, at % PK);
-    const int64_t stride = kind == 0 ? p.k_l : kind == 1 ? p.v_l : p.q_l;
-    voff[i] = j * 8 < (kind == 1 ? width : p.dk) ? r * (int)stride * 2 + j * 16 : 0x7fffff00;
+  // Tokens from here on count in the last state so much that what two terms of W V leave out would show; for outputs two
+  // are enough.
+  int late = 0;
+  if constexpr (!HALF) {
+    const float from_end = 10.f / -lg;  // tokens until less than 2^-10 is left
+    const float to = (float)(n - begin) - from_end;
+    late = !p.state_out ? left : to > 0.f ? (int)to / C * C : 0;
+    late = late < left ? late : left;
   }
-  const uint32_t lds0 = lds_offset(smem);
-  const auto copy = [&](int t0, int stage) {
-    const int live = left - t0 < C ? left - t0 : C;  // rows past them are out of the buffers' range
-    const u32x4_t kr = row_buffer(k + (int64_t)t0 * p.k_l * 2, ((live - 1) * (int)p.k_l + p.dk) * 2);
-    const u32x4_t vr = row_buffer(v + (int64_t)t0 * p.v_l * 2, ((live - 1) * (int)p.v_l + width) * 2);
-    const u32x4_t qr = STATE ? kr : row_buffer(q + (int64_t)t0 * p.q_l * 2, ((live - 1) * (int)p.q_l + p.dk) * 2);
-#pragma unroll
-    for (int i = 0; i < NCW; ++i) {
-      const int c = wave + i * NW;
-      if (NC % NW != 0 && c >= NC) break;
-      lds_copy(c < PK ? kr : c < PK + PV ? vr : qr, lds0 + stage * kStage + c * 1024, voff[i]);
-    }
-  };
   // Where in LDS a lane's share begins: of 16 rows, their values 32 m + 8 g ..; of 32 tokens transposed, the columns 32 m + 8 p
   // .. (p = a % 4) of K and 16 c .. of the wave's of V.  What else an address has is the same for all lanes.
   int at_rows[NM], at_k[NM], at_v[NV];
@@ -268,17 +279,7 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
     asm volatile("" ::: "memory");
   };
 
-  // Tokens from here on count in the last state so much that what two terms of W V leave out would show; for outputs two
-  // are enough.
-  int late = 0;
-  if constexpr (!HALF) {
-    const float from_end = 10.f / -lg;  // tokens until less than 2^-10 is left
-    const float to = (float)(n - begin) - from_end;
-    late = !p.state_out ? left : to > 0.f ? (int)to / C * C : 0;
-    late = late < left ? late : left;
-  }
   uint8_t* const sP = smem + STAGES * kStage;
-  if (left > 0) copy(0, 0);
   int t0 = 0, stage = 0;
   const auto chunk = [&](auto terms) {
     constexpr int TERMS = decltype(terms)::value;

@@ -546,8 +546,8 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
   if constexpr (!STATE) {
     // tokens behind the sequence's last one
     const int end = p.L - begin < p.seg_len ? p.L - begin : p.seg_len, pieces = width / 8;
-    for (int i = tid; i < (end - left) * pieces; i += 64 * NW)
-      *reinterpret_cast<u32x4_t*>(out + (int64_t)(left + i / pieces) * p.o_l + i % pieces * 8) = u32x4_t{0, 0, 0, 0};
+    for (int64_t i = tid; i < (int64_t)(end - left) * pieces; i += 64 * NW)
+      *reinterpret_cast<u32x4_t*>(out + (left + i / pieces) * p.o_l + i % pieces * 8) = u32x4_t{0, 0, 0, 0};
   }
   float* to = STATE ? p.parts + (bh * (p.segs - 1) + seg) * matrix
               : p.state_out && seg == (n > 0 ? (n - 1) / p.seg_len : 0) ? p.state_out + b * p.so_b + h * p.so_h

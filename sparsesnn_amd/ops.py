@@ -1218,6 +1218,18 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
     return out
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", lambda: 0)  # absent in CPU-only builds
+
+
+def _launch(entry, device: torch.device, what: str, *args):
+    """Calls an entry with its device as the current one: the default stream's handle is the same for every device."""
+    if device.index == _current_device():
+        check(entry(*args, _stream(device)), what)
+    else:
+        with torch.cuda.device(device):
+            check(entry(*args, _stream(device)), what)
+
+
 def _heads_out(t, shape, dtype, name: str, device):
     """An output (B, L, heads, d) given by the caller: any strides, the values of a head side by side."""
     if not isinstance(t, torch.Tensor):
@@ -1314,8 +1326,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         out_q = torch.empty_like(q, memory_format=torch.contiguous_format)
     if out_k is None and k is not None:
         out_k = torch.empty_like(k, memory_format=torch.contiguous_format)
-    check(_lib.load().sengine_amd_rotary(desc, q.data_ptr(), _ptr(k), positions.data_ptr(), frequencies.data_ptr(),
-                                         out_q.data_ptr(), _ptr(out_k), _stream(dev)), "rotary")
+    _launch(_lib.load().sengine_amd_rotary, dev, "rotary", desc, q.data_ptr(), _ptr(k), positions.data_ptr(),
+            frequencies.data_ptr(), out_q.data_ptr(), _ptr(out_k))
     return out_q, out_k
 
 
@@ -1405,9 +1417,8 @@ def linear_e2m1(x: torch.Tensor, weight: torch.Tensor, group_scale: torch.Tensor
     if out is None:
         out = x.new_empty(shape) if out_dtype is x.dtype else torch.empty(shape, dtype=out_dtype, device=dev)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    check(_lib.load().sengine_amd_linear_e2m1_ws(
-        desc, x.data_ptr(), weight.data_ptr(), group_scale.data_ptr(), _ptr(row_scale), _ptr(bias), _ptr(residual),
-        out.data_ptr(), _ptr(ws), size, _stream(dev)), "linear_e2m1")
+    _launch(_lib.load().sengine_amd_linear_e2m1_ws, dev, "linear_e2m1", desc, x.data_ptr(), weight.data_ptr(),
+            group_scale.data_ptr(), _ptr(row_scale), _ptr(bias), _ptr(residual), out.data_ptr(), _ptr(ws), size)
     return out
 
 
@@ -1507,7 +1518,6 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
             if x & 15 and t.numel():
                 raise SEngineError(f"{name}: must begin at a multiple of 16 bytes")
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    check(_lib.load().sengine_amd_decay_attention_ws(
-        desc, qp, kp, vp, decay.data_ptr(), sp or None, _ptr(lengths), op, tp, _ptr(ws), size, _stream(dev)),
-        "decay_attention")
+    _launch(_lib.load().sengine_amd_decay_attention_ws, dev, "decay_attention", desc, qp, kp, vp, decay.data_ptr(),
+            sp or None, _ptr(lengths), op, tp, _ptr(ws), size)
     return out, state_out

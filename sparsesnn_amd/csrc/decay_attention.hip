@@ -125,7 +125,8 @@ static hipError_t run_steps(const DecayParams& p, hipStream_t stream) {
 }
 
 // Prefix of the segments' states: place s holds what segment s adds to a state of zeros, and afterwards the state that
-// segment s + 1 begins with.  Thread = four values of a state.
+// segment s + 1 begins with.  Thread = four values of a state.  A state that is updated in place is copied: the segment
+// that ends a sequence may write it before the first one has read it.
 __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p, int per_state) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t bh = i / per_state;
@@ -136,6 +137,7 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p, int per_
   const int last = n > 0 ? (n - 1) / p.seg_len : 0;  // the last segment with tokens
   float run[4] = {0.f, 0.f, 0.f, 0.f};
   if (p.state) load_floats<float, 4>(p.state + b * p.s_b + h * p.s_h + at, run);
+  if (p.begun) store_floats(p.begun + bh * (int64_t)(p.dk * p.dv) + at, run);
   const float g = decay_power(decay_log2(p.decay[h]), p.seg_len);
   float* part = p.parts + bh * (p.segs - 1) * (int64_t)(p.dk * p.dv) + at;
   constexpr int U = 8;  // segments whose loads are under way together
@@ -186,7 +188,7 @@ static DecayPlan plan(const sengine_decay_desc* d) {
 }
 
 static size_t workspace_of(const sengine_decay_desc* d, const DecayPlan& q) {
-  return (size_t)d->B * d->H * (q.segs - 1) * d->dk * d->dv * 4;
+  return (size_t)d->B * d->H * q.segs * d->dk * d->dv * 4;  // the segments' states, and those that the sequences begin with
 }
 
 template <class T, int DKP, int BLOCKS>
@@ -289,6 +291,7 @@ extern "C" int sengine_amd_decay_attention_ws(const sengine_decay_desc* d, const
   if (plan_.segs > 1 && (!workspace || workspace_bytes < workspace_of(d, plan_)))
     plan_ = {false, 1, (int)(((int64_t)d->L + kDecayChunk - 1) / kDecayChunk * kDecayChunk)};
   p.parts = static_cast<float*>(workspace);
+  if (plan_.segs > 1 && state && state == state_out) p.begun = p.parts + (int64_t)d->B * d->H * (plan_.segs - 1) * matrix;
   return (int)(d->type == SENGINE_ENC_F16 ? run<_Float16>(p, plan_, stream) : run<__bf16>(p, plan_, stream));
 }
 

@@ -41,6 +41,7 @@ struct DecayParams {
   float* state_out;    // or null
   const int32_t* lengths;
   float* parts;        // (B, H, segs - 1) states
+  float* begun;        // (B, H) copies of a state that is updated in place, or null
   int B, L, H, dk, dv;
   int segs, seg_len;
   float scale;
@@ -243,6 +244,7 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
   const int64_t matrix = (int64_t)p.dk * p.dv;
   const float* from = STATE ? nullptr
                       : seg > 0 ? (left > 0 ? p.parts + (bh * (p.segs - 1) + seg - 1) * matrix : nullptr)
+                      : p.begun ? p.begun + bh * matrix
                       : p.state ? p.state + b * p.s_b + h * p.s_h
                                 : nullptr;
 #pragma unroll

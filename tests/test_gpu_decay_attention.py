@@ -48,6 +48,22 @@ def test_decay_attention(dev, B, L, H, dk, dv, dtype):
            ref.decay_attention(q, k, v, decay, state, None, 0.3))
 
 
+@pytest.mark.parametrize("B,L,H,dk,dv", [(1, 1500, 2, 64, 64), (3, 3000, 67, 128, 128), (4, 3000, 50, 64, 64)])
+def test_state_in_place_of_segments(dev, B, L, H, dk, dv):
+    """The last segment of a sequence writes the state that the first one reads, in any order: more of them than the chip
+    holds at once, sequences that end in their first segment, and an empty one."""
+    g = _gen(dev, L + H)
+    q, k, v, decay, state = _case(g, B, L, H, dk, dv, BF16)
+    lengths = torch.full((B,), L, dtype=torch.int32, device=dev)
+    if B > 1:
+        lengths[0], lengths[-1] = 40, 0
+    want = ops.decay_attention(q, k, v, decay, state=state, lengths=lengths)
+    for _ in range(3):
+        held = state.clone()
+        got = ops.decay_attention(q, k, v, decay, state=held, lengths=lengths, state_out=held)
+        assert torch.equal(got[0], want[0]) and torch.equal(held, want[1])
+
+
 @pytest.mark.parametrize("L", [1, 7, 100, 1000])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_lengths(dev, L, dtype):

@@ -167,9 +167,11 @@ struct DecayPlan {
 constexpr int kDecaySteps = 16;
 
 static DecayPlan plan(const sengine_decay_desc* d) {
-  // the chunks' copies have offsets of 31 bits from a chunk's first token on
-  const auto near = [](int64_t stride) { return stride >= 0 && stride < 1 << 23; };
-  if (d->L <= kDecaySteps || !near(d->q_stride[1]) || !near(d->k_stride[1]) || !near(d->v_stride[1]))
+  // The chunks' copies have offsets of 31 bits from a chunk's first token on.  A row past the last token must be out of
+  // the copies' range, or the last token's own: rows that overlap go one by one.
+  const auto copied = [](int64_t stride, int size) { return stride == 0 || (stride >= size && stride < 1 << 23); };
+  if (d->L <= kDecaySteps || !copied(d->q_stride[1], d->dk) || !copied(d->k_stride[1], d->dk) ||
+      !copied(d->v_stride[1], d->dv))
     return {true, 1, d->L};
   const int chunks = (int)(((int64_t)d->L + kDecayChunk - 1) / kDecayChunk);
   // Rounds of workgroups over the chip, times the chunks of one and a start, half as much again for the pass that makes the

@@ -64,6 +64,22 @@ def test_state_in_place_of_segments(dev, B, L, H, dk, dv):
         assert torch.equal(got[0], want[0]) and torch.equal(held, want[1])
 
 
+@pytest.mark.parametrize("step", [0, 8, 16, 24])
+def test_rows_that_overlap(dev, step):
+    """Tokens whose rows begin `step` values apart: a row past the last token would lie within the last ones, and what is
+    no number there belongs to other columns."""
+    g = _gen(dev, step)
+    L, d = 100, 24
+    q, k, v, decay, _ = _case(g, 1, L, 1, d, d, BF16)
+    spread = lambda t: torch.as_strided(t.flatten(), (1, L, 1, d), (0, step, 0, 1))
+    k, v = spread(k), spread(v)
+    _check(ops.decay_attention(q, k, v, decay), ref.decay_attention(q, k, v, decay))
+    for t in (k, v):
+        t[0, L - 1, 0, d - 1] = math.nan
+        got, want = ops.decay_attention(q, k, v, decay), ops.decay_attention(q, k.contiguous(), v.contiguous(), decay)
+        assert all(torch.equal(a.isnan(), b.isnan()) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("L", [1, 7, 100, 1000])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_lengths(dev, L, dtype):

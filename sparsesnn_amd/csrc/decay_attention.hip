@@ -208,7 +208,13 @@ static hipError_t run_chunks(const DecayParams& p, hipStream_t stream) {
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  decay_chunk_kernel<T, DKP, NV, NW, false><<<dim3((unsigned)(parts * p.segs)), dim3(64 * NW), 0, stream>>>(p);
+  // Where each has a CU to itself, workgroups of twice the waves.  Measured, us, waves of 16 and of 32 columns: 16 heads of
+  // 128 x 128 in bf16, 300 tokens 29 and 37, 1000 tokens 34 and 39; two workgroups a CU, 6 x 12 heads of 64 x 80 over 777
+  // tokens, 35.5 and 31.5.
+  if (NV > 1 && parts * p.segs <= 256)
+    decay_chunk_kernel<T, DKP, 1, BLOCKS, false><<<dim3((unsigned)(parts * p.segs)), dim3(64 * BLOCKS), 0, stream>>>(p);
+  else
+    decay_chunk_kernel<T, DKP, NV, NW, false><<<dim3((unsigned)(parts * p.segs)), dim3(64 * NW), 0, stream>>>(p);
   return hipGetLastError();
 }
 

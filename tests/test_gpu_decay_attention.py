@@ -64,6 +64,16 @@ def test_state_in_place_of_segments(dev, B, L, H, dk, dv):
         assert torch.equal(got[0], want[0]) and torch.equal(held, want[1])
 
 
+@pytest.mark.parametrize("B,L,H,dk,dv", [(8, 70, 36, 128, 128), (2, 300, 40, 64, 200), (5, 130, 70, 96, 96),
+                                         (4, 100, 70, 24, 72), (2, 2100, 24, 128, 128), (1, 1100, 40, 32, 88)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_many_workgroups(dev, B, L, H, dk, dv, dtype):
+    """More workgroups than the chip has CUs, where waves are wider."""
+    g = _gen(dev, B + 3 * L + dk + 7 * dv)
+    q, k, v, decay, state = _case(g, B, L, H, dk, dv, dtype)
+    _check(ops.decay_attention(q, k, v, decay, state=state), ref.decay_attention(q, k, v, decay, state))
+
+
 @pytest.mark.parametrize("step", [0, 8, 16, 24])
 def test_rows_that_overlap(dev, step):
     """Tokens whose rows begin `step` values apart: a row past the last token would lie within the last ones, and what is

@@ -4,7 +4,8 @@
 // alone and have outputs of zero.
 //
 // Two forms.  Few tokens: token by token, the state in registers (decay_step_kernel); its time is the state's reading and
-// writing.  Many: 64 tokens at a time as matrix products (decay_chunk.h).
+// writing: one token of 128 x 32 heads of 128 x 128, 541 MB, 102 us (5.3 TB/s).  Many: 64 tokens at a time as matrix products
+// (decay_chunk.h).
 #include "decay_chunk.h"
 
 namespace sengine {

@@ -52,7 +52,8 @@ __device__ __forceinline__ void across_groups(u32x4_t& v) {
 //
 // Measured, bf16 and groups of 32, us a call among others: 8 x 8192 x 8192 14.7 (36 MB of codes and scales: 2.4 TB/s; NT = 1
 // 18.5), 1 x 13.8, 32 x 23.6 (37), 64 x 39 (67); 1 x 4096 x 4096 10.0 (NT = 2 9.9: the host's time), 64 x 1024 x 4096 18.6
-// (21).  8 x 8192 x 8192 with waves that take segments in turn, not ranges: 20.
+// (21).  8 x 8192 x 8192 with waves that take segments in turn, not ranges: 20; the loads of codes and scales alone take 10,
+// with x 11, with the widening and the products of what they bring 15.
 template <class T, int MT, int NT, int G, int W, int U, int XB>
 __global__ __launch_bounds__(64 * W, NT == 2 ? 2 : 3) void linear_e2m1_kernel(E2m1Params p) {
   constexpr int NG = 4 / G;  // scales of a segment

@@ -158,6 +158,11 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p, int per_
   }
 }
 
+// Whether wide heads take waves of 16 columns, not of 32: where every workgroup has a CU to itself.  Measured, us, waves of 16
+// and of 32: 16 heads of 128 x 128 in bf16, 300 tokens 29 and 37, 1000 tokens 34 and 39; two workgroups a CU, 6 x 12 heads of
+// 64 x 80 over 777 tokens, 35.5 and 31.5.
+static bool decay_narrow(int dv, int64_t workgroups) { return decay_own(decay_blocks(dv)) > 1 && workgroups <= 256; }
+
 struct DecayPlan {
   bool steps;        // token by token
   int segs, seg_len;  // segments of a sequence that are computed beside each other, tokens of one
@@ -176,15 +181,19 @@ static DecayPlan plan(const sengine_decay_desc* d) {
     return {true, 1, d->L};
   const int chunks = (int)(((int64_t)d->L + kDecayChunk - 1) / kDecayChunk);
   // Rounds of workgroups over the chip, times the chunks of one and a start, half as much again for the pass that makes the
-  // segments' states; and two launches more and the states' joining, in the time of chunks.
+  // segments' states; and two launches more and the states' joining, in the time of chunks, of which narrow waves have
+  // two thirds.  Measured, us, without segments and in this many: 16 heads of 128 x 128, 150 tokens 21, 300 tokens 29 and
+  // 25 (5); 4000 tokens 47 (16), 51 (32), 79 (63); 8 x 16 heads of them over 500 tokens 46, 54 (4).
   const int64_t heads = (int64_t)d->B * d->H * ((d->dv + kDecayColumns - 1) / kDecayColumns);
   const int64_t slots = 256 * decay_resident(d->dk, d->dv);
+  const auto pass = [&](int64_t workgroups, int per) {
+    return (float)((workgroups + slots - 1) / slots) * (float)(per + 1) * (decay_narrow(d->dv, workgroups) ? 2.f / 3.f : 1.f);
+  };
   int best = chunks;  // chunks of a segment
-  float least = (float)((heads + slots - 1) / slots) * (float)(chunks + 1);
+  float least = pass(heads, chunks);
   for (int segs = 2; segs <= chunks && segs <= 256 && (segs - 1) * heads <= 2 * slots; ++segs) {
     const int per = (chunks + segs - 1) / segs;
-    const int64_t rounds = (heads * ((chunks + per - 1) / per) + slots - 1) / slots;
-    const float cost = 1.5f * (float)rounds * (float)(per + 1) + 3.f + (float)segs / 16.f;
+    const float cost = 1.5f * pass(heads * ((chunks + per - 1) / per), per) + 1.5f + (float)segs / 16.f;
     if (cost < least) least = cost, best = per;
   }
   return {false, (chunks + best - 1) / best, best * kDecayChunk};
@@ -209,10 +218,7 @@ static hipError_t run_chunks(const DecayParams& p, hipStream_t stream) {
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  // Where each has a CU to itself, workgroups of twice the waves.  Measured, us, waves of 16 and of 32 columns: 16 heads of
-  // 128 x 128 in bf16, 300 tokens 29 and 37, 1000 tokens 34 and 39; two workgroups a CU, 6 x 12 heads of 64 x 80 over 777
-  // tokens, 35.5 and 31.5.
-  if (NV > 1 && parts * p.segs <= 256)
+  if (NV > 1 && decay_narrow(p.dv, parts * p.segs))
     decay_chunk_kernel<T, DKP, 1, BLOCKS, false><<<dim3((unsigned)(parts * p.segs)), dim3(64 * BLOCKS), 0, stream>>>(p);
   else
     decay_chunk_kernel<T, DKP, NV, NW, false><<<dim3((unsigned)(parts * p.segs)), dim3(64 * NW), 0, stream>>>(p);

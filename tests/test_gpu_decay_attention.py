@@ -65,10 +65,11 @@ def test_state_in_place_of_segments(dev, B, L, H, dk, dv):
 
 
 @pytest.mark.parametrize("B,L,H,dk,dv", [(8, 70, 36, 128, 128), (2, 300, 40, 64, 200), (5, 130, 70, 96, 96),
-                                         (4, 100, 70, 24, 72), (2, 2100, 24, 128, 128), (1, 1100, 40, 32, 88)])
+                                         (4, 100, 70, 24, 72), (2, 2100, 24, 128, 128), (1, 1100, 40, 32, 88),
+                                         (6, 777, 12, 64, 80), (1, 1100, 56, 32, 88)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_many_workgroups(dev, B, L, H, dk, dv, dtype):
-    """More workgroups than the chip has CUs, where waves are wider."""
+    """About as many workgroups as the chip has CUs, and more, where waves are wider."""
     g = _gen(dev, B + 3 * L + dk + 7 * dv)
     q, k, v, decay, state = _case(g, B, L, H, dk, dv, dtype)
     _check(ops.decay_attention(q, k, v, decay, state=state), ref.decay_attention(q, k, v, decay, state))

@@ -623,6 +623,8 @@ int sengine_amd_linear_e2m1_ws(const sengine_linear_e2m1_desc* d, const void* x,
  * (null = zeros) and state_out (null = not wanted) are fp32 matrices (dk, dv), contiguous, with strides per
  * (batch, head) in elements, at multiples of 16 bytes; state_out receives the state behind a sequence's last token, the
  * state itself where it has none.  out is zero behind the last token.  The state, sums and powers of the decay are fp32.
+ * More than 16 tokens are products of 16-bit values: the state and what a token adds to it enter them with all of their 24
+ * bits in bf16 and with 22 in fp16 (an addition in steps of |k| 2^-36 at the finest), the weights within 64 tokens with 16.
  * A value that is not finite reaches the outputs from its own token on and the state.  state_out may be state itself;
  * otherwise outputs share no memory with inputs.
  * With scratch memory (16-byte aligned, of at least sengine_amd_decay_attention_workspace's bytes; what it holds before

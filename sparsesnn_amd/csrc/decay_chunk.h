@@ -21,12 +21,14 @@
 //   * K^T (W V) has its rows, dk, permuted so that a lane ends with eight neighbouring ones of a column: as they lie they
 //     are the operand of S^T Q^T.
 //
-// Rounding.  S is fp32.  What a 16-bit instruction takes of it and of the fp32 weights Q K^T . D is a sum of two 16-bit
-// values (of bf16, 16 bits; S of fp16, 22), so that O is as exact as its own rounding; W V, which makes S, is a sum of
-// two: in bf16 of three where the last state keeps more than 2^-10 of it, in fp16 with the second 2^11 times larger so that
-// it does not fall below the type's range.  Weights
-// easily pass fp16's range: they are bf16 values always, and fp16 values of V are sums of two of them, exactly.  A
-// column of S is scaled by a power of two to fp16's range.
+// Rounding.  S is fp32.  What a 16-bit instruction takes of it, and W V, which makes it, are in bf16 sums of three values,
+// which have all of its 24 bits whatever the age of a token: later keys may be small or zero, so that an early token is all
+// that a state holds, and outputs may be differences of its values.  (Two instead of three: 400 us for 431 at 65536 tokens of
+// 16 heads of 128 x 128, 76.8 for 79.7 at 8 x 1000; outputs 1.1e-4 for 5.5e-5 of the exact ones' size from those,
+// rounded.)  In fp16 they are sums of two: 22 bits, S with a column scaled by a power of two to fp16's range; of W V the
+// second one is 2^11 times larger, so that a token adds at most |k| 2^-36 on top, where the decay has taken it below the
+// type's range.  The fp32 weights Q K^T . D, which only their own chunk sees, are sums of two bf16 values, 16 bits, on both
+// types, as they easily pass fp16's range, and fp16 values of V are sums of two of them, exactly.
 //
 // A value of V that is not finite must not reach the tokens before it, and 0 times it would: a chunk that holds one
 // takes it out and marks the outputs that it belongs to instead.
@@ -168,6 +170,7 @@ template <class T, int DKP, int NV, int NW, bool STATE>
 __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void decay_chunk_kernel(DecayParams p) {
   constexpr bool HALF = __is_same(T, _Float16);
   constexpr int C = kDecayChunk, STAGES = STATE ? 2 : 1;
+  constexpr int TERMS = HALF ? 2 : 3;  // values of T that the state's products take for one of it
   constexpr int PK = DKP / 8, PV = NV * NW == 3 ? 8 : NV * NW * 2;  // pieces of a row of Q or K, of V
   constexpr int NM = DKP / 32, NK = DKP / 16;
   constexpr int NC = PK * (STATE ? 1 : 2) + PV, NCW = (NC + NW - 1) / NW;  // copies of 1 KB a chunk, of a wave
@@ -259,15 +262,6 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
 #pragma unroll
       for (int i = 0; i < 4; ++i) S[f][c][i] = from && has_state(f, c, i, p.dk) ? from[state_at(f, c, i)] : 0.f;
 
-  // Tokens from here on count in the last state so much that what two terms of W V leave out would show; for outputs two
-  // are enough.
-  int late = 0;
-  if constexpr (!HALF) {
-    const float from_end = 10.f / -lg;  // tokens until less than 2^-10 is left
-    const float to = (float)(n - begin) - from_end;
-    late = !p.state_out ? left : to > 0.f ? (int)to / C * C : 0;
-    late = late < left ? late : left;
-  }
   // Where in LDS a lane's share begins: of 16 rows, their values 32 m + 8 g ..; of 32 tokens transposed, the columns 32 m + 8 p
   // .. (p = a % 4) of K and 16 c .. of the wave's of V.  What else an address has is the same for all lanes.
   int at_rows[NM], at_k[NM], at_v[NV];
@@ -288,8 +282,7 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
 
   uint8_t* const sP = smem + STAGES * kStage;
   int t0 = 0, stage = 0;
-  const auto chunk = [&](auto terms) {
-    constexpr int TERMS = decltype(terms)::value;
+  while (t0 < left) {
     // this wave's copies have landed and its reads of the blocks are done; so are all waves'
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     meet();
@@ -360,26 +353,25 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
         }
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
-          u32x4_t hi[NV], lo[NV], r[4];
+          u32x4_t part[NV][TERMS], r[4];
 #pragma unroll
           for (int c = 0; c < NV; ++c) {
             float s[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] = HALF ? S[2 * m + e / 4][c][e % 4] * up[c] : S[2 * m + e / 4][c][e % 4];
-            hi[c] = decay_term<T>(s);
-            lo[c] = decay_pack<T>(s);
+#pragma unroll
+            for (int u = 0; u < TERMS - 1; ++u) part[c][u] = decay_term<T>(s);
+            part[c][TERMS - 1] = decay_pack<T>(s);
           }
 #pragma unroll
           for (int x = 0; x < 4; ++x)
             r[x] = *reinterpret_cast<const u32x4_t*>(smem + kQ + at_rows[m] + x * 16 * PK * 16);
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+          for (int u = 0; u < TERMS; ++u)
 #pragma unroll
-            for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<T>(hi[c], r[x], O[x][c]);
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<T>(lo[c], r[x], O[x][c]);
+              for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<T>(part[c][u], r[x], O[x][c]);
         }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -400,7 +392,7 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
         for (int c = 0; c < NV; ++c) S[f][c] *= passed;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        u32x4_t w[NV][3];
+        u32x4_t w[NV][TERMS];
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
           typedef T vec_t __attribute__((ext_vector_type(8)));
@@ -415,8 +407,8 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
             for (int e = 0; e < 8; ++e) y[e] *= 2048.f;
             w[c][1] = decay_pack<T>(y);
           } else {
-            w[c][1] = TERMS == 3 ? decay_term<T>(y) : decay_pack<T>(y);
-            if constexpr (TERMS == 3) w[c][2] = decay_pack<T>(y);
+            w[c][1] = decay_term<T>(y);
+            w[c][2] = decay_pack<T>(y);
           }
         }
         constexpr int G = NK < 4 ? NK : 4;  // fragments at a time, so that none waits for its own sums
@@ -440,11 +432,9 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
                 for (int i = 0; i < 4; ++i) S[f0 + f][c][i] = __builtin_fmaf(rest[f][i], 1.f / 2048.f, S[f0 + f][c][i]);
             } else {
 #pragma unroll
-              for (int f = 0; f < G; ++f) S[f0 + f][c] = mma_64b<T>(r[f], w[c][1], S[f0 + f][c]);
-              if constexpr (TERMS == 3) {
+              for (int u = 1; u < TERMS; ++u)
 #pragma unroll
-                for (int f = 0; f < G; ++f) S[f0 + f][c] = mma_64b<T>(r[f], w[c][2], S[f0 + f][c]);
-              }
+                for (int f = 0; f < G; ++f) S[f0 + f][c] = mma_64b<T>(r[f], w[c][u], S[f0 + f][c]);
             }
           }
         }
@@ -542,12 +532,6 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
     }
     t0 += C;
     stage ^= STAGES - 1;
-  };
-  if constexpr (HALF) {
-    while (t0 < left) chunk(Int<2>{});
-  } else {
-    while (t0 < late) chunk(Int<2>{});
-    while (t0 < left) chunk(Int<3>{});
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives the workgroup's use of LDS
   if constexpr (!STATE) {

@@ -1484,8 +1484,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: to
     what the sequences begin with, zeros where None: a prompt is one call, and its state the next call's, of a token or of
     many.  lengths (B,) int32: the tokens of each sequence (clamped to 0..L); what lies behind them is not used, its
     outputs are zeros and leave the state alone.  Any strides whose rows are contiguous and begin at multiples of 16
-    bytes.  The state and all sums are fp32; long prompts are matrix products of 16-bit operands that hold what is not
-    16-bit by itself, state and weights, as sums of two or three.  A value of v that is not finite reaches the outputs
+    bytes.  The state and all sums are fp32; more than 16 tokens are matrix products of 16-bit operands, which hold
+    what is not 16-bit by itself as sums of two or three: state and additions to it with all of their bits in bf16 and 22 in
+    fp16, the weights within 64 tokens with 16.  A value of v that is not finite reaches the outputs
     from its own token on.  `state_out` may be `state`, updated in place; otherwise outputs share no memory with inputs.
     Few heads of many tokens are computed in segments through scratch memory of torch's allocator, joined in a fixed
     order."""

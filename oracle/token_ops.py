@@ -161,11 +161,12 @@ def decay_attention(q, k, v, decay, state=None, lengths=None, scale=None):
     # up to |k| 2^-36, whatever its age (F; chunks' own decay is left out of it).  A term's decay after
     # m tokens is a product of powers, each off by its exponent's rounding (a logarithm off by a unit, a product: |ln g|
     # 2^-22 a token) and by a unit itself, one a chunk of 64 tokens and a few more.  Outputs take the weights Q K^T . D as
-    # sums of two values, 2^-18 of them in bf16 and 2^-23 in fp16, and the state whole in bf16, as a sum of two values in
-    # fp16; they have sums of dk and 64 terms.
+    # sums of two bf16 values on both types: the first is off by 2^-8 of the weight's power of two, so that the second lies
+    # below that and is off by 2^-8 of it and half, 2^-17 together; they take the state whole in bf16, as a sum of two
+    # values and off by 2^-22 in fp16.  They have sums of dk and 64 terms.
     each = torch.where(g > 0, -torch.log(g.clamp(min=1e-30)), 0.0) * 2.0**-22 + 2.0**-27 + 6 * U
     low = 2.0**-36 if q.dtype == torch.float16 else 0
-    two = 2.0**-17 if q.dtype == torch.bfloat16 else 2.0**-21
+    two = 2.0**-17 if q.dtype == torch.bfloat16 else 2.0**-17 + 2.0**-22
     n = torch.full((B,), L, device=q.device) if lengths is None else lengths.long().clamp(0, L)
     for t in range(int(n.max()) if B and L else 0):
         on = (t < n)[:, None, None, None]

@@ -28,7 +28,7 @@
 // rounded.)  In fp16 they are sums of two: 22 bits, S with a column scaled by a power of two to fp16's range; of W V the
 // second one is 2^11 times larger, so that a token adds at most |k| 2^-36 on top, where the decay has taken it below the
 // type's range.  The fp32 weights Q K^T . D, which only their own chunk sees, are sums of two bf16 values, 16 bits, on both
-// types, as they easily pass fp16's range, and fp16 values of V are sums of two of them, exactly.
+// types, as they easily pass fp16's range, and fp16 values of V are sums of two of them, exactly; all four products count.
 //
 // A value of V that is not finite must not reach the tokens before it, and 0 times it would: a chunk that holds one
 // takes it out and marks the outputs that it belongs to instead.
@@ -512,6 +512,10 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void dec
             for (int x = 2 * y; x < 4; ++x)
 #pragma unroll
               for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<__bf16>(second[c], hi[x], O[x][c]);
+#pragma unroll
+            for (int x = 2 * y; x < 4; ++x)
+#pragma unroll
+              for (int c = 0; c < NV; ++c) O[x][c] = mma_64b<__bf16>(second[c], lo[x], O[x][c]);
           }
         }
       }

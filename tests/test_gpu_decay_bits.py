@@ -50,3 +50,24 @@ def test_outputs_of_states_that_almost_cancel(dev, L, H, dk, dv):
     # output rounds by 2^-8 of itself at the most
     bound = big * (6 * 2 * U) + want.abs() * (2.0**-8 + 4 * U)
     assert ((o.double() - want[:, None]).abs() <= bound[:, None]).all()
+
+
+@pytest.mark.parametrize("L,H,dk,dv", [(64, 40, 16, 48), (50, 8, 64, 128), (30, 300, 32, 64)])
+@pytest.mark.parametrize("dtype", [torch.float16, BF16])
+def test_weights_within_a_chunk_that_almost_cancel(dev, L, H, dk, dv, dtype):
+    """Two tokens whose weighted values are alike but for their sign and last bits: every part of both counts."""
+    g = _gen(dev, L + H)
+    q, k, v = (torch.zeros(1, L, H, n, dtype=dtype, device=dev) for n in (dk, dk, dv))
+    a = 1 + torch.rand(H, generator=g, device=dev).to(dtype)
+    q[..., 2], q[..., dk - 1] = 1.0, a
+    k[:, 1, :, 2], k[:, 6, :, dk - 1] = 1.0, 1.0
+    v[:, 6] = _randn(g, 1, H, dv, dtype=dtype)
+    v[:, 1] = (-a.double()[:, None] * v[:, 6].double()).to(dtype)
+    o, _ = ops.decay_attention(q, k, v, torch.ones(H, device=dev), scale=1024.0)
+    size = (a.double()[:, None] * v[:, 6].double()).abs() * 1024
+    want = (v[:, 1].double() + a.double()[:, None] * v[:, 6].double()) * 1024
+    # the weights, 1 and a, have 11 bits at the most: their parts are exact, as are those of the values; up to eight products
+    # of parts are added in 24 bits, each sum off by 2 U of up to twice the size; an output rounds by half a step
+    step = torch.finfo(dtype).eps / 2
+    bound = size * (8 * 2 * 2 * U) + want.abs() * (step + 4 * U) + torch.finfo(dtype).smallest_normal * step
+    assert ((o[:, 6:].double() - want[:, None]).abs() <= bound[:, None]).all()

@@ -64,15 +64,16 @@ constexpr int kDecayColumns = 128;  // most columns of V of a workgroup
 // Columns of V of a workgroup, in 16s; how many of them a wave has, and the waves a SIMD that its registers are limited to.
 // Measured, us: 64 columns, 64 heads of 64 over 12544 tokens, bf16: a wave 16 columns and two waves a SIMD 151, three 166, 32
 // columns 187; 48 columns of fp16: three 154, two 165; 128 columns, 16 heads of 128 over 65536 tokens: a wave 32 columns 394,
-// 16 columns 487.
+// 16 columns 487; the same in fp16, where 32 columns keep 38 registers in memory, 475 and 506.  Keys of more than 64 values do
+// not fit three waves a SIMD: 4 x 6000 tokens, 16 heads of 128 x 48, fp16 three 213, two 123 (bf16 156, 120), 128 x 32 108, 104.
 __host__ __device__ constexpr int decay_blocks(int dv) { return dv <= 32 ? 2 : dv <= 48 ? 3 : dv <= 64 ? 4 : 8; }
 __host__ __device__ constexpr int decay_own(int blocks) { return blocks == 8 ? 2 : 1; }
-__host__ __device__ constexpr int decay_waves(int blocks) { return blocks < 4 ? 3 : 2; }
+__host__ __device__ constexpr int decay_waves(int dk, int blocks) { return blocks < 4 && dk <= 64 ? 3 : 2; }
 
 // Workgroups that a CU holds.
 inline int decay_resident(int dk, int dv) {
   const int blocks = decay_blocks(dv), pk = dk <= 32 ? 4 : dk <= 64 ? 8 : 16, pv = blocks == 3 ? 8 : blocks * 2;
-  const int by_lds = 160 / (2 * pk + pv + 12 + 1), by_waves = 4 * decay_waves(blocks) / (blocks / decay_own(blocks));
+  const int by_lds = 160 / (2 * pk + pv + 12 + 1), by_waves = 4 * decay_waves(dk, blocks) / (blocks / decay_own(blocks));
   return by_lds < by_waves ? by_lds : by_waves;
 }
 
@@ -167,7 +168,7 @@ __device__ __forceinline__ int decay_operand(int x, int y) { return x < 2 ? x : 
 // DKP: dk rounded up to 32, 64 or 128; NW waves of 16 NV columns.  STATE: a segment's state from a state of zeros,
 // without outputs.
 template <class T, int DKP, int NV, int NW, bool STATE>
-__global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(NV * NW)) void decay_chunk_kernel(DecayParams p) {
+__global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(DKP, NV * NW)) void decay_chunk_kernel(DecayParams p) {
   constexpr bool HALF = __is_same(T, _Float16);
   constexpr int C = kDecayChunk, STAGES = STATE ? 2 : 1;
   constexpr int TERMS = HALF ? 2 : 3;  // values of T that the state's products take for one of it

@@ -963,6 +963,18 @@ def _layout(t):
     return None if t is None else (t.dtype, t.shape, t.stride(), t.device)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", lambda: 0)  # absent in CPU-only builds
+
+
+def _launch(entry, device: torch.device, what: str, *args):
+    """Calls an entry with its device as the current one: the default stream's handle is the same for every device."""
+    if device.index == _current_device():
+        check(entry(*args, _stream(device)), what)
+    else:
+        with torch.cuda.device(device):
+            check(entry(*args, _stream(device)), what)
+
+
 def _rms_norm_plan(key, x, weight, residual, eps, out_dtype, out, stream_out, scale):
     """(descriptor, output's type, whether that is e4m3, rows' shape, device, whether x is dense) of a checked call."""
     _token_input(x, "x")
@@ -1034,8 +1046,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
         stream_out = torch.empty_like(x) if dense else torch.empty(shape, dtype=x.dtype, device=dev)
     if eight and scale is None:
         scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
-    check(_lib.load().sengine_amd_rms_norm(desc, x.data_ptr(), _ptr(residual), _ptr(weight), out.data_ptr(),
-                                           _ptr(stream_out), _ptr(scale), _stream(dev)), "rms_norm")
+    _launch(_lib.load().sengine_amd_rms_norm, dev, "rms_norm", desc, x.data_ptr(), _ptr(residual), _ptr(weight),
+            out.data_ptr(), _ptr(stream_out), _ptr(scale))
     return (out, stream_out, scale) if eight else (out, stream_out)
 
 
@@ -1121,9 +1133,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     if out is None:
         out = torch.empty(shape, dtype=out_dtype, device=dev)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    check(_lib.load().sengine_amd_linear_ws(
-        desc, x.data_ptr(), weight.data_ptr(), _ptr(x_scale), _ptr(weight_scale), _ptr(bias), _ptr(residual),
-        out.data_ptr(), _ptr(ws), size, _stream(dev)), "linear")
+    _launch(_lib.load().sengine_amd_linear_ws, dev, "linear", desc, x.data_ptr(), weight.data_ptr(), _ptr(x_scale),
+            _ptr(weight_scale), _ptr(bias), _ptr(residual), out.data_ptr(), _ptr(ws), size)
     return out
 
 
@@ -1213,21 +1224,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Op
             if p & 15 and t.numel():
                 raise SEngineError(f"{name}: must begin at a multiple of 16 bytes")
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    check(_lib.load().sengine_amd_cross_attention_ws(
-        desc, qp, kp, vp, _ptr(key_lengths), _ptr(key_mask), op, _ptr(ws), size, _stream(dev)), "cross_attention")
+    _launch(_lib.load().sengine_amd_cross_attention_ws, dev, "cross_attention", desc, qp, kp, vp, _ptr(key_lengths),
+            _ptr(key_mask), op, _ptr(ws), size)
     return out
-
-
-_current_device = getattr(torch._C, "_cuda_getDevice", lambda: 0)  # absent in CPU-only builds
-
-
-def _launch(entry, device: torch.device, what: str, *args):
-    """Calls an entry with its device as the current one: the default stream's handle is the same for every device."""
-    if device.index == _current_device():
-        check(entry(*args, _stream(device)), what)
-    else:
-        with torch.cuda.device(device):
-            check(entry(*args, _stream(device)), what)
 
 
 def _heads_out(t, shape, dtype, name: str, device):

@@ -200,10 +200,8 @@ extern "C" int sengine_amd_cross_attention_ws(const sengine_cross_desc* d, const
   if (!rows_fit(d)) return set_error(-2, "cross_attention: too many query rows");
   if (d->B == 0 || d->Lq == 0) return 0;
   if (!q || !out || (d->Lk > 0 && (!k || !v))) return set_error(-1, "cross_attention: null q, k, v or out");
-  // rows less than d elements apart: among them the same memory for several sequences, queries or heads
-  const auto apart = [&](int32_t n, int64_t s) { return n == 1 || s >= d->d || s <= -d->d; };
-  if (!apart(d->B, d->out_stride[0]) || !apart(d->Lq, d->out_stride[1]) || !apart(d->Hq, d->out_stride[2]))
-    return set_error(-2, "cross_attention: output rows overlap");
+  const int32_t rows_of[3] = {d->B, d->Lq, d->Hq};
+  if (!rows_apart(d->d, 3, rows_of, d->out_stride)) return set_error(-2, "cross_attention: output rows overlap");
   CrossParams p{};
   p.q = q;
   p.k = k;

@@ -272,12 +272,11 @@ extern "C" int sengine_amd_decay_attention_ws(const sengine_decay_desc* d, const
   if (d->B == 0) return 0;
   if (!decay || (d->L > 0 && (!q || !k || !v || !out)))
     return set_error(-1, "decay_attention: null q, k, v, decay or out");
-  const auto apart = [](int32_t n, int64_t s, int64_t size) { return n == 1 || s >= size || s <= -size; };
-  if (d->L > 0 && (!apart(d->B, d->out_stride[0], d->dv) || !apart(d->L, d->out_stride[1], d->dv) ||
-                   !apart(d->H, d->out_stride[2], d->dv)))
+  const int32_t rows_of[3] = {d->B, d->L, d->H}, states_of[2] = {d->B, d->H};
+  if (d->L > 0 && !rows_apart(d->dv, 3, rows_of, d->out_stride))
     return set_error(-2, "decay_attention: output rows overlap");
   const int64_t matrix = (int64_t)d->dk * d->dv;
-  if (state_out && (!apart(d->B, d->state_out_stride[0], matrix) || !apart(d->H, d->state_out_stride[1], matrix)))
+  if (state_out && !rows_apart(matrix, 2, states_of, d->state_out_stride))
     return set_error(-2, "decay_attention: output states overlap");
   const auto rows = [&](const void* a, const int64_t* s) {
     return (uintptr_t)a % 16 == 0 && (d->B == 1 || s[0] % 8 == 0) && (d->L == 1 || s[1] % 8 == 0) &&

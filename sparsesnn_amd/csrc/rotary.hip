@@ -195,10 +195,9 @@ extern "C" int sengine_amd_rotary(const sengine_rotary_desc* d, const void* q, c
   if (d->B == 0 || d->L == 0) return 0;
   if (!q || !out_q || !positions || !frequencies || (d->Hk > 0 && (!k || !out_k)))
     return set_error(-1, "rotary: null q, k, positions, frequencies or output");
-  const auto apart = [&](int32_t n, int64_t s) { return n == 1 || s >= d->d || s <= -d->d; };
   for (int w = 0; w < (d->Hk ? 2 : 1); ++w) {
-    const int64_t* s = w ? d->out_k_stride : d->out_q_stride;
-    if (!apart(d->B, s[0]) || !apart(d->L, s[1]) || !apart(w ? d->Hk : d->Hq, s[2]))
+    const int32_t n[3] = {d->B, d->L, w ? d->Hk : d->Hq};
+    if (!rows_apart(d->d, 3, n, w ? d->out_k_stride : d->out_q_stride))
       return set_error(-2, "rotary: output rows overlap");
   }
   RotaryParams p{};

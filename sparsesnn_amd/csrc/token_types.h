@@ -52,6 +52,26 @@ inline int type_bytes(int code) {
 // Whether one launch can have so many workgroups: its threads count to 2^32 - 1.
 inline bool launchable(int64_t wgs, int threads) { return wgs <= 0xffffffffll / threads; }
 
+// Whether the rows of `size` elements of a tensor of up to three dimensions share no memory: those of every dimension lie
+// outside of what the dimensions with smaller strides span.
+inline bool rows_apart(int64_t size, int dims, const int32_t* n, const int64_t* stride) {
+  __int128 span = size;
+  bool taken[3] = {false, false, false};
+  for (int i = 0; i < dims; ++i) {
+    int next = -1;  // the smallest stride left
+    __int128 least = 0;
+    for (int j = 0; j < dims; ++j) {
+      const __int128 s = stride[j] < 0 ? -(__int128)stride[j] : (__int128)stride[j];
+      if (!taken[j] && n[j] > 1 && (next < 0 || s < least)) next = j, least = s;
+    }
+    if (next < 0) break;
+    if (least < span) return false;
+    taken[next] = true;
+    span += (n[next] - 1) * least;
+  }
+  return true;
+}
+
 // One element of a run-time type (a vector of coefficients read once per column).
 __device__ __forceinline__ float load_as_float(const void* p, int code, int64_t i) {
   if (code == SENGINE_ENC_F32) return static_cast<const float*>(p)[i];

@@ -195,6 +195,8 @@ extern "C" int sengine_amd_rotary(const sengine_rotary_desc* d, const void* q, c
   if (d->B == 0 || d->L == 0) return 0;
   if (!q || !out_q || !positions || !frequencies || (d->Hk > 0 && (!k || !out_k)))
     return set_error(-1, "rotary: null q, k, positions, frequencies or output");
+  // more tokens than a launch has workgroups for, in whatever pieces
+  if (!launchable(((int64_t)d->B * d->L + kRotTokens - 1) / kRotTokens, 256)) return (int)hipErrorInvalidConfiguration;
   for (int w = 0; w < (d->Hk ? 2 : 1); ++w) {
     const int32_t n[3] = {d->B, d->L, w ? d->Hk : d->Hq};
     if (!rows_apart(d->d, 3, n, w ? d->out_k_stride : d->out_q_stride))

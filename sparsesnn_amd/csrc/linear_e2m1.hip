@@ -15,22 +15,35 @@ struct E2m1Params {
   int groups;            // scales of a row
 };
 
-// Eight codes of a dword as T.
+// Eight codes of a dword as T, times a power of two.
 template <class T>
-__device__ __forceinline__ u32x4_t widen_e2m1(uint32_t v) {
+__device__ __forceinline__ u32x4_t widen_e2m1(uint32_t v, float power) {
   u32x4_t r;
   if constexpr (__is_same(T, _Float16)) {
-    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, 1.f, 0));
-    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, 1.f, 1));
-    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, 1.f, 2));
-    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, 1.f, 3));
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, power, 0));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, power, 1));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, power, 2));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, power, 3));
   } else {
-    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.f, 0));
-    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.f, 1));
-    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.f, 2));
-    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.f, 3));
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, power, 0));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, power, 1));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, power, 2));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, power, 3));
   }
   return r;
+}
+
+// A group's scale s as power * rest, |rest| in 1..2.  bf16 codes take the power along: a bf16 value times a code alone may
+// pass the range where it times code and scale does not.  fp16 values have no such products, and a power of 1.  (s = 0 and
+// NaN: rest is 0 and NaN.)  8 x 8192 x 8192 takes 14.6 us with it, 14.4 without.
+template <class T>
+__device__ __forceinline__ void split_scale(float s, float& power, float& rest) {
+  power = 1.f, rest = s;
+  if constexpr (__is_same(T, __bf16)) {
+    const uint32_t e = __builtin_bit_cast(uint32_t, s) & 0x7f800000u;
+    power = __builtin_bit_cast(float, e);
+    rest = s * __builtin_bit_cast(float, (254u << 23) - e);
+  }
 }
 
 // Four dwords a lane, lane group g (of 16) with dwords 4 g .. 4 g + 3 of a row's 16: afterwards with dwords g, 4 + g,
@@ -127,19 +140,21 @@ __global__ __launch_bounds__(64 * W, NT == 2 ? 2 : 3) void linear_e2m1_kernel(E2
                         __builtin_amdgcn_cvt_f32_fp8(scales, 2), __builtin_amdgcn_cvt_f32_fp8(scales, 3)};
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
+      float power, rest;
+      split_scale<T>(s[n], power, rest);
       float4_t sum[MT];
 #pragma unroll
       for (int t = 0; t < MT; ++t) sum[t] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int m = n * G; m < (n + 1) * G; ++m) {
-        const u32x4_t b = widen_e2m1<T>(w[m]);
+        const u32x4_t b = widen_e2m1<T>(w[m], power);
 #pragma unroll
         for (int t = 0; t < MT; ++t) sum[t] = mma_64b<T>(x[t][m], b, sum[t]);
       }
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][i][e] = __builtin_fmaf(sum[t][e], s[n], acc[t][i][e]);
+        for (int e = 0; e < 4; ++e) acc[t][i][e] = __builtin_fmaf(sum[t][e], rest, acc[t][i][e]);
     }
   };
   // Codes and scales are on their way U to 2 U segments ahead of their use, x, which the caches hold, up to one.
@@ -225,7 +240,7 @@ __global__ __launch_bounds__(256) void widen_e2m1_kernel(E2m1Params p, T* out, i
   }
   const float s = __builtin_amdgcn_cvt_f32_fp8((uint32_t)p.scale[n * p.scale_stride + (k >> shift)], 0);
   typedef T vec_t __attribute__((ext_vector_type(8)));
-  vec_t v = __builtin_bit_cast(vec_t, widen_e2m1<T>(codes));
+  vec_t v = __builtin_bit_cast(vec_t, widen_e2m1<T>(codes, 1.f));
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = (T)((float)v[e] * s);
   *reinterpret_cast<vec_t*>(out + n * width + k) = v;

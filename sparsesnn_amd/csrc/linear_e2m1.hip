@@ -249,8 +249,15 @@ __global__ __launch_bounds__(256) void widen_e2m1_kernel(E2m1Params p, T* out, i
 // Whether a call with scratch memory widens the weight there and multiplies it as a 16-bit one: where the kernel above would
 // take more than a round of 32 columns and 64 token rows a CU.  Measured (bf16, us; widened and not): 128 x 8192 x 8192 64 and
 // 76, 256 x 4096 x 4096 32 and 41, 4000 x 384 x 384 14 and 18; 128 x 4096 x 4096 30 and 22, 1000 x 384 x 384 14 and 10; 70 x
-// 8192 x 8192 62 and 59.
-static bool widens(int64_t M, int64_t N) { return M > 64 && (N + 31) / 32 * ((M + 63) / 64) > 256; }
+// 8192 x 8192 56 to 60 and 56.  Rows of x that are no whole pieces of 16 bytes (or lie backwards or far apart) keep linear's
+// tiles off, and the weight's way through memory pays from three times 64 rows on: 70 x 8192 x 8190 134 and 98, 128 rows 133
+// and 117 (of 8192 values 8196 apart 125 and 56, 8199 apart 127 and 148), 256 rows 142 and 230, 256 x 4096 x 4094 68 and 69,
+// 4000 x 384 x 390 18 and 31.
+static bool widens(const LinearParams& p) {
+  const bool whole = ((uintptr_t)p.x | (uintptr_t)p.kbytes | (uintptr_t)p.x_stride) % 16 == 0 && p.x_stride >= 0 &&
+                     p.x_stride < 1 << 22;
+  return p.M > (whole ? 64 : 128) && ((int64_t)p.N + 31) / 32 * ((p.M + 63) / 64) > 256;
+}
 
 static LinearParams widened(const E2m1Params& p, const void* weight) {
   LinearParams q = p.lin;
@@ -285,7 +292,7 @@ static hipError_t by_rows(const E2m1Params& p, hipStream_t stream) {
 
 template <class T>
 static hipError_t run(const E2m1Params& p, int group, uint8_t* workspace, size_t bytes, hipStream_t stream) {
-  if (widens(p.lin.M, p.lin.N) && p.lin.K > 0 && workspace && bytes >= widened_bytes(p.lin)) {
+  if (widens(p.lin) && p.lin.K > 0 && workspace && bytes >= widened_bytes(p.lin)) {
     const int width = (p.lin.K + 7) / 8 * 8;
     const int64_t wgs = ((int64_t)p.lin.N * (width / 8) + 255) / 256;
     if (!launchable(wgs, 256)) return hipErrorInvalidConfiguration;
@@ -375,13 +382,13 @@ extern "C" int sengine_amd_linear_e2m1(const sengine_linear_e2m1_desc* d, const 
 extern "C" int sengine_amd_linear_e2m1_workspace(const sengine_linear_e2m1_desc* d, size_t* bytes) {
   if (!d || !bytes) return set_error(-1, "linear_e2m1_workspace: null argument");
   *bytes = 0;
-  if (d->N < 1 || d->K < 1 || !sizes_fit(d) || !widens(d->M, d->N)) return 0;  // no need, or refused by the entry
-  E2m1Params p{};
+  if (d->N < 1 || d->K < 1 || !sizes_fit(d)) return 0;  // refused by the entry, or no weight
+  E2m1Params p{};  // x unknown: taken to begin at a multiple of 16 bytes
   p.lin.M = d->M;
   p.lin.N = d->N;
   p.lin.K = d->K;
   p.lin.kbytes = d->K * 2;
   p.lin.x_stride = d->x_stride * 2;
-  *bytes = widened_bytes(p.lin) + linear_scaled_workspace(widened(p, nullptr));
+  if (widens(p.lin)) *bytes = widened_bytes(p.lin) + linear_scaled_workspace(widened(p, nullptr));
   return 0;
 }

@@ -88,13 +88,13 @@ def e2m1_groups(w: torch.Tensor, group: int = 32):
     N, K = w.shape
     groups = -(-K // group)
     w = w.detach().float()
-    row = w.abs().amax(-1) / (E2M1_MAX * E4M3_MAX) if K else torch.zeros(N, device=w.device)
+    row = w.abs().amax(-1) / (E2M1_MAX * E4M3_MAX) if K else w.new_zeros(N)
     row = torch.where(row > 0, row, torch.ones_like(row))
     v = torch.nn.functional.pad(w / row[:, None], (0, groups * group - K)).view(N, groups, group)
     scale = (v.abs().amax(-1) / E2M1_MAX).clamp(max=E4M3_MAX).to(torch.float8_e4m3fn)
     s = scale.float()[:, :, None]
     v = (v / torch.where(s > 0, s, torch.ones_like(s))).view(N, groups * group)[:, :K]
-    codes = torch.bucketize(v.abs(), torch.tensor(E2M1_MIDDLES, device=w.device))
+    codes = torch.bucketize(v.abs(), w.new_tensor(E2M1_MIDDLES))
     codes = (codes + 8 * (v < 0)).to(torch.uint8)
     return codes[:, ::2] | codes[:, 1::2] << 4, scale, row
 
@@ -160,7 +160,8 @@ class TokenReader:
         """The mixers' states of B sequences without a token: a list for `read`, which updates them in place."""
         d = self.embed // self.heads
         dev = self.p["norm.weight"].device
-        return [None if g is None else torch.zeros((B, self.heads, d, d), device=dev) for g in self.decay]
+        return [None if g is None else torch.zeros((B, self.heads, d, d), dtype=torch.float32, device=dev)
+                for g in self.decay]
 
     def encode(self, tokens: torch.Tensor, positions: Optional[torch.Tensor] = None):
         """Every block's (keys, values) of the tokens (B, N, C): each (B, N, heads, C / heads).  positions, as

@@ -1308,7 +1308,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if type(sections) is not tuple:
         sections = tuple(sections)
     key = None
-    if out_q is None and out_k is None:
+    # 8.0 and True would find the calls of 8 and 1
+    if out_q is None and out_k is None and {*map(type, sections)} == {int}:
         try:
             key = ("rotary", q.dtype, q.shape, q.stride(), q.device, _layout(k), positions.dtype, positions.shape,
                    positions.stride(), positions.device, frequencies.dtype, frequencies.shape, frequencies.stride(),

@@ -134,7 +134,7 @@ __device__ __forceinline__ auto decay_term(float (&x)[N]) {
 // A power of two that brings values up to `most` (its bits, the sign cleared) to fp16's upper range, and its inverse.
 __device__ __forceinline__ void decay_range(uint32_t most, float& up, float& down) {
   int e = (int)(most >> 23);
-  e = e < 81 ? 81 : e > 250 ? 250 : e;
+  e = e < 15 ? 15 : e;  // both stay normal values
   up = __builtin_bit_cast(float, (uint32_t)(268 - e) << 23);
   down = __builtin_bit_cast(float, (uint32_t)(e - 14) << 23);
 }

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(DKP, NV * NW)) voi
   __shared__ __attribute__((aligned(1024))) uint8_t smem[STAGES * kStage + (STATE ? 0 : 2 * kP)];
   __shared__ float powers[16 + C + 1], behind[2 * C];  // scale g^(n - 16), zeros up to there; g^(C - 1 - j), zeros behind
   const int tid = (int)threadIdx.x, lane = tid & 63;
-  const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, a = lane & 15;
   // neighbouring heads of a segment on one XCD: where their rows share cache lines they are fetched once
   const int segs = STATE ? p.segs - 1 : p.segs;
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(DKP, NV * NW)) voi
   const auto transposed = [&](int at, int pitch) { return read_transposed(smem + at, smem + at + 16 * pitch); };
   const auto meet = [&]() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if constexpr (NW > 1) __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
 
@@ -475,8 +475,8 @@ __global__ __launch_bounds__(64 * NW, STATE ? 4 : decay_waves(DKP, NV * NW)) voi
         }
       }
     }
-    if (STAGES == 1 || !STATE) meet();  // the blocks are written, and K, V and Q have been read
-    if (STAGES == 1 && t0 + C < left) copy(t0 + C, 0);
+    if constexpr (!STATE) meet();  // the blocks are written, and K, V and Q have been read
+    if (!STATE && t0 + C < left) copy(t0 + C, 0);
     if constexpr (!STATE) {
       if (used) {  // (Q K^T . D) V
 #pragma unroll

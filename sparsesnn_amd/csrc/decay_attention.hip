@@ -159,8 +159,8 @@ __global__ __launch_bounds__(256) void decay_scan_kernel(DecayParams p, int per_
 }
 
 // Whether wide heads take waves of 16 columns, not of 32: where every workgroup has a CU to itself.  Measured, us, waves of 16
-// and of 32: 16 heads of 128 x 128 in bf16, 300 tokens 29 and 37, 1000 tokens 34 and 39; two workgroups a CU, 6 x 12 heads of
-// 64 x 80 over 777 tokens, 35.5 and 31.5.
+// and of 32: 16 heads of 128 x 128 in bf16, 300 tokens 25 and 29, 1000 tokens 35 and 39; two workgroups a CU, 6 x 12 heads of
+// 64 x 80 over 777 tokens, 36 and 31.
 static bool decay_narrow(int dv, int64_t workgroups) { return decay_own(decay_blocks(dv)) > 1 && workgroups <= 256; }
 
 struct DecayPlan {
@@ -168,8 +168,8 @@ struct DecayPlan {
   int segs, seg_len;  // segments of a sequence that are computed beside each other, tokens of one
 };
 
-// Most tokens that go one by one.  Measured, us, one by one and as a chunk: 64 x 32 heads of 128 x 128, 16 tokens 78 and 87, 32
-// tokens 127 and 97; 16 heads of 128 x 128, 16 tokens 11 and 16, 32 tokens 18 and 16.
+// Most tokens that go one by one.  Measured, us, one by one and as a chunk: 64 x 32 heads of 128 x 128, 16 tokens 80 and 91, 32
+// tokens 128 and 101; 16 heads of 128 x 128, 16 tokens 11 and 12, 32 tokens 18 and 12.
 constexpr int kDecaySteps = 16;
 
 static DecayPlan plan(const sengine_decay_desc* d) {
@@ -182,8 +182,11 @@ static DecayPlan plan(const sengine_decay_desc* d) {
   const int chunks = (int)(((int64_t)d->L + kDecayChunk - 1) / kDecayChunk);
   // Rounds of workgroups over the chip, times the chunks of one and a start, half as much again for the pass that makes the
   // segments' states; and two launches more and the states' joining, in the time of chunks, of which narrow waves have
-  // two thirds.  Measured, us, without segments and in this many: 16 heads of 128 x 128, 150 tokens 21, 300 tokens 29 and
-  // 25 (5); 4000 tokens 47 (16), 51 (32), 79 (63); 8 x 16 heads of them over 500 tokens 46, 54 (4).
+  // two thirds.  Measured, us, without segments and in this many: 16 heads of 128 x 128, 150 tokens 22, 300 tokens 32 and
+  // 25 (5); 4000 tokens 49 (16), 53 (32), 80 (63); 8 x 16 heads of them over 500 tokens 50, 54 (4).  Narrow heads, bf16: 8
+  // heads of 16 x 16, 150 tokens 12, 193 tokens 15 and 13 (4), 300 tokens 17 and 13 (5); 4 x 8 heads of 48 x 48, 150 tokens 15,
+  // 193 tokens 18 and 17 (4), 300 tokens 21 and 17 (5); 4 x 16 heads of 64 x 64, where four segments are two rounds, 193 tokens
+  // 17 and 18, 400 tokens 25 and 23 (7).
   const int64_t heads = (int64_t)d->B * d->H * ((d->dv + kDecayColumns - 1) / kDecayColumns);
   const int64_t slots = 256 * decay_resident(d->dk, d->dv);
   const auto pass = [&](int64_t workgroups, int per) {

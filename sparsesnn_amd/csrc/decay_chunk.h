@@ -10,9 +10,9 @@
 // Few heads: a first pass makes each segment's state from a state of zeros (K and V only, copies one chunk ahead), and
 // decay_scan_kernel joins them, so that K and V are read twice.
 //
-// Measured: 16 heads of 128 x 128 over 65536 tokens, bf16, in 32 segments: 120 us (4.5 TB/s), 12 and 275 (3.9 TB/s; matrix
-// cores 30 %, vector unit 35 %, waves waiting 35 %).  64 heads of 48 x 48 over 12544 tokens, fp16, in 16 segments: 45, 6 and 108
-// (2.8 TB/s; 11 %, 30 %, 42 %: a chunk's products, splits and reads follow each other in a wave, and LDS and registers leave
+// Measured: 16 heads of 128 x 128 over 65536 tokens, bf16, in 32 segments: 122 us (4.4 TB/s), 12 and 312 (3.4 TB/s; matrix
+// cores 38 %, vector unit 40 %, waves waiting 31 %).  64 heads of 48 x 48 over 12544 tokens, fp16, in 16 segments: 45, 6 and 107
+// (2.9 TB/s; 12 %, 30 %, 40 %: a chunk's products, splits and reads follow each other in a wave, and LDS and registers leave
 // three waves a SIMD).
 //
 // All products are 16x16x32 matrix instructions, laid out so that what one leaves is what the next one takes:
@@ -23,9 +23,8 @@
 //
 // Rounding.  S is fp32.  What a 16-bit instruction takes of it, and W V, which makes it, are in bf16 sums of three values,
 // which have all of its 24 bits whatever the age of a token: later keys may be small or zero, so that an early token is all
-// that a state holds, and outputs may be differences of its values.  (Two instead of three: 400 us for 431 at 65536 tokens of
-// 16 heads of 128 x 128, 76.8 for 79.7 at 8 x 1000; outputs 1.1e-4 for 5.5e-5 of the exact ones' size from those,
-// rounded.)  In fp16 they are sums of two: 22 bits, S with a column scaled by a power of two to fp16's range; of W V the
+// that a state holds, and outputs may be differences of its values.  (Two instead of three: 400 us for 424 at 65536 tokens of
+// 16 heads of 128 x 128, 77 for 79 at 8 x 1000; outputs 1.1e-4 for 5.5e-5 of the exact ones' size from those, rounded.)  In fp16 they are sums of two: 22 bits, S with a column scaled by a power of two to fp16's range; of W V the
 // second one is 2^11 times larger, so that a token adds at most |k| 2^-36 on top, where the decay has taken it below the
 // type's range.  The fp32 weights Q K^T . D, which only their own chunk sees, are sums of two bf16 values, 16 bits, on both
 // types, as they easily pass fp16's range, and fp16 values of V are sums of two of them, exactly; all four products count.
@@ -62,9 +61,9 @@ constexpr int kDecayChunk = 64;
 constexpr int kDecayColumns = 128;  // most columns of V of a workgroup
 
 // Columns of V of a workgroup, in 16s; how many of them a wave has, and the waves a SIMD that its registers are limited to.
-// Measured, us: 64 columns, 64 heads of 64 over 12544 tokens, bf16: a wave 16 columns and two waves a SIMD 151, three 166, 32
-// columns 187; 48 columns of fp16: three 154, two 165; 128 columns, 16 heads of 128 over 65536 tokens: a wave 32 columns 394,
-// 16 columns 487; the same in fp16, where 32 columns keep 38 registers in memory, 475 and 506.  Keys of more than 64 values do
+// Measured, us: 64 columns, 64 heads of 64 over 12544 tokens, bf16: a wave 16 columns and two waves a SIMD 157, three 168, 32
+// columns 189; 48 columns of fp16: three 155, two 166; 128 columns, 16 heads of 128 over 65536 tokens: a wave 32 columns 438,
+// 16 columns 523; the same in fp16, where 32 columns keep 38 registers in memory, 472 and 518.  Keys of more than 64 values do
 // not fit three waves a SIMD: 4 x 6000 tokens, 16 heads of 128 x 48, fp16 three 213, two 123 (bf16 156, 120), 128 x 32 108, 104.
 __host__ __device__ constexpr int decay_blocks(int dv) { return dv <= 32 ? 2 : dv <= 48 ? 3 : dv <= 64 ? 4 : 8; }
 __host__ __device__ constexpr int decay_own(int blocks) { return blocks == 8 ? 2 : 1; }

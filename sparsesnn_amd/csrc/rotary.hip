@@ -7,12 +7,12 @@
 //
 // Bandwidth bound: queries and keys are read and written once, in one launch.  32768 tokens x 40 heads x 128 bf16, neighbouring
 // pairs: 118 us (5.7 TB/s; two items a thread in flight 123), pairs P apart 126 (one item 129).  8 x 12544 tokens x 16 heads x
-// 48 fp16, pairs P apart: 64 us (4.8 TB/s; two half lines an access), neighbouring 53; workgroups of twice the tokens 69, of
-// four times 76.  A single token: 3.2 us.
+// 48 fp16, pairs P apart: 64 to 69 us (4.5 to 4.8 TB/s; two half lines an access), neighbouring 53; workgroups of twice the
+// tokens 69 for 64, of four times 76.  The same in fp32 133 and 115 us (4.6, 5.4 TB/s).  A single token: 3.2 us.
 //
 // A workgroup takes a few tokens: their sines and cosines, which all heads share, go to LDS; then its threads go through
 // the tokens' pieces of VEC values in the order in which they lie in memory.  With a head or two the angles are the time: 62 x
-// 8930 tokens of two heads x 32 fp16, 16 pairs, 43 us of the 28 that the bytes take.
+// 8930 tokens of two heads x 32 fp16, 16 pairs, 44 us of the 28 that the bytes take.
 #include "token_types.h"
 
 namespace sengine {

@@ -24,10 +24,11 @@
 // Rounding.  S is fp32.  What a 16-bit instruction takes of it, and W V, which makes it, are in bf16 sums of three values,
 // which have all of its 24 bits whatever the age of a token: later keys may be small or zero, so that an early token is all
 // that a state holds, and outputs may be differences of its values.  (Two instead of three: 400 us for 424 at 65536 tokens of
-// 16 heads of 128 x 128, 77 for 79 at 8 x 1000; outputs 1.1e-4 for 5.5e-5 of the exact ones' size from those, rounded.)  In fp16 they are sums of two: 22 bits, S with a column scaled by a power of two to fp16's range; of W V the
-// second one is 2^11 times larger, so that a token adds at most |k| 2^-36 on top, where the decay has taken it below the
-// type's range.  The fp32 weights Q K^T . D, which only their own chunk sees, are sums of two bf16 values, 16 bits, on both
-// types, as they easily pass fp16's range, and fp16 values of V are sums of two of them, exactly; all four products count.
+// 16 heads of 128 x 128, 77 for 79 at 8 x 1000; outputs 1.1e-4 for 5.5e-5 of the exact ones' size from those, rounded.)
+// In fp16 they are sums of two: 22 bits, S with a column scaled by a power of two to fp16's range; of W V the second one is
+// 2^11 times larger, so that a token is off by at most |k| 2^-36 on top, where the decay has taken it below the type's range.
+// The fp32 weights Q K^T . D, which only their own chunk sees, are sums of two bf16 values, 16 bits, on both types, as they
+// easily pass fp16's range, and fp16 values of V are sums of two of them, exactly; all four products count.
 //
 // A value of V that is not finite must not reach the tokens before it, and 0 times it would: a chunk that holds one
 // takes it out and marks the outputs that it belongs to instead.
